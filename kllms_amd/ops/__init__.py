@@ -102,7 +102,11 @@ def store_kv(
     v_scale: Optional[torch.Tensor] = None,
 ) -> None:
     """k_scale/v_scale: [NB, KVH, BS] fp32 per-row dequant scales, REQUIRED
-    when the caches are fp8 (written here: s = amax(|row|)/448), None for bf16."""
+    when the caches are fp8 (written here: s = amax(|row|)/448), None for bf16.
+    4-bit caches are uint8 [NB, KVH, BS, D / 2] with scales bf16 [NB, KVH, BS, D / 64, 2],
+    the steps and least values of groups of 64 values (torch_ref.kv4_quantize), written here too.
+    Slots that are read later have to differ: two rows of one slot leave a mixture of both."""
+    _check_kv4(k_cache, k_scale, v_scale)
     if k.is_cuda and not _force_torch():
         none = _none(k, torch.float32)
         _hip_or_raise().store_kv(
@@ -113,8 +117,25 @@ def store_kv(
     torch_ref.store_kv(k, v, k_cache, v_cache, slot_mapping, k_scale, v_scale)
 
 
+def _check_kv4(k_cache, k_scale, v_scale) -> None:
+    if k_cache.dtype == torch.uint8 and (k_scale is None or v_scale is None):
+        raise ValueError("a 4-bit cache needs k_scale and v_scale, the steps and least values of its groups")
+
+
+def load_kv(k_cache, v_cache, slots, k_scale, v_scale) -> Tuple[torch.Tensor, torch.Tensor]:
+    """What the 4-bit caches' rows at flat slots stand for, rounded to bf16: (k, v) [T, KVH, D], the inverse of
+    store_kv. Rows of slots outside the cache are NaN."""
+    _check_kv4(k_cache, k_scale, v_scale)
+    if k_cache.dtype != torch.uint8:
+        raise ValueError(f"load_kv reads 4-bit caches (uint8): got {k_cache.dtype}")
+    if k_cache.is_cuda and not _force_torch():
+        return _hip_or_raise().load_kv4(k_cache, v_cache, slots, k_scale, v_scale)
+    return torch_ref.load_kv(k_cache, v_cache, slots, k_scale, v_scale)
+
+
 def rope_store(q, k, v, positions, cos_sin, k_cache, v_cache, slot_mapping, k_scale=None, v_scale=None) -> None:
     """rope_inplace(q, k) and store_kv(k, v): one launch for aligned rows of head size 128, else the two."""
+    _check_kv4(k_cache, k_scale, v_scale)
     if (q.is_cuda and not _force_torch() and q.dtype == k.dtype == v.dtype == torch.bfloat16
             and q.shape[2] == 128 and k.stride(0) == v.stride(0)
             and all(t.stride(0) % 8 == 0 and t.data_ptr() % 16 == 0 and t.stride(2) == 1 and t.stride(1) == 128
@@ -231,9 +252,26 @@ def paged_prefill_plan(segs, device, rows: int = 256) -> tuple:
     return PagedGroups(upload(torch.tensor(groups, dtype=torch.int32).t().contiguous(), device), rows), short
 
 
-def attn_segments_paged(q, k_cache, v_cache, block_tables, context_lens, scale, plan, short, seg_tables, seg_start):
-    """Rows of long segments on the matrix cores against the paged bf16 cache, the others row by row (GPU only)."""
+def paged_plan(segs, heads: int, kv_heads: int, device, cache_dtype=torch.bfloat16) -> tuple:
+    """What attn_segments_paged takes of segments [(start position, rows)]: (groups of rows that attend together, or None,
+    [(first row, rows)] of those that attend row by row). Made once for all layers of a pass."""
+    rows = sum(n for _, n in segs)
+    if cache_dtype == torch.bfloat16 and paged_prefill_pays(segs, kv_heads):
+        return paged_prefill_plan(segs, device, 64 if paged_prefill_few(segs, heads) else 256)
+    return None, [(0, rows)] if rows else []
+
+
+def attn_segments_paged(q, k_cache, v_cache, block_tables, context_lens, scale, plan, short, seg_tables, seg_start,
+                        k_scale=None, v_scale=None):
+    """Rows of long segments on the matrix cores against the paged bf16 or 4-bit cache, the others row by row (GPU only).
+    ``plan`` and ``short``: of paged_plan for this cache's type."""
+    _check_kv4(k_cache, k_scale, v_scale)
     out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    if k_cache.dtype == torch.uint8:
+        for r, n in short:
+            _hip_or_raise().attn_decode4(q[r:r + n], k_cache, v_cache, block_tables[r:r + n], context_lens[r:r + n], scale,
+                                         k_scale, v_scale, None, out[r:r + n])
+        return out
     _hip_or_raise().attn_prefill_paged(out, q, k_cache, v_cache, plan.groups, seg_tables, seg_start, scale, plan.rows)
     f = _none(q, torch.float32)
     for r, n in short:
@@ -276,8 +314,13 @@ def attn_decode_paged(
     arrived: Optional[torch.Tensor] = None,
 ) -> torch.Tensor:
     """``arrived``: an int32 zero for each row and kv head, zero again afterwards; with it, contexts that several workgroups
-    share are merged in the same launch. Zeros for ATTN_COUNTER_GAP times as many keep the counters in cache lines of their own."""
-    if q.is_cuda and not _force_torch():
+    share are merged in the same launch. Zeros for ATTN_COUNTER_GAP times as many keep the counters in cache lines of their own.
+    k_scale/v_scale: what store_kv writes for fp8 and 4-bit caches."""
+    if k_cache.dtype == torch.uint8:
+        _check_kv4(k_cache, k_scale, v_scale)
+        if q.is_cuda and not _force_torch():
+            return _hip_or_raise().attn_decode4(q, k_cache, v_cache, block_tables, context_lens, scale, k_scale, v_scale, arrived)
+    elif q.is_cuda and not _force_torch():
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
         none = _none(q, torch.float32)
         _hip_or_raise().attn_decode_paged(

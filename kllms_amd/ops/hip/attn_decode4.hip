@@ -1,0 +1,582 @@
+// Paged decode attention (one query row for each stream) against a cache held in 4 bits (kv4.h), for gfx950.
+//
+// With k_td = n_td s_tg + m_tg for the values d of group g, n a whole number of 0..15:
+//
+//   score_t = sum_g s_tg (sum_d q_d n_td) + m_tg (sum_d q_d)      out_d = sum_t (p_t s_tg) n_td + sum_t p_t m_tg
+//
+// so the matrix cores multiply the whole numbers themselves, and step and least value meet sums, not elements: 36
+// vector instructions for the 64 values that a lane unpacks of 64 keys' K, where a value at a time took 128. A nibble masked out of its
+// half of a word is an fp16 number as it stands, n * 2^-24 (below the normal ones, which the matrix cores take as they
+// are), or 16 times that, which the other operand or the end makes good. q and p s are fp16 too: q's 8 bits are exact
+// once its largest is scaled into fp16's range, p s is rounded to 11 bits, which is 2^-12 of each and
+// a quarter of what the result's own rounding leaves when it is summed over keys.
+//
+// A wave takes 64 keys at a time and keeps its own running max and sum; four waves to a workgroup, Z workgroups to a context
+// (attn_decode4_shares), merged by the last of them to arrive or by a second launch where the caller has no counters.
+//
+//   scores   S[key][column] (16x16x32), column n is head n % GQA in set n / GQA. All sets hold the same scores; set j
+//            works on GQA of a lane's 16 alone: no exponential is computed twice, a lane loads the scales of GQA keys
+//   P V      O^T = V^T P^T: P's columns have the keys of their set and zeros for the others, sets are added up at the end
+//   max      renewed only when a score passes it by more than 8 (in powers of two), which leaves p s below fp16's end
+//   steps    p s is scaled by the power of two above the largest step of V so far, renewed like the max
+//
+// Nothing goes through LDS before the end. Key 4 r + c of 16 is row 4 c + r of a score tile: the rows that an instruction
+// loads of V, four of 64 bytes, are neighbours in memory then.
+//
+// What bounds it: the cache's bytes where contexts are many or long, else the chain of loads of one tile.
+
+#include <algorithm>
+
+#include "kv4.h"
+
+typedef _Float16 f16x8_mfma __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x2_cvt __attribute__((ext_vector_type(2)));
+typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
+typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+
+#define NTHREADS 256
+#define TKEYS 64           // keys of a wave's tile
+#define PART_STRIDE 132    // of a head's partial: 128 sums, max, sum of exponentials
+#define FAR 16             // loads and stores past the L2, from and to other XCDs' workgroups
+#define LAG 8.0f           // how far a score may pass the running max, in powers of two
+#define ROOM 128.0f        // 2^15 / 2^LAG
+#define LOG2E 1.44269504088896340736f
+
+union Frag4 {
+  u32x4 u;
+  f16x8_mfma m;
+};
+
+__device__ __forceinline__ uint32_t pack_f16(float a, float b) {
+  const f32x2 x = {a, b};
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector(x, f16x2_cvt));
+}
+
+// How many workgroups share a context: one for every ``per`` rounds of four tiles, ``most`` at most, and of those as many as
+// are all equally long.
+struct Decode4Shares {
+  int per, most;
+};
+__host__ __device__ __forceinline__ int shares4_of(int tiles, const Decode4Shares& s) {
+  const int rounds = (tiles + 3) / 4;
+  int z = (rounds + s.per - 1) / s.per;
+  z = z < s.most ? z : s.most;
+  if (z <= 1) return 1;
+  const int each = (rounds + z - 1) / z;
+  return (rounds + each - 1) / each;
+}
+
+// The partials [Z, GQA, PART_STRIDE] of a (stream, kv head), in their order, to its rows of the result, by all threads
+template <int GQA>
+__device__ __forceinline__ void merge4(bf16_t* __restrict__ out, const float* all, int Z, float (&sums)[NTHREADS][4],
+                                       float (&ml)[NTHREADS][2]) {
+  constexpr int SETS = NTHREADS / (32 * GQA), DEEP = 8;
+  const int tid = threadIdx.x, h = (tid >> 5) % GQA, d = (tid & 31) * 4, set = tid / (32 * GQA);
+  const auto far = __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(all), 0, Z * GQA * PART_STRIDE * 4, 0x00020000);
+  float M = -INFINITY, sum = 0.0f;
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+  for (int z0 = set; z0 < Z; z0 += DEEP * SETS) {
+    f32x4 part[DEEP];
+    f32x2 of[DEEP];
+#pragma unroll
+    for (int e = 0; e < DEEP; ++e) {       // behind the last one zeros
+      const int at = ((z0 + e * SETS) * GQA + h) * PART_STRIDE * 4;
+      of[e] = __builtin_bit_cast(f32x2, __builtin_amdgcn_raw_buffer_load_b64(far, at + 512, 0, FAR));
+      part[e] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(far, at + d * 4, 0, FAR));
+    }
+    const float before = M;
+#pragma unroll
+    for (int e = 0; e < DEEP; ++e)
+      if (z0 + e * SETS < Z) M = fmaxf(M, of[e][0]);
+    const float a = before == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(before - M);
+    sum *= a;
+    acc *= a;
+#pragma unroll
+    for (int e = 0; e < DEEP; ++e)
+      if (z0 + e * SETS < Z) {
+        const float w = of[e][0] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(of[e][0] - M);
+        sum += of[e][1] * w;
+        acc += part[e] * w;
+      }
+  }
+  if constexpr (SETS > 1) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) sums[tid][r] = acc[r];
+    ml[tid][0] = M;
+    ml[tid][1] = sum;
+    __syncthreads();
+    if (set > 0) return;
+    float top = M;
+#pragma unroll
+    for (int e = 1; e < SETS; ++e) top = fmaxf(top, ml[tid + e * 32 * GQA][0]);
+    const float a = M == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(M - top);
+    sum *= a;
+    acc *= a;
+#pragma unroll
+    for (int e = 1; e < SETS; ++e) {
+      const float m = ml[tid + e * 32 * GQA][0], w = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - top);
+      sum += ml[tid + e * 32 * GQA][1] * w;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) acc[r] += sums[tid + e * 32 * GQA][r] * w;
+    }
+  }
+  bf16x4_vec v;
+  // no key at all: zeros. (A sum that is no number stays none)
+#pragma unroll
+  for (int r = 0; r < 4; ++r) v[r] = f32_to_bf16(sum == 0.0f ? 0.0f : acc[r] / sum);
+  *reinterpret_cast<bf16x4_vec*>((short*)out + h * 128 + d) = v;
+}
+
+// WHOLE: blocks of a multiple of 16 keys
+template <int GQA, bool WHOLE>
+__global__ __launch_bounds__(NTHREADS, 3) void attn_decode4_kernel(
+    float* __restrict__ partials,          // [B, KVH, Z, GQA, PART_STRIDE]
+    bf16_t* __restrict__ out,              // written where one workgroup has the context, or by the last one with ``arrived``
+    const bf16_t* __restrict__ q,          // [B, H, 128], row stride q_stride
+    const uint32_t* __restrict__ k_cache, const uint32_t* __restrict__ v_cache,    // [NB, KVH, BS, 16] words
+    const uint32_t* __restrict__ k_scale, const uint32_t* __restrict__ v_scale,    // [NB, KVH, BS, 2] words (step, least)
+    const int* __restrict__ block_tables, const int* __restrict__ context_lens, int* __restrict__ arrived, int apart,
+    float scale, int block_size, uint32_t block_inverse, int max_blocks, int64_t q_stride, Decode4Shares shares) {
+  constexpr int SETS = 16 / GQA;
+  __shared__ __attribute__((aligned(16))) float o_lds[4][16][PART_STRIDE];
+  __shared__ float m_lds[4][16], l_lds[4][16];
+  __shared__ int last_lds;
+  const int g_kv = blockIdx.x, num_kv_heads = gridDim.x, b = blockIdx.y, z = blockIdx.z;
+  const int L = (int)min((int64_t)context_lens[b], (int64_t)max_blocks * block_size);
+  const int tiles = (max(L, 0) + TKEYS - 1) / TKEYS;
+  const int Z = shares4_of(tiles, shares);
+  if (z >= Z) return;
+  const int tid = threadIdx.x, lane = tid & 63, col = lane & 15, grp = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int head = col % GQA, set = col / GQA;
+
+  // ---- q: largest element to 2^14, exponents that fp16 holds; sums of its groups -------------
+  Frag4 qf[4];
+  float q_back, q_sum[2];
+  {
+    const short* qp = (const short*)q + (int64_t)b * q_stride + (g_kv * GQA + head) * 128 + grp * 4;
+    bf16x4_vec raw[4][2];
+#pragma unroll
+    for (int a = 0; a < 4; ++a)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) raw[a][h] = *reinterpret_cast<const bf16x4_vec*>(qp + a * 32 + h * 16);
+    float most = 0.0f, sum[2] = {0.0f, 0.0f};
+#pragma unroll
+    for (int a = 0; a < 4; ++a)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float x = bf16_to_f32(raw[a][h][i]);
+          most = fmaxf(most, fabsf(x));
+          sum[a >> 1] += x;
+        }
+#pragma unroll
+    for (int off = 16; off <= 32; off <<= 1) {
+      most = fmaxf(most, __shfl_xor(most, off));
+      sum[0] += __shfl_xor(sum[0], off);
+      sum[1] += __shfl_xor(sum[1], off);
+    }
+    const int e = max((int)(__float_as_uint(most) >> 23) - 127, -90);
+    const float up = ldexpf(1.0f, 14 - e);
+#pragma unroll
+    for (int a = 0; a < 4; ++a) {
+      const float u = a & 1 ? up * 0.0625f : up;       // nibbles 1 and 3 of a half stand 16 times too high
+#pragma unroll
+      for (int i = 0; i < 4; ++i) qf[a].u[i] = pack_f16(bf16_to_f32(raw[a][0][i]) * u, bf16_to_f32(raw[a][1][i]) * u);
+    }
+    const float by = scale * LOG2E;
+    q_back = ldexpf(by, e - 14 + 24);
+    q_sum[0] = sum[0] * by;
+    q_sum[1] = sum[1] * by;
+  }
+
+  // ---- which of a tile's keys this lane weighs: score tile tt_of(i), register r_of(i) ----------
+  // GQA 8: r 2 set + (i & 1), tt i / 2; 4: r set, tt i; 2: r set & 3, tt 2 (set / 4) + i; 1: r set & 3, tt set / 4
+  auto key_in_tile = [&](int i) {
+    const int r = GQA == 8 ? 2 * set + (i & 1) : set & 3;
+    const int tt = GQA == 8 ? i >> 1 : GQA == 4 ? i : GQA == 2 ? 2 * (set >> 2) + i : set >> 2;
+    return 16 * tt + 4 * r + grp;
+  };
+  // where p goes in P's fragment: words 0 and 1 of a score tile's two, by register
+  const int r_mine = GQA == 8 ? 2 * set : set & 3;
+  const uint32_t half = GQA == 8 ? 0xffffffffu : r_mine & 1 ? 0xffff0000u : 0x0000ffffu;
+  const uint32_t keep[2] = {r_mine < 2 ? half : 0u, r_mine < 2 ? 0u : half};
+
+  const int* bt = block_tables + (int64_t)b * max_blocks;
+  auto block_of = [&](int key) {           // key / block_size by its reciprocal, which is off by one at most
+    const int n = (int)__umulhi((uint32_t)key, block_inverse), rest = key - n * block_size;
+    return n - (rest < 0) + (rest >= block_size);
+  };
+
+  u32x4 kraw[4];
+  uint32_t vraw[4][4];
+  u32x2 ks[GQA], vs[GQA];
+  constexpr int IDS = WHOLE ? 4 : 1;
+  int ids[IDS];                            // WHOLE: blocks of a tile's four sixteens; else the block of this lane's key
+  auto ask = [&](int t) {
+#pragma unroll
+    for (int i = 0; i < IDS; ++i) {
+      const int key = min(t * TKEYS + (WHOLE ? i * 16 : lane), L - 1);
+      ids[i] = bt[block_of(key)];
+    }
+  };
+  const int k_row = 4 * (col & 3) + (col >> 2);        // key of row ``col`` of a score tile
+  auto load_k = [&](int t, const int64_t (&base)[4], int row) {
+    if constexpr (WHOLE) {
+#pragma unroll
+      for (int tt = 0; tt < 4; ++tt) kraw[tt] = *reinterpret_cast<const u32x4*>(k_cache + base[tt] * 16 + (k_row * 16 + grp * 4));
+#pragma unroll
+      for (int i = 0; i < GQA; ++i) {
+        const int key = key_in_tile(i), tt = key >> 4;
+        int64_t at = base[0];
+        if constexpr (GQA >= 4) {
+          at = base[GQA == 8 ? i >> 1 : i];
+        } else {
+#pragma unroll
+          for (int e = 1; e < 4; ++e) at = tt == e ? base[e] : at;
+        }
+        ks[i] = *reinterpret_cast<const u32x2*>(k_scale + (at + (key & 15)) * 2);
+        vs[i] = *reinterpret_cast<const u32x2*>(v_scale + (at + (key & 15)) * 2);
+      }
+    } else {
+#pragma unroll
+      for (int tt = 0; tt < 4; ++tt) {
+        const int64_t r = __shfl(row, 16 * tt + k_row);
+        kraw[tt] = *reinterpret_cast<const u32x4*>(k_cache + r * 16 + grp * 4);
+      }
+#pragma unroll
+      for (int i = 0; i < GQA; ++i) {
+        const int64_t r = __shfl(row, key_in_tile(i));
+        ks[i] = *reinterpret_cast<const u32x2*>(k_scale + r * 2);
+        vs[i] = *reinterpret_cast<const u32x2*>(v_scale + r * 2);
+      }
+    }
+  };
+  auto load_v = [&](const int64_t (&base)[4], int row) {
+#pragma unroll
+    for (int tt = 0; tt < 4; ++tt)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        if constexpr (WHOLE) vraw[tt][r] = v_cache[base[tt] * 16 + ((4 * r + grp) * 16 + col)];
+        else vraw[tt][r] = v_cache[(int64_t)__shfl(row, 16 * tt + 4 * r + grp) * 16 + col];
+      }
+  };
+  // rows of the cache: of the four sixteens' first keys, or of this lane's key; those behind the context repeat what is in it
+  auto rows_of = [&](int t, int64_t (&base)[4], int& row) {
+    if constexpr (WHOLE) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int key = min(t * TKEYS + i * 16, (L - 1) & ~15);
+        base[i] = ((int64_t)ids[i] * num_kv_heads + g_kv) * block_size + (key - block_of(key) * block_size);
+      }
+    } else {
+      const int key = min(t * TKEYS + lane, L - 1);
+      row = (ids[0] * num_kv_heads + g_kv) * block_size + (key - block_of(key) * block_size);
+    }
+  };
+
+  f32x4 o[8];
+#pragma unroll
+  for (int p = 0; p < 8; ++p) o[p] = f32x4{0.f, 0.f, 0.f, 0.f};
+  float m_run = -INFINITY, l_run = 0.0f, low_run[2] = {0.0f, 0.0f};      // of this lane's head and keys
+  float cap = 0.0f, to_cap = 0.0f;         // power of two from V's largest step so far on; what p s is multiplied by
+
+  const int step = Z * 4;
+  int t = z * 4 + wave;
+  int64_t base[4];
+  int row = 0;
+  if (t < tiles) {
+    ask(t);
+    rows_of(t, base, row);
+    load_k(t, base, row);
+    load_v(base, row);
+    ask(min(t + step, tiles - 1));
+  }
+#pragma unroll 1
+  for (; t < tiles; t += step) {
+    const bool more = t + step < tiles;
+    if (more) {
+      rows_of(t + step, base, row);
+      ask(min(t + 2 * step, tiles - 1));
+    }
+    // ---- scores of whole numbers, a group at a time ---------------------------------------
+    float x[GQA];
+    {
+      f32x4 acc[4][2];
+#pragma unroll
+      for (int tt = 0; tt < 4; ++tt) {
+        Frag4 f[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t w = kraw[tt][i], w8 = w >> 8;
+          f[0].u[i] = w & 0x000f000fu;
+          f[1].u[i] = w & 0x00f000f0u;
+          f[2].u[i] = w8 & 0x000f000fu;
+          f[3].u[i] = w8 & 0x00f000f0u;
+        }
+        const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+          acc[tt][g] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f[2 * g].m, qf[2 * g].m, zero, 0, 0, 0);
+          acc[tt][g] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f[2 * g + 1].m, qf[2 * g + 1].m, acc[tt][g], 0, 0, 0);
+        }
+      }
+      auto mine = [&](int i, int g) {      // of the registers of all sets, this one's
+        if constexpr (GQA == 8) return set ? acc[i >> 1][g][2 + (i & 1)] : acc[i >> 1][g][i & 1];
+        auto of = [&](int tt) {
+          const f32x4 a = acc[tt][g];
+          const float lo = set & 1 ? a[1] : a[0], hi = set & 1 ? a[3] : a[2];
+          return set & 2 ? hi : lo;
+        };
+        if constexpr (GQA == 4) return of(i);
+        if constexpr (GQA == 2) return set & 4 ? of(2 + i) : of(i);
+        const float lo = set & 4 ? of(1) : of(0), hi = set & 4 ? of(3) : of(2);
+        return set & 8 ? hi : lo;
+      };
+#pragma unroll
+      for (int i = 0; i < GQA; ++i) {
+        const float whole = __builtin_fmaf(kv4_step(ks[i][1]), mine(i, 1), kv4_step(ks[i][0]) * mine(i, 0));
+        const float low = __builtin_fmaf(kv4_least(ks[i][1]), q_sum[1], kv4_least(ks[i][0]) * q_sum[0]);
+        x[i] = __builtin_fmaf(whole, q_back, low);
+      }
+    }
+    float v_step[GQA][2], v_low[GQA][2];
+#pragma unroll
+    for (int i = 0; i < GQA; ++i)
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+        v_step[i][g] = kv4_step(vs[i][g]);
+        v_low[i][g] = kv4_least(vs[i][g]);
+      }
+    if (t * TKEYS + TKEYS > L) {           // what lies behind the context is another's
+#pragma unroll
+      for (int i = 0; i < GQA; ++i)
+        if (t * TKEYS + key_in_tile(i) >= L) {
+          x[i] = -INFINITY;
+#pragma unroll
+          for (int g = 0; g < 2; ++g) v_step[i][g] = v_low[i][g] = 0.0f;
+        }
+    }
+    if (more) load_k(t + step, base, row);
+    // ---- the max and the largest step, renewed when they have to be ---------------------------
+    float top = x[0], wide = fmaxf(v_step[0][0], v_step[0][1]);
+#pragma unroll
+    for (int i = 1; i < GQA; ++i) {
+      top = fmaxf(top, x[i]);
+      wide = fmaxf(wide, fmaxf(v_step[i][0], v_step[i][1]));
+    }
+    if (__any(top > m_run + LAG || wide > cap)) {
+#pragma unroll
+      for (int off = GQA; off <= 32; off <<= 1) top = fmaxf(top, __shfl_xor(top, off));
+#pragma unroll
+      for (int off = 1; off <= 32; off <<= 1) wide = fmaxf(wide, __shfl_xor(wide, off));
+      const float m_new = fmaxf(m_run, top);
+      const float alpha = m_run == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m_run - m_new);
+      m_run = m_new;
+      float shrink = 1.0f;
+      if (wide > cap) {                    // 2^(e + 1), within what its inverse times ROOM can be
+        const int e = min(max((int)(__float_as_uint(wide) >> 23) - 126, -110), 127);
+        const float cap_new = ldexpf(1.0f, e);
+        shrink = cap > 0.0f ? cap / cap_new : 0.0f;
+        cap = cap_new;
+        to_cap = ROOM / cap;
+      }
+      l_run *= alpha;
+      low_run[0] *= alpha;
+      low_run[1] *= alpha;
+#pragma unroll
+      for (int p = 0; p < 8; ++p) o[p] *= alpha * shrink;
+    }
+    // ---- P, and P times V's steps to fragments ------------------------------------------------
+    const float m_use = m_run == -INFINITY ? 0.0f : m_run;
+    Frag4 pf[2][2];                        // [32 keys][group]
+    {
+      uint32_t w[GQA][2];
+      float ps[GQA][2];
+#pragma unroll
+      for (int i = 0; i < GQA; ++i) {
+        const float p = __builtin_amdgcn_exp2f(x[i] - m_use);
+        l_run += p;
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+          ps[i][g] = p * (v_step[i][g] * to_cap);
+          low_run[g] = __builtin_fmaf(p, v_low[i][g], low_run[g]);
+          if constexpr (GQA < 8) w[i][g] = pack_f16(ps[i][g], ps[i][g]);
+        }
+      }
+#pragma unroll
+      for (int tt = 0; tt < 4; ++tt)
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+          uint32_t v;
+          if constexpr (GQA == 8) v = pack_f16(ps[2 * tt][g], ps[2 * tt + 1][g]);
+          else if constexpr (GQA == 4) v = w[tt][g];
+          else if constexpr (GQA == 2) v = set >> 2 == tt >> 1 ? w[tt & 1][g] : 0u;
+          else v = set >> 2 == tt ? w[0][g] : 0u;
+#pragma unroll
+          for (int e = 0; e < 2; ++e) pf[tt >> 1][g].u[(tt & 1) * 2 + e] = v & keep[e];
+        }
+    }
+    // ---- P V: 32 keys at a time, a nibble a column tile -----------------------------------------
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      Frag4 f[8];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t a = vraw[2 * s + (e >> 1)][(e & 1) * 2], c = vraw[2 * s + (e >> 1)][(e & 1) * 2 + 1];
+        const uint32_t lo = __builtin_amdgcn_perm(c, a, 0x05040100), hi = __builtin_amdgcn_perm(c, a, 0x07060302);
+        const uint32_t lo8 = lo >> 8, hi8 = hi >> 8;
+        f[0].u[e] = lo & 0x000f000fu;
+        f[1].u[e] = lo & 0x00f000f0u;
+        f[2].u[e] = lo8 & 0x000f000fu;
+        f[3].u[e] = lo8 & 0x00f000f0u;
+        f[4].u[e] = hi & 0x000f000fu;
+        f[5].u[e] = hi & 0x00f000f0u;
+        f[6].u[e] = hi8 & 0x000f000fu;
+        f[7].u[e] = hi8 & 0x00f000f0u;
+      }
+#pragma unroll
+      for (int p = 0; p < 8; ++p) o[p] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f[p].m, pf[s][(p & 3) >> 1].m, o[p], 0, 0, 0);
+    }
+    if (more) load_v(base, row);
+  }
+
+  // ---- this wave's sums, then the sets' and the waves' ------------------------------------------
+#pragma unroll
+  for (int off = 16; off <= 32; off <<= 1) {
+    l_run += __shfl_xor(l_run, off);
+    low_run[0] += __shfl_xor(low_run[0], off);
+    low_run[1] += __shfl_xor(low_run[1], off);
+  }
+  const float back = cap * (16777216.0f / ROOM);       // 2^24: the nibbles'
+#pragma unroll
+  for (int p = 0; p < 8; ++p) {
+    const int g = (p & 3) >> 1;
+    f32x4 v;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) v[r] = __builtin_fmaf(o[p][r], p & 1 ? back * 0.0625f : back, low_run[g]);
+    *reinterpret_cast<f32x4*>(&o_lds[wave][col][32 * (p & 3) + 16 * (p >> 2) + 4 * grp]) = v;
+  }
+  if (lane < 16) {
+    m_lds[wave][lane] = m_run;
+    l_lds[wave][lane] = l_run;
+  }
+  __syncthreads();
+  float* const part = partials + (((int64_t)b * num_kv_heads + g_kv) * gridDim.z + z) * (GQA * PART_STRIDE);
+  bf16_t* const to = out + ((int64_t)b * num_kv_heads + g_kv) * GQA * 128;
+  constexpr int VEC = GQA > 2 ? GQA / 2 : 1;
+  if (tid * VEC < GQA * 128) {
+    const int h = tid * VEC >> 7, d = tid * VEC & 127;
+    float M = m_lds[0][h];
+#pragma unroll
+    for (int w = 1; w < 4; ++w) M = fmaxf(M, m_lds[w][h]);
+    float acc[VEC] = {}, l = 0.0f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const float e = m_lds[w][h] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m_lds[w][h] - M);
+#pragma unroll
+      for (int j = 0; j < SETS; ++j) {
+        l += l_lds[w][h + GQA * j] * e;
+#pragma unroll
+        for (int r = 0; r < VEC; ++r) acc[r] += o_lds[w][h + GQA * j][d + r] * e;
+      }
+    }
+    if (Z == 1) {
+#pragma unroll
+      for (int r = 0; r < VEC; ++r) ((short*)to)[h * 128 + d + r] = f32_to_bf16(l == 0.0f ? 0.0f : acc[r] / l);
+    } else {
+      const auto far = __builtin_amdgcn_make_buffer_rsrc(part, 0, GQA * PART_STRIDE * 4, 0x00020000);
+#pragma unroll
+      for (int r = 0; r < VEC; ++r) __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(acc[r]), far, (h * PART_STRIDE + d + r) * 4, 0, FAR);
+      if (d == 0) __builtin_amdgcn_raw_buffer_store_b64(u32x2{__float_as_uint(M), __float_as_uint(l)}, far, (h * PART_STRIDE + 128) * 4, 0, FAR);
+    }
+  }
+  if (Z == 1 || !arrived) return;
+  // ---- the last workgroup to arrive merges the partials ------------------------------------------
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  if (tid == 0) {
+    int* const count = arrived + ((int64_t)b * num_kv_heads + g_kv) * apart;
+    last_lds = __hip_atomic_fetch_add(count, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == Z - 1;
+    if (last_lds) __hip_atomic_store(count, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  __syncthreads();
+  if (!last_lds) return;
+  merge4<GQA>(to, part - (int64_t)z * (GQA * PART_STRIDE), Z, reinterpret_cast<float(&)[NTHREADS][4]>(o_lds[0]),
+              reinterpret_cast<float(&)[NTHREADS][2]>(o_lds[1]));
+}
+
+// the same for callers without counters
+template <int GQA>
+__global__ __launch_bounds__(NTHREADS) void attn_decode4_merge_kernel(bf16_t* __restrict__ out, const float* __restrict__ partials,
+                                                                     const int* __restrict__ context_lens, int grid_z, int64_t most,
+                                                                     Decode4Shares shares) {
+  __shared__ float sums[NTHREADS][4], ml[NTHREADS][2];
+  const int g_kv = blockIdx.x, num_kv_heads = gridDim.x, b = blockIdx.y;
+  const int L = (int)min((int64_t)context_lens[b], most);
+  const int Z = shares4_of((max(L, 0) + TKEYS - 1) / TKEYS, shares);
+  if (Z == 1) return;
+  const int64_t pair = (int64_t)b * num_kv_heads + g_kv;
+  merge4<GQA>(out + pair * GQA * 128, partials + pair * grid_z * (GQA * PART_STRIDE), Z, sums, ml);
+}
+
+// rows of a launch: they lie on the grid's y, which ends at 65535
+#define MAX_ROWS 65535
+
+static Decode4Shares attn_decode4_shares(int B, int num_kv_heads) {
+  const int64_t pairs = (int64_t)B * num_kv_heads;
+  Decode4Shares s;
+  s.per = 1;
+  s.most = (int)std::max<int64_t>(1, std::min<int64_t>(768 / pairs, 128));
+  return s;
+}
+
+// workgroups per context of a launch; max_ctx: positions of the table
+extern "C" int attn_decode4_splits(int B, int num_kv_heads, int max_ctx) {
+  const int tiles = (int)(((int64_t)max_ctx + TKEYS - 1) / TKEYS), rounds = (tiles + 3) / 4;
+  const Decode4Shares s = attn_decode4_shares(B < MAX_ROWS ? B : MAX_ROWS, num_kv_heads);
+  return std::max(1, std::min(rounds, s.most));
+}
+
+// floats of a launch's partials for each (row, kv head, workgroup, head of it)
+extern "C" int attn_decode4_part() { return PART_STRIDE; }
+
+extern "C" void launch_attn_decode4(bf16_t* out, float* partials, int* arrived, int apart, const bf16_t* q, const void* k_cache,
+                                    const void* v_cache, const void* k_scale, const void* v_scale, const int* block_tables,
+                                    const int* context_lens, float scale, int num_q_heads, int num_kv_heads, int block_size,
+                                    int max_blocks, int max_ctx, int64_t q_stride, int B, hipStream_t stream) {
+  const int gqa = num_q_heads / num_kv_heads, splits = attn_decode4_splits(B, num_kv_heads, max_ctx);
+  const Decode4Shares sh = attn_decode4_shares(B < MAX_ROWS ? B : MAX_ROWS, num_kv_heads);
+  const uint32_t inverse = block_size > 1 ? (uint32_t)(((1ull << 32) + block_size - 1) / block_size) : ~0u;
+  for (int b0 = 0; b0 < B; b0 += MAX_ROWS) {
+    const int rows = B - b0 < MAX_ROWS ? B - b0 : MAX_ROWS;
+    const dim3 grid(num_kv_heads, rows, splits);
+    bf16_t* o = out + (int64_t)b0 * num_q_heads * 128;
+    const bf16_t* q0 = q + (int64_t)b0 * q_stride;
+    const int* bt = block_tables + (int64_t)b0 * max_blocks;
+    int* a0 = arrived ? arrived + (int64_t)b0 * num_kv_heads * apart : nullptr;
+#define LAUNCH(G, W)                                                                                                    \
+  hipLaunchKernelGGL((attn_decode4_kernel<G, W>), grid, dim3(NTHREADS), 0, stream, partials, o, q0, (const uint32_t*)k_cache, \
+                     (const uint32_t*)v_cache, (const uint32_t*)k_scale, (const uint32_t*)v_scale, bt, context_lens + b0, a0,  \
+                     apart, scale, block_size, inverse, max_blocks, q_stride, sh)
+#define DISPATCH(G)                                                                                                       \
+  do {                                                                                                                    \
+    if (block_size % 16 == 0) LAUNCH(G, true);                                                                            \
+    else LAUNCH(G, false);                                                                                                \
+    if (splits > 1 && !arrived)                                                                                           \
+      hipLaunchKernelGGL(attn_decode4_merge_kernel<G>, dim3(num_kv_heads, rows), dim3(NTHREADS), 0, stream, o, partials,  \
+                         context_lens + b0, splits, (int64_t)max_blocks * block_size, sh);                                \
+  } while (0)
+    switch (gqa) {
+      case 1: DISPATCH(1); break;
+      case 2: DISPATCH(2); break;
+      case 4: DISPATCH(4); break;
+      default: DISPATCH(8); break;
+    }
+#undef DISPATCH
+#undef LAUNCH
+  }
+}

@@ -34,6 +34,11 @@ extern "C" __global__ void mfma_selftest_kernel(float*, const bf16_t*, const bf1
               ((t).scalar_type() == at::kBFloat16 || (t).scalar_type() == at::kFloat8_e4m3fn), \
               #t " must be a contiguous bf16 or fp8-e4m3 KV cache on GPU")
 
+#define CHECK_ANY_CACHE(t) \
+  TORCH_CHECK((t).is_cuda() && (t).is_contiguous() && \
+              ((t).scalar_type() == at::kBFloat16 || (t).scalar_type() == at::kFloat8_e4m3fn || (t).scalar_type() == at::kByte), \
+              #t " must be a contiguous bf16, fp8-e4m3 or 4-bit (uint8) KV cache on GPU")
+
 #define CHECK_BF16_ROWS(t) \
   TORCH_CHECK((t).is_cuda() && (t).scalar_type() == at::kBFloat16 && (t).dim() == 3 && \
               (t).stride(2) == 1 && (t).stride(1) == (t).size(2), #t " must be a bf16 [T,H,D] row view")
@@ -86,8 +91,120 @@ void rope_inplace(torch::Tensor q, torch::Tensor k, torch::Tensor positions, tor
                      H, KVH, D, (int)q.stride(0), (int)k.stride(0));
 }
 
+// The 4-bit caches [NB, KVH, BS, 64] uint8 and their scales [NB, KVH, BS, 2, 2] bf16, on one device
+static void check_kv4(const torch::Tensor& k_cache, const torch::Tensor& v_cache, const torch::Tensor& k_scale,
+                      const torch::Tensor& v_scale, const torch::Tensor& like, const char* who) {
+  for (const auto& c : {k_cache, v_cache})
+    TORCH_CHECK(c.scalar_type() == at::kByte && c.dim() == 4 && c.size(3) == 64 && c.is_contiguous() && c.sizes() == k_cache.sizes() &&
+                    c.device() == like.device() && reinterpret_cast<uintptr_t>(c.data_ptr()) % 16 == 0,
+                who, ": 4-bit caches are contiguous uint8 [blocks, kv heads, block, 64] (head size 128) on 16 bytes");
+  for (const auto& c : {k_scale, v_scale})
+    TORCH_CHECK(c.scalar_type() == at::kBFloat16 && c.is_contiguous() && c.dim() == 5 && c.size(0) == k_cache.size(0) &&
+                    c.size(1) == k_cache.size(1) && c.size(2) == k_cache.size(2) && c.size(3) == 2 && c.size(4) == 2 &&
+                    c.device() == like.device() && reinterpret_cast<uintptr_t>(c.data_ptr()) % 8 == 0,
+                who, ": scales of 4-bit caches are contiguous bf16 [blocks, kv heads, block, 2, 2]");
+  TORCH_CHECK(k_cache.size(0) * k_cache.size(1) * k_cache.size(2) < (1LL << 31), who, ": cache rows exceed 32-bit indexing");
+}
+
+static bool rows_aligned(const torch::Tensor& t);
+
+extern "C" void launch_kv4_store(const bf16_t*, const bf16_t*, void*, void*, void*, void*, const int64_t*, int, int, int64_t, int64_t, int,
+                                 int64_t, hipStream_t);
+extern "C" void launch_kv4_load(bf16_t*, bf16_t*, const void*, const void*, const void*, const void*, const int64_t*, int, int, int,
+                                int64_t, hipStream_t);
+
+static void store_kv4(torch::Tensor k, torch::Tensor v, torch::Tensor k_cache, torch::Tensor v_cache, torch::Tensor slots,
+                      torch::Tensor k_scale, torch::Tensor v_scale) {
+  CHECK_BF16_ROWS(k); CHECK_BF16_ROWS(v);
+  check_kv4(k_cache, v_cache, k_scale, v_scale, k, "store_kv");
+  const int64_t T = k.size(0), G = k.size(1);
+  TORCH_CHECK(k.size(2) == 128 && v.sizes() == k.sizes() && v.device() == k.device() && k_cache.size(1) == G, "store_kv: rows [T, kv heads, 128]");
+  TORCH_CHECK(slots.scalar_type() == at::kLong && slots.dim() == 1 && slots.numel() == T && slots.is_contiguous() &&
+                  slots.device() == k.device(), "store_kv: a slot for each row, int64");
+  TORCH_CHECK(T < (1LL << 31), "store_kv: rows exceed 32-bit indexing");
+  if (T == 0 || k_cache.numel() == 0) return;
+  const c10::DeviceGuard device(k.device());
+  if (!rows_aligned(k)) k = k.clone(at::MemoryFormat::Contiguous);
+  if (!rows_aligned(v)) v = v.clone(at::MemoryFormat::Contiguous);
+  launch_kv4_store(cbf(k), cbf(v), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
+                   slots.data_ptr<int64_t>(), (int)T, (int)G, k.stride(0), v.stride(0), (int)k_cache.size(2),
+                   k_cache.size(0) * k_cache.size(2), cur_stream());
+}
+
+// What the 4-bit caches' rows at the slots stand for, rounded to bf16: (k, v) [T, kv heads, 128]
+std::tuple<torch::Tensor, torch::Tensor> load_kv4(torch::Tensor k_cache, torch::Tensor v_cache, torch::Tensor slots,
+                                                  torch::Tensor k_scale, torch::Tensor v_scale) {
+  TORCH_CHECK(k_cache.is_cuda(), "load_kv: a cache on the GPU");
+  check_kv4(k_cache, v_cache, k_scale, v_scale, k_cache, "load_kv");
+  TORCH_CHECK(slots.scalar_type() == at::kLong && slots.dim() == 1 && slots.is_contiguous() && slots.device() == k_cache.device(),
+              "load_kv: slots int64 [T]");
+  const int64_t T = slots.numel(), G = k_cache.size(1);
+  TORCH_CHECK(T < (1LL << 31), "load_kv: rows exceed 32-bit indexing");
+  const c10::DeviceGuard device(k_cache.device());
+  auto k = torch::empty({T, G, 128}, k_scale.options()), v = torch::empty_like(k);
+  if (k.numel() == 0) return {k, v};
+  launch_kv4_load(bf(k), bf(v), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
+                  slots.data_ptr<int64_t>(), (int)T, (int)G, (int)k_cache.size(2), k_cache.size(0) * k_cache.size(2), cur_stream());
+  return {k, v};
+}
+
+extern "C" int attn_decode4_splits(int B, int num_kv_heads, int max_ctx);
+extern "C" int attn_decode4_part();
+extern "C" void launch_attn_decode4(bf16_t*, float*, int*, int, const bf16_t*, const void*, const void*, const void*, const void*,
+                                    const int*, const int*, float, int, int, int, int, int, int64_t, int, hipStream_t);
+
+// Rows of tables int32 [B, MAXB] and lengths int32 [B] beside q [B, H, 128]
+static void check_contexts(const torch::Tensor& q, const torch::Tensor& tables, const torch::Tensor& lens, const char* who) {
+  TORCH_CHECK(tables.scalar_type() == at::kInt && tables.dim() == 2 && tables.is_contiguous() && tables.size(0) == q.size(0) &&
+                  tables.device() == q.device() && lens.scalar_type() == at::kInt && lens.is_contiguous() &&
+                  lens.numel() == q.size(0) && lens.device() == q.device(),
+              who, ": block tables int32 [rows, blocks] and lengths int32 [rows] on q's device");
+}
+
+// attn_decode_paged of the 4-bit caches
+torch::Tensor attn_decode4(torch::Tensor q, torch::Tensor k_cache, torch::Tensor v_cache, torch::Tensor block_tables,
+                           torch::Tensor context_lens, double scale, torch::Tensor k_scale, torch::Tensor v_scale,
+                           std::optional<torch::Tensor> arrived, std::optional<torch::Tensor> into) {
+  CHECK_BF16_ROWS(q);
+  check_kv4(k_cache, v_cache, k_scale, v_scale, q, "attn_decode_paged");
+  check_contexts(q, block_tables, context_lens, "attn_decode_paged");
+  const int64_t B = q.size(0), H = q.size(1), KVH = k_cache.size(1), BS = k_cache.size(2), max_blocks = block_tables.size(1);
+  TORCH_CHECK(q.size(2) == 128 && KVH > 0 && H % KVH == 0, "attn_decode_paged: head size 128, whole groups of heads");
+  const int64_t gqa = H / KVH;
+  TORCH_CHECK(gqa == 1 || gqa == 2 || gqa == 4 || gqa == 8, "attn_decode_paged: 1, 2, 4 or 8 heads to a kv head");
+  TORCH_CHECK(max_blocks < (1LL << 31) && B < (1LL << 31), "attn_decode_paged: sizes");
+  const c10::DeviceGuard device(q.device());
+  auto out = into ? *into : torch::empty({B, H, 128}, q.options());
+  TORCH_CHECK(out.is_contiguous() && out.sizes() == q.sizes() && out.scalar_type() == at::kBFloat16 && out.device() == q.device(),
+              "attn_decode_paged: result");
+  if (B == 0) return out;
+  if (max_blocks == 0 || k_cache.numel() == 0) return out.zero_();     // every context is empty
+  if (!rows_aligned(q)) q = q.clone(at::MemoryFormat::Contiguous);
+  const int longest = (int)std::min<int64_t>(max_blocks * BS, INT32_MAX);
+  const int splits = attn_decode4_splits((int)B, (int)KVH, longest);
+  int apart = 1;
+  if (arrived) {
+    TORCH_CHECK(arrived->is_contiguous() && arrived->scalar_type() == at::kInt && arrived->numel() >= B * KVH &&
+                    arrived->device() == q.device(), "arrived: an int32 zero for each row and kv head");
+    apart = (int)std::min<int64_t>(arrived->numel() / (B * KVH), 32);
+  }
+  auto partials = torch::empty({splits > 1 ? std::min<int64_t>(B, 65535) * KVH * splits * gqa * attn_decode4_part() : 0},
+                               q.options().dtype(torch::kFloat));
+  launch_attn_decode4(bf(out), partials.data_ptr<float>(), arrived ? arrived->data_ptr<int>() : nullptr, apart, cbf(q),
+                      k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), block_tables.data_ptr<int>(),
+                      context_lens.data_ptr<int>(), (float)scale, (int)H, (int)KVH, (int)BS, (int)max_blocks, longest, q.stride(0),
+                      (int)B, cur_stream());
+  return out;
+}
+
+// what a step's kernels write to: 0 bf16, 1 e4m3, 2 four bits
+static int cache_kind(const torch::Tensor& k_cache) {
+  return k_cache.scalar_type() == at::kByte ? CACHE_KV4 : k_cache.scalar_type() == at::kFloat8_e4m3fn ? CACHE_FP8 : CACHE_BF16;
+}
+
 void store_kv(torch::Tensor k, torch::Tensor v, torch::Tensor k_cache, torch::Tensor v_cache,
               torch::Tensor slot_mapping, torch::Tensor k_scale, torch::Tensor v_scale) {
+  if (k_cache.scalar_type() == at::kByte) return store_kv4(k, v, k_cache, v_cache, slot_mapping, k_scale, v_scale);
   CHECK_BF16_ROWS(k); CHECK_BF16_ROWS(v); CHECK_KV_CACHE(k_cache); CHECK_KV_CACHE(v_cache);
   TORCH_CHECK(k.stride(0) == v.stride(0), "k/v must share the token stride");
   const int T = k.size(0), KVH = k.size(1), D = k.size(2);
@@ -115,18 +232,18 @@ void store_kv(torch::Tensor k, torch::Tensor v, torch::Tensor k_cache, torch::Te
 }
 
 extern "C" void launch_rope_store(bf16_t* q, bf16_t* k, const bf16_t* v, const int64_t* positions,
-                                  const float* cos_sin, void* k_cache, void* v_cache, float* k_scale, float* v_scale,
+                                  const float* cos_sin, void* k_cache, void* v_cache, void* k_scale, void* v_scale,
                                   const int64_t* slots, int T, int H, int G, int q_stride, int kv_stride,
-                                  int block_size, int fp8, hipStream_t stream);
+                                  int block_size, int kind, hipStream_t stream);
 
 // rope_inplace and store_kv of rows of head size 128 in one launch; views of 16-byte aligned rows
 void rope_store(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor positions, torch::Tensor cos_sin,
                 torch::Tensor k_cache, torch::Tensor v_cache, torch::Tensor slots, torch::Tensor k_scale,
                 torch::Tensor v_scale) {
-  CHECK_BF16_ROWS(q); CHECK_BF16_ROWS(k); CHECK_BF16_ROWS(v); CHECK_KV_CACHE(k_cache); CHECK_KV_CACHE(v_cache);
+  CHECK_BF16_ROWS(q); CHECK_BF16_ROWS(k); CHECK_BF16_ROWS(v); CHECK_ANY_CACHE(k_cache); CHECK_ANY_CACHE(v_cache);
   const int T = q.size(0), H = q.size(1), G = k.size(1), BS = k_cache.size(2);
   TORCH_CHECK(q.size(2) == 128 && k.size(2) == 128 && v.sizes() == k.sizes() && k.size(0) == T &&
-                  k.stride(0) == v.stride(0) && k_cache.size(1) == G && k_cache.size(3) == 128 &&
+                  k.stride(0) == v.stride(0) && k_cache.size(1) == G && k_cache.size(3) == (k_cache.scalar_type() == at::kByte ? 64 : 128) &&
                   v_cache.sizes() == k_cache.sizes() && v_cache.scalar_type() == k_cache.scalar_type(),
               "rope_store: sizes");
   for (const auto& t : {q, k, v})
@@ -135,17 +252,18 @@ void rope_store(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor
                   slots.scalar_type() == at::kLong && slots.is_contiguous() && slots.numel() == T &&
                   cos_sin.scalar_type() == at::kFloat && cos_sin.is_contiguous() && cos_sin.size(-1) == 128,
               "rope_store: positions, slots or angles");
-  const int fp8 = k_cache.scalar_type() == at::kFloat8_e4m3fn ? 1 : 0;
-  if (fp8)
+  const int kind = cache_kind(k_cache);
+  if (kind == CACHE_KV4) check_kv4(k_cache, v_cache, k_scale, v_scale, k, "rope_store");
+  if (kind == CACHE_FP8)
     TORCH_CHECK(k_scale.numel() == k_cache.size(0) * G * BS && k_scale.is_contiguous() &&
                     k_scale.scalar_type() == at::kFloat && v_scale.numel() == k_scale.numel() &&
                     v_scale.is_contiguous() && v_scale.scalar_type() == at::kFloat,
                 "fp8 rope_store requires [NB, KVH, BS] fp32 k_scale/v_scale");
   if (T == 0) return;
   launch_rope_store(bf(q), bf(k), cbf(v), positions.data_ptr<int64_t>(), cos_sin.data_ptr<float>(), k_cache.data_ptr(),
-                    v_cache.data_ptr(), fp8 ? k_scale.data_ptr<float>() : nullptr,
-                    fp8 ? v_scale.data_ptr<float>() : nullptr, slots.data_ptr<int64_t>(), T, H, G, (int)q.stride(0),
-                    (int)k.stride(0), BS, fp8, cur_stream());
+                    v_cache.data_ptr(), kind ? k_scale.data_ptr() : nullptr,
+                    kind ? v_scale.data_ptr() : nullptr, slots.data_ptr<int64_t>(), T, H, G, (int)q.stride(0),
+                    (int)k.stride(0), BS, kind, cur_stream());
 }
 
 // mask_size: -1 for plain decode rows, from 0 (plain causal) on for those of a block-local layer
@@ -578,9 +696,9 @@ extern "C" void launch_add_norm_rows(bf16_t* out, bf16_t* residual, const float*
                                      const bf16_t* table, const bf16_t* w, int S, int M, int n, int64_t vocab,
                                      float eps, int* unknown, int* clear, int clears, hipStream_t stream);
 extern "C" void launch_rope_store_rows(bf16_t* q_out, const float* part, const bf16_t* bias, const int64_t* positions,
-                                       const float* cos_sin, void* k_cache, void* v_cache, float* k_scale,
-                                       float* v_scale, const int64_t* slots, int S, int M, int H, int G,
-                                       int block_size, int fp8, hipStream_t stream);
+                                       const float* cos_sin, void* k_cache, void* v_cache, void* k_scale,
+                                       void* v_scale, const int64_t* slots, int S, int M, int H, int G,
+                                       int block_size, int kind, hipStream_t stream);
 extern "C" void launch_decode_inputs(int64_t* ids, int64_t* positions, int64_t* slots, int* ctx, int* tables,
                                      const int64_t* ids_in, const int64_t* positions_in, const int64_t* slots_in,
                                      const int* ctx_in, const int* tables_in, int B, int bs, int nb, int mb,
@@ -623,10 +741,10 @@ std::vector<torch::Tensor> embed_norm_rows(torch::Tensor ids, torch::Tensor tabl
 torch::Tensor rope_store_rows(torch::Tensor part, torch::Tensor bias, int64_t H, torch::Tensor positions,
                               torch::Tensor cos_sin, torch::Tensor k_cache, torch::Tensor v_cache,
                               torch::Tensor slots, torch::Tensor k_scale, torch::Tensor v_scale) {
-  CHECK_KV_CACHE(k_cache); CHECK_KV_CACHE(v_cache);
+  CHECK_ANY_CACHE(k_cache); CHECK_ANY_CACHE(v_cache);
   TORCH_CHECK(part.is_cuda() && part.is_contiguous() && part.scalar_type() == at::kFloat && part.dim() == 3);
   const int S = part.size(0), M = part.size(1), G = k_cache.size(1), BS = k_cache.size(2);
-  TORCH_CHECK(k_cache.size(3) == 128 && v_cache.sizes() == k_cache.sizes() &&
+  TORCH_CHECK(k_cache.size(3) == (k_cache.scalar_type() == at::kByte ? 64 : 128) && v_cache.sizes() == k_cache.sizes() &&
                   v_cache.scalar_type() == k_cache.scalar_type() && part.size(2) == (H + 2 * G) * 128 && S >= 1 &&
                   M >= 1, "rope_store_rows: sizes");
   TORCH_CHECK(positions.scalar_type() == at::kLong && positions.is_contiguous() && positions.numel() == M &&
@@ -635,8 +753,9 @@ torch::Tensor rope_store_rows(torch::Tensor part, torch::Tensor bias, int64_t H,
               "rope_store_rows: positions, slots or angles");
   TORCH_CHECK(bias.numel() == 0 || (bias.scalar_type() == at::kBFloat16 && bias.is_contiguous() &&
                                     bias.numel() == part.size(2)), "rope_store_rows: bias");
-  const int fp8 = k_cache.scalar_type() == at::kFloat8_e4m3fn ? 1 : 0;
-  if (fp8)
+  const int kind = cache_kind(k_cache);
+  if (kind == CACHE_KV4) check_kv4(k_cache, v_cache, k_scale, v_scale, part, "rope_store_rows");
+  if (kind == CACHE_FP8)
     TORCH_CHECK(k_scale.numel() == k_cache.size(0) * G * BS && k_scale.is_contiguous() &&
                     k_scale.scalar_type() == at::kFloat && v_scale.numel() == k_scale.numel() &&
                     v_scale.is_contiguous() && v_scale.scalar_type() == at::kFloat,
@@ -644,9 +763,9 @@ torch::Tensor rope_store_rows(torch::Tensor part, torch::Tensor bias, int64_t H,
   auto q = torch::empty({M, H, 128}, part.options().dtype(torch::kBFloat16));
   launch_rope_store_rows(bf(q), part.data_ptr<float>(), bias.numel() ? cbf(bias) : nullptr,
                          positions.data_ptr<int64_t>(), cos_sin.data_ptr<float>(), k_cache.data_ptr(),
-                         v_cache.data_ptr(), fp8 ? k_scale.data_ptr<float>() : nullptr,
-                         fp8 ? v_scale.data_ptr<float>() : nullptr, slots.data_ptr<int64_t>(), S, M, (int)H, G, BS,
-                         fp8, cur_stream());
+                         v_cache.data_ptr(), kind ? k_scale.data_ptr() : nullptr,
+                         kind ? v_scale.data_ptr() : nullptr, slots.data_ptr<int64_t>(), S, M, (int)H, G, BS,
+                         kind, cur_stream());
   return q;
 }
 
@@ -753,6 +872,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("rope_inplace", &rope_inplace);
   m.def("store_kv", &store_kv);
   m.def("rope_store", &rope_store);
+  m.def("load_kv4", &load_kv4);
+  m.def("attn_decode4", &attn_decode4, py::arg("q"), py::arg("k_cache"), py::arg("v_cache"), py::arg("block_tables"),
+        py::arg("context_lens"), py::arg("scale"), py::arg("k_scale"), py::arg("v_scale"), py::arg("arrived") = py::none(),
+        py::arg("into") = py::none());
+  m.def("attn_decode4_splits", &attn_decode4_splits);
   // workgroups of a context at most, by rows, kv heads, heads of each, positions of the table, fp8, block-local, counters
   m.def("attn_decode_splits", &attn_decode_splits);
   m.def("attn_decode_paged", &attn_decode_paged, py::arg("out"), py::arg("q"), py::arg("k_cache"),

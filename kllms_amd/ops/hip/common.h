@@ -12,6 +12,9 @@
 
 typedef __hip_bfloat16 bf16_t;
 
+// what a paged cache holds: bf16, e4m3 with a scale a row, 4 bits (kv4.h)
+enum { CACHE_BF16 = 0, CACHE_FP8 = 1, CACHE_KV4 = 2 };
+
 // 8 bf16 = 16 bytes: one dwordx4 load per lane (G13: always vectorize bf16).
 typedef short bf16x8_vec __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));

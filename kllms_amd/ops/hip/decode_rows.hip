@@ -16,7 +16,7 @@
 
 #include <type_traits>
 
-#include "common.h"
+#include "kv4.h"
 
 #define DR_THREADS 1024
 
@@ -136,13 +136,13 @@ extern "C" void launch_add_norm_rows(bf16_t* out, bf16_t* residual, const float*
 }
 
 // qkv sums [S, M, (H + 2G) * 128] (+ bias): q and k rotated (entry i with i + 64), q
-// out as bf16 rows, k and v into the paged cache - as bf16, or as e4m3 with a scale
-// per row (amax / 448 of the bf16 row). A wave per (row, head), two dims a lane.
-template <bool FP8>
+// out as bf16 rows, k and v into the paged cache - as bf16, as e4m3 with a scale
+// per row (amax / 448 of the bf16 row), or in 4 bits (kv4.h). A wave per (row, head), two dims a lane.
+template <int KIND>
 __global__ void __launch_bounds__(256) rope_store_rows_kernel(
     bf16_t* __restrict__ q_out, const float* __restrict__ part, const bf16_t* __restrict__ bias,
     const int64_t* __restrict__ positions, const float* __restrict__ cos_sin, void* __restrict__ k_cache,
-    void* __restrict__ v_cache, float* __restrict__ k_scale, float* __restrict__ v_scale,
+    void* __restrict__ v_cache, void* __restrict__ k_scale, void* __restrict__ v_scale,
     const int64_t* __restrict__ slots, int S, int M, int H, int G, int block_size) {
   const int m = blockIdx.y;
   const int lane = threadIdx.x & 63;
@@ -186,14 +186,24 @@ __global__ void __launch_bounds__(256) rope_store_rows_kernel(
   const bool is_k = head < H + G;
   const int g = head - H - (is_k ? 0 : G);
   const int64_t row = ((slot / block_size) * G + g) * block_size + slot % block_size;
-  if constexpr (FP8) {
+  if constexpr (KIND == CACHE_KV4) {
+    // the halves of a row are its groups; word n is of the lanes n, n + 16, n + 32, n + 48
+    const float x = bf16_to_f32(lo), y = bf16_to_f32(hi);
+    const Kv4Group ga(-wave_reduce_max(-x), wave_reduce_max(x), __ballot(x != x) == 0);
+    const Kv4Group gb(-wave_reduce_max(-y), wave_reduce_max(y), __ballot(y != y) == 0);
+    uint32_t w = (ga.code(x) | gb.code(y) << 8) << (4 * ((lane >> 5) + 4 * (lane >> 4 & 1)));
+    w |= __shfl_xor(w, 16);
+    w |= __shfl_xor(w, 32);
+    if (lane < 16) ((uint32_t*)(is_k ? k_cache : v_cache))[row * (KV4_BYTES / 4) + lane] = w;
+    if (lane < KV4_GROUPS) ((uint32_t*)(is_k ? k_scale : v_scale))[row * KV4_GROUPS + lane] = lane ? gb.word() : ga.word();
+  } else if constexpr (KIND == CACHE_FP8) {
     const float x = bf16_to_f32(lo), y = bf16_to_f32(hi);
     const float sc = fmaxf(wave_reduce_max(fmaxf(fabsf(x), fabsf(y))) * (1.0f / 448.0f), 1e-8f);
     const float inv = 1.0f / sc;
     unsigned char* o = (unsigned char*)(is_k ? k_cache : v_cache) + row * 128;
     o[lane] = f32_to_fp8(x * inv);
     o[lane + 64] = f32_to_fp8(y * inv);
-    if (lane == 0) (is_k ? k_scale : v_scale)[row] = sc;
+    if (lane == 0) ((float*)(is_k ? k_scale : v_scale))[row] = sc;
   } else {
     short* o = (short*)(is_k ? k_cache : v_cache) + row * 128;
     o[lane] = lo;
@@ -202,16 +212,14 @@ __global__ void __launch_bounds__(256) rope_store_rows_kernel(
 }
 
 extern "C" void launch_rope_store_rows(bf16_t* q_out, const float* part, const bf16_t* bias, const int64_t* positions,
-                                       const float* cos_sin, void* k_cache, void* v_cache, float* k_scale,
-                                       float* v_scale, const int64_t* slots, int S, int M, int H, int G,
-                                       int block_size, int fp8, hipStream_t stream) {
-  const dim3 grid((H + 2 * G + 3) / 4, M);
-  if (fp8)
-    hipLaunchKernelGGL(rope_store_rows_kernel<true>, grid, dim3(256), 0, stream, q_out, part, bias, positions,
-                       cos_sin, k_cache, v_cache, k_scale, v_scale, slots, S, M, H, G, block_size);
-  else
-    hipLaunchKernelGGL(rope_store_rows_kernel<false>, grid, dim3(256), 0, stream, q_out, part, bias, positions,
-                       cos_sin, k_cache, v_cache, k_scale, v_scale, slots, S, M, H, G, block_size);
+                                       const float* cos_sin, void* k_cache, void* v_cache, void* k_scale,
+                                       void* v_scale, const int64_t* slots, int S, int M, int H, int G,
+                                       int block_size, int kind, hipStream_t stream) {
+  hipLaunchKernelGGL(kind == CACHE_KV4   ? rope_store_rows_kernel<CACHE_KV4>
+                     : kind == CACHE_FP8 ? rope_store_rows_kernel<CACHE_FP8>
+                                         : rope_store_rows_kernel<CACHE_BF16>,
+                     dim3((H + 2 * G + 3) / 4, M), dim3(256), 0, stream, q_out, part, bias, positions, cos_sin, k_cache, v_cache,
+                     k_scale, v_scale, slots, S, M, H, G, block_size);
 }
 
 // Inputs of a captured decode step, in one launch (twelve copies and fills otherwise):

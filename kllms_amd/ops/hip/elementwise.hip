@@ -6,7 +6,7 @@
 // RoPE precomputed on host — Appendix B: on-device trig turns memory-bound
 // into VALU-bound).
 
-#include "common.h"
+#include "kv4.h"
 
 // --------------------------------------------------------------------------
 // RMSNorm: one block per row, row length N (multiple of 8), bf16 in/out.
@@ -217,17 +217,17 @@ extern "C" __global__ void __launch_bounds__(256) store_kv_fp8_kernel(
 
 // --------------------------------------------------------------------------
 // RoPE and cache store of whole rows in one pass (head size 128): q and k rotated in
-// place (entry i with i + 64, as rope_kernel), k and v into the paged cache as bf16 or as
-// e4m3 with a scale per row (as store_kv_fp8_kernel). A thread holds entries c..c+7 and
+// place (entry i with i + 64, as rope_kernel), k and v into the paged cache as bf16, as
+// e4m3 with a scale per row (as store_kv_fp8_kernel) or in 4 bits (kv4.h). A thread holds entries c..c+7 and
 // c+64..c+71 of a head: 16-byte accesses throughout, where a rotation of 2-byte accesses
 // with a workgroup per head and the store behind it took 132 us for 12000 rows of 48
 // heads and this takes 50 (320 MB, 6.4 TB/s).
 // --------------------------------------------------------------------------
-template <bool FP8>
+template <int KIND>
 __global__ void __launch_bounds__(256) rope_store_kernel(
     bf16_t* __restrict__ q, bf16_t* __restrict__ k, const bf16_t* __restrict__ v,
     const int64_t* __restrict__ positions, const float* __restrict__ cos_sin, void* __restrict__ k_cache,
-    void* __restrict__ v_cache, float* __restrict__ k_scale, float* __restrict__ v_scale,
+    void* __restrict__ v_cache, void* __restrict__ k_scale, void* __restrict__ v_scale,
     const int64_t* __restrict__ slots, int64_t n, int H, int G, int q_stride, int kv_stride, int block_size) {
   const int heads = H + 2 * G;
   for (int64_t idx = (int64_t)blockIdx.x * 256 + threadIdx.x; idx < n; idx += (int64_t)gridDim.x * 256) {
@@ -258,7 +258,10 @@ __global__ void __launch_bounds__(256) rope_store_kernel(
     const int g = head - H - (is_v ? G : 0);
     const int64_t slot = slots[t];
     const int64_t at = ((slot / block_size) * G + g) * block_size + slot % block_size;
-    if constexpr (FP8) {
+    if constexpr (KIND == CACHE_KV4) {
+      kv4_store_row((uint32_t*)(is_v ? v_cache : k_cache) + at * (KV4_BYTES / 4), (uint32_t*)(is_v ? v_scale : k_scale) + at * KV4_GROUPS,
+                    piece, a, b);
+    } else if constexpr (KIND == CACHE_FP8) {
       float amax = 0.0f;
 #pragma unroll
       for (int j = 0; j < 8; ++j)
@@ -275,7 +278,7 @@ __global__ void __launch_bounds__(256) rope_store_kernel(
       unsigned char* o = (unsigned char*)(is_v ? v_cache : k_cache) + at * 128 + piece * 8;
       *reinterpret_cast<u8x8_vec*>(o) = lo;
       *reinterpret_cast<u8x8_vec*>(o + 64) = hi;
-      if (piece == 0) (is_v ? v_scale : k_scale)[at] = sc;
+      if (piece == 0) ((float*)(is_v ? v_scale : k_scale))[at] = sc;
     } else {
       short* o = (short*)(is_v ? v_cache : k_cache) + at * 128 + piece * 8;
       *reinterpret_cast<bf16x8_vec*>(o) = a;
@@ -285,16 +288,15 @@ __global__ void __launch_bounds__(256) rope_store_kernel(
 }
 
 extern "C" void launch_rope_store(bf16_t* q, bf16_t* k, const bf16_t* v, const int64_t* positions,
-                                  const float* cos_sin, void* k_cache, void* v_cache, float* k_scale, float* v_scale,
+                                  const float* cos_sin, void* k_cache, void* v_cache, void* k_scale, void* v_scale,
                                   const int64_t* slots, int T, int H, int G, int q_stride, int kv_stride,
-                                  int block_size, int fp8, hipStream_t stream) {
+                                  int block_size, int kind, hipStream_t stream) {
   const int64_t n = (int64_t)T * (H + 2 * G) * 8;
   const int64_t blocks = (n + 255) / 256;
   const dim3 grid((unsigned)(blocks < 16384 ? blocks : 16384));
-  if (fp8)
-    hipLaunchKernelGGL(rope_store_kernel<true>, grid, dim3(256), 0, stream, q, k, v, positions, cos_sin, k_cache,
-                       v_cache, k_scale, v_scale, slots, n, H, G, q_stride, kv_stride, block_size);
-  else
-    hipLaunchKernelGGL(rope_store_kernel<false>, grid, dim3(256), 0, stream, q, k, v, positions, cos_sin, k_cache,
-                       v_cache, k_scale, v_scale, slots, n, H, G, q_stride, kv_stride, block_size);
+  hipLaunchKernelGGL(kind == CACHE_KV4   ? rope_store_kernel<CACHE_KV4>
+                     : kind == CACHE_FP8 ? rope_store_kernel<CACHE_FP8>
+                                         : rope_store_kernel<CACHE_BF16>,
+                     grid, dim3(256), 0, stream, q, k, v, positions, cos_sin, k_cache, v_cache, k_scale, v_scale, slots, n, H, G,
+                     q_stride, kv_stride, block_size);
 }

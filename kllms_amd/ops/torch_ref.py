@@ -94,6 +94,60 @@ def silu_mul(gate: torch.Tensor, up: torch.Tensor) -> torch.Tensor:
 
 # --- paged KV cache -----------------------------------------------------------
 
+KV4_GROUP = 64
+_KV4_LEAST_STEP = torch.finfo(torch.float32).tiny
+
+
+def kv4_groups(head_dim: int) -> int:
+    """Groups of a row of the 4-bit cache: runs of 64 values, or the whole of a shorter row."""
+    if head_dim % 8 or (head_dim > KV4_GROUP and head_dim % KV4_GROUP):
+        raise ValueError(f"a 4-bit cache holds rows of a multiple of 64 values, or of up to 64 in eights: got {head_dim}")
+    return max(1, head_dim // KV4_GROUP)
+
+
+def kv4_quantize(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Rows x [..., D] in 4 bits: (codes uint8 [..., D / 2], scales bf16 [..., groups, 2]).
+
+    A group's scales are its step, (most - least) / 15, and its least value; a value is the whole number of steps above
+    the least one, to the nearest, halves to even. Rows are taken as bf16, of which the least value is exact. A group
+    with a value that is no finite number, or whose range is none, is NaN as a whole. A row's D / 8 words of 32 bits
+    (little-endian): nibble p of word n is value D / 4 (p mod 4) + D / 8 (p div 4) + n."""
+    D = x.shape[-1]
+    g = x.to(torch.bfloat16).float().unflatten(-1, (kv4_groups(D), -1))
+    least, most = g.amin(-1, keepdim=True), g.amax(-1, keepdim=True)
+    step = ((most - least) / 15).to(torch.bfloat16).float()
+    step = torch.where(step >= _KV4_LEAST_STEP, step, torch.zeros_like(step))
+    n = torch.where(step > 0, torch.round((g - least) / step), torch.zeros_like(g))
+    fine = torch.isfinite(most - least)
+    none = torch.full_like(step, float("nan"))
+    n = torch.where(fine, n.clamp(0, 15), torch.zeros_like(n)).flatten(-2).to(torch.uint8)
+    scales = torch.cat((torch.where(fine, step, none), torch.where(fine, least, none)), -1).to(torch.bfloat16)
+    n = n.unflatten(-1, (4, 2, D // 8)).movedim(-1, -3).transpose(-1, -2).flatten(-2)     # [word, nibble 4 h + a]
+    return (n[..., 0::2] | (n[..., 1::2] << 4)).flatten(-2), scales
+
+
+def kv4_values(codes: torch.Tensor, scales: torch.Tensor) -> torch.Tensor:
+    """What rows of the 4-bit cache stand for, fp32 [..., D]: code * step + least."""
+    D = codes.shape[-1] * 2
+    n = torch.stack((codes & 15, codes >> 4), -1).unflatten(-2, (D // 8, 4)).flatten(-2)  # [word, nibble]
+    n = n.unflatten(-1, (2, 4)).movedim(-3, -1).transpose(-2, -3).flatten(-3).float()
+    s = scales.float()
+    return (n.unflatten(-1, (scales.shape[-2], -1)) * s[..., :1] + s[..., 1:]).flatten(-2)
+
+
+def load_kv(k_cache, v_cache, slots, k_scale, v_scale):
+    """Rows of the 4-bit caches at flat slots by value, bf16 [T, KVH, D]; NaN for slots outside the cache."""
+    NB, _, BS, _ = k_cache.shape
+    known = (slots >= 0) & (slots < NB * BS)
+    at = torch.where(known, slots, torch.zeros_like(slots))
+    blk, off = at // BS, at % BS
+    out = []
+    for cache, scale in ((k_cache, k_scale), (v_cache, v_scale)):
+        rows = kv4_values(cache[blk, :, off], scale[blk, :, off])
+        out.append(torch.where(known[:, None, None], rows, torch.full_like(rows, float("nan"))).to(torch.bfloat16))
+    return tuple(out)
+
+
 def store_kv(
     k: torch.Tensor,
     v: torch.Tensor,
@@ -109,8 +163,18 @@ def store_kv(
     fp8 caches with k_scale/v_scale ([NB, KVH, BS] fp32): each (token, head)
     row is quantized with its OWN scale s = max(amax(|row|)/448, 1e-8), the
     scale written alongside — outlier rows no longer saturate e4m3.
+    4-bit caches (uint8 [NB, KVH, BS, D / 2]) with k_scale/v_scale bf16
+    [NB, KVH, BS, groups, 2]: kv4_quantize; rows of slots outside the cache
+    go nowhere.
     """
     num_blocks, kv_heads, block_size, head_dim = k_cache.shape
+    if k_cache.dtype == torch.uint8:
+        known = (slot_mapping >= 0) & (slot_mapping < num_blocks * block_size)
+        at = slot_mapping[known]
+        blk, off = at // block_size, at % block_size
+        for rows, cache, scale in ((k, k_cache, k_scale), (v, v_cache, v_scale)):
+            cache[blk, :, off], scale[blk, :, off] = kv4_quantize(rows[known])
+        return
     blk = slot_mapping // block_size
     off = slot_mapping % block_size
     if k_scale is not None:
@@ -169,8 +233,9 @@ def attn_decode_paged(
 
     q: [B, H, D]; caches [num_blocks, KVH, block_size, D];
     block_tables: [B, max_blocks] int32; context_lens: [B] (length INCLUDING
-    the token being decoded, whose K/V are already stored). k_scale/v_scale
-    ([NB, KVH, BS] fp32, fp8 caches only): per-row dequant multipliers.
+    the token being decoded, whose K/V are already stored). k_scale/v_scale:
+    of fp8 caches [NB, KVH, BS] fp32 per-row dequant multipliers, of 4-bit
+    caches (uint8) the groups' steps and least values (kv4_quantize).
     """
     B, H, D = q.shape
     _, KVH, BS, _ = k_cache.shape
@@ -180,6 +245,13 @@ def attn_decode_paged(
         L = int(context_lens[b])
         nblk = (L + BS - 1) // BS
         blocks = block_tables[b, :nblk].long()
+        if k_cache.dtype == torch.uint8:
+            kk, vv = (kv4_values(c[blocks], s[blocks]).permute(1, 0, 2, 3).reshape(KVH, nblk * BS, D)[:, :L]
+                      for c, s in ((k_cache, k_scale), (v_cache, v_scale)))
+            rows = q[b].float().view(KVH, rep, D)
+            p = torch.softmax(rows @ kk.transpose(1, 2) * scale, dim=-1)
+            out[b] = (p @ vv).view(H, D).to(q.dtype)
+            continue
         kk = k_cache[blocks].permute(1, 0, 2, 3).reshape(KVH, nblk * BS, D)[:, :L].float()
         vv = v_cache[blocks].permute(1, 0, 2, 3).reshape(KVH, nblk * BS, D)[:, :L].float()
         if k_scale is not None:

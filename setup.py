@@ -24,6 +24,8 @@ SOURCES = [
         "bindings.hip",
         "elementwise.hip",
         "attn_decode.hip",
+        "attn_decode4.hip",
+        "kv4_rows.hip",
         "attn_prefill.hip",
         "sampling.hip",
         "mfma_selftest.hip",

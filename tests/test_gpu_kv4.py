@@ -1,0 +1,284 @@
+"""Kernels of the 4-bit cache against float64."""
+
+import pytest
+import torch
+
+from kllms_amd import ops
+from kllms_amd.ops import torch_ref
+
+from kv4_oracle import attention64, values64
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+D = 128
+
+
+def rows(*shape, seed=0, spread=0.0):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(*shape, generator=g)
+    if spread:
+        x = x * torch.exp2(torch.randn(*shape[:-1], 1, generator=g) * spread)
+    return x.bfloat16()
+
+
+def special_rows(T, G, seed):
+    x = rows(T, G, D, seed=seed, spread=4.0)
+    if T >= 6:
+        x[0] = 1.5
+        x[1, 0, 3] = float("nan")
+        x[2, 0, 100] = float("-inf")
+        x[3, 0, :64] = 0
+        x[4, 0, 1], x[4, 0, 2] = 3e38, -3e38
+        x[5] = x[5] * 1e-39
+    return x
+
+
+@pytest.mark.parametrize("T,G,BS", [(1, 1, 1), (7, 3, 5), (120, 8, 16), (2049, 2, 32)])
+def test_store_and_load(T, G, BS):
+    NB = -(-T // BS) + 3
+    k, v = special_rows(T, G, 1), special_rows(T, G, 2)
+    wide = torch.cat((k, v, k), 1).to(DEV)                        # rows of a fused projection
+    slots = torch.randperm(NB * BS)[:T]
+    g = torch.Generator().manual_seed(3)
+    caches = [torch.randint(0, 256, (NB, G, BS, D // 2), dtype=torch.uint8, generator=g) for _ in range(2)]
+    scales = [torch.randn(NB, G, BS, 2, 2, generator=g).bfloat16() for _ in range(2)]
+    dev = [t.to(DEV) for t in caches + scales]
+    ops.store_kv(wide[:, :G], wide[:, G:2 * G], dev[0], dev[1], slots.to(DEV), dev[2], dev[3])
+    torch_ref.store_kv(k, v, *caches, slots, *scales)
+    for got, want in zip(dev, caches + scales):                   # also the rows that nobody wrote
+        assert torch.equal(got.cpu().view(torch.uint8), want.view(torch.uint8)) if got.dtype == torch.uint8 else \
+            torch.equal(got.cpu().float().nan_to_num(7e37), want.float().nan_to_num(7e37))
+    slots[0] = NB * BS                                            # outside: loads NaN
+    for got, want in zip(ops.load_kv(*dev[:2], slots.to(DEV), *dev[2:]), torch_ref.load_kv(*caches, slots, *scales)):
+        assert torch.equal(got.cpu().float().nan_to_num(7e37), want.float().nan_to_num(7e37))
+
+
+def test_rows_for_no_slot_go_nowhere_and_odd_rows_are_taken():
+    T, G, BS, NB = 5, 2, 4, 3
+    base = torch.randn(T, 3 * G * D + 1).bfloat16().to(DEV)
+    k = base[:, 1:1 + G * D].unflatten(1, (G, D))                 # rows off 16 bytes, an odd stride
+    v = torch.randn(T, G, D).bfloat16().to(DEV)
+    kc, vc = (torch.zeros(NB, G, BS, D // 2, dtype=torch.uint8, device=DEV) for _ in range(2))
+    ks, vs = (torch.zeros(NB, G, BS, 2, 2, dtype=torch.bfloat16, device=DEV) for _ in range(2))
+    slots = torch.tensor([2, -1, NB * BS, 7, 1 << 40], device=DEV)
+    ops.store_kv(k, v, kc, vc, slots, ks, vs)
+    a, b = ops.load_kv(kc, vc, slots, ks, vs)
+    for got, x in ((a, k), (b, v)):
+        assert torch.equal(got[[0, 3]].cpu(), torch_ref.kv4_values(*torch_ref.kv4_quantize(x.cpu()[[0, 3]])).bfloat16())
+    assert int((ks != 0).sum()) == 2 * G * 4 and int((kc.view(NB, G, BS, -1) != 0).any(-1).sum()) == 2 * G
+
+
+@pytest.mark.parametrize("T,H,G,BS", [(1, 4, 1, 16), (33, 32, 8, 16), (300, 8, 4, 5)])
+def test_rope_store(T, H, G, BS):
+    NB = -(-T // BS) + 2
+    qkv = special_rows(T, H + 2 * G, 5).to(DEV)
+    qkv[:, :H] = rows(T, H, D, seed=6).to(DEV)
+    qkv[:, H:H + G] = rows(T, G, D, seed=7).to(DEV)               # what is turned is finite; values are what they are
+    cos_sin = torch_ref.build_cos_sin_cache(D, 4096, 1e4, "cpu").to(DEV)
+    pos = torch.randint(0, 4096, (T,), device=DEV)
+    slots = torch.randperm(NB * BS, device=DEV)[:T]
+
+    def caches():
+        return [torch.zeros(NB, G, BS, D // 2, dtype=torch.uint8, device=DEV) for _ in range(2)] + \
+            [torch.zeros(NB, G, BS, 2, 2, dtype=torch.bfloat16, device=DEV) for _ in range(2)]
+
+    def same(x, y):
+        return all(torch.equal(s.float().nan_to_num(7e37), t.float().nan_to_num(7e37)) for s, t in zip(x, y))
+
+    for at in (pos, pos * 0):
+        one, two = qkv.clone(), qkv.clone()
+        a, b = caches(), caches()
+        ops.rope_store(*one.split([H, G, G], 1), at, cos_sin, a[0], a[1], slots, a[2], a[3])
+        torch_ref.rope_inplace(two[:, :H], two[:, H:H + G], at, cos_sin)
+        # a product and a sum of it rounded to bf16 from fp32: of neighbouring values at most, where one lies between
+        assert torch.allclose(one.float(), two.float(), rtol=2 ** -7, atol=2 ** -20, equal_nan=True)
+        ops.store_kv(one[:, H:H + G], one[:, H + G:], b[0], b[1], slots, b[2], b[3])
+        assert same(a, b)
+    # a decode step's form, from sums in two shares; at position 0, where turning rounds nothing
+    c = caches()
+    flat = qkv.view(1, T, -1).float()
+    part = torch.cat((flat * 0.5, flat * 0.5)).contiguous()
+    got = ops.rope_store_rows(part, None, H, pos * 0, cos_sin, c[0], c[1], slots, c[2], c[3])
+    assert torch.equal(got, one[:, :H]) and same(a, c)
+
+
+def case(ctx, gqa, KVH, BS, seed=0, width=None, shared=0, spread=0.0, behind=True):
+    """q, caches, scales, tables, lengths; what lies behind a context is another's: any codes, scales that are none."""
+    g = torch.Generator().manual_seed(seed)
+    B = len(ctx)
+    need = [max(1, -(-c // BS)) for c in ctx]
+    NB = sum(need) + 2
+    perm = torch.randperm(NB, generator=g).tolist()
+    tables = torch.zeros(B, width or max(need), dtype=torch.int32)
+    kc, vc = (torch.randint(0, 256, (NB, KVH, BS, D // 2), dtype=torch.uint8, generator=g) for _ in range(2))
+    ks, vs = (torch.full((NB, KVH, BS, 2, 2), float("nan") if behind else 0.0).bfloat16() for _ in range(2))
+    if behind:
+        ks[::2], vs[::2] = float("inf"), 3e38
+    for b in range(B):
+        own = [perm.pop() for _ in range(need[b])]
+        if b and shared:
+            n = min(shared, min(ctx[0], ctx[b]) // BS)
+            own[:n] = tables[0, :n].tolist()
+        tables[b, :need[b]] = torch.tensor(own, dtype=torch.int32)
+    for b in range(B):
+        at = torch.arange(ctx[b])
+        blk, off = tables[b].long()[at // BS], at % BS
+        for i, (cache, scale) in enumerate(((kc, ks), (vc, vs))):
+            cache[blk, :, off], scale[blk, :, off] = torch_ref.kv4_quantize(rows(ctx[b], KVH, D, seed=seed * 7 + 2 * b + i, spread=spread))
+    return rows(B, KVH * gqa, D, seed=seed + 99), kc, vc, ks, vs, tables, torch.tensor(ctx, dtype=torch.int32)
+
+
+def check(out, q, kc, vc, ks, vs, tables, n, scale):
+    want, off = attention64(q, kc, vc, ks, vs, tables, n, scale)
+    far = (out.double().cpu() - want).abs()
+    assert bool((far <= off).all()), f"{float((far / off).max())} of what is allowed, at {torch.nonzero(far > off)[:3].tolist()}"
+
+
+def both(q, kc, vc, ks, vs, tables, n, scale):
+    """The result, the same with counters and without."""
+    dev = [t.to(DEV) for t in (q, kc, vc, tables, n, ks, vs)]
+    q, kc, vc, tables, n, ks, vs = dev
+    out = ops.attn_decode_paged(q, kc, vc, tables, n, scale, ks, vs)
+    arrived = torch.zeros(q.shape[0] * kc.shape[1] * ops.ATTN_COUNTER_GAP, dtype=torch.int32, device=DEV)
+    joined = ops.attn_decode_paged(q, kc, vc, tables, n, scale, ks, vs, arrived)
+    assert torch.equal(joined.nan_to_num(7e37), out.nan_to_num(7e37))
+    assert not bool(arrived.any())
+    return out
+
+
+@pytest.mark.parametrize("gqa,KVH,BS", [(1, 2, 16), (2, 1, 8), (4, 8, 16), (8, 2, 32), (4, 3, 5), (1, 1, 1), (2, 2, 48), (8, 1, 7)])
+@pytest.mark.parametrize("ctx,width", [
+    ([1], None), ([0, 1, 15, 16, 17], None), ([63, 64, 65, 0], None), ([255, 256, 257, 1000], None),
+    ([1, 1000, 300, 17], 256),                        # a table much wider than the contexts
+    ([700 - 13 * i for i in range(30)], None),        # several tiles for a wave
+])
+def test_decode(gqa, KVH, BS, ctx, width):
+    args = case(ctx, gqa, KVH, BS, seed=gqa + BS + len(ctx), width=width and width * 16 // BS + 1, shared=3)
+    check(both(*args, D ** -0.5), *args, D ** -0.5)
+
+
+@pytest.mark.parametrize("gqa,KVH,BS", [(4, 8, 16), (8, 1, 16), (1, 2, 6), (2, 1, 32)])
+def test_long_contexts_in_shares(gqa, KVH, BS):
+    args = case([9000, 5], gqa, KVH, BS, seed=gqa)
+    check(both(*args, D ** -0.5), *args, D ** -0.5)
+
+
+@pytest.mark.parametrize("gqa", [1, 2, 4, 8])
+@pytest.mark.parametrize("spread", [3.0, 20.0])
+def test_steps_and_scores_of_very_different_sizes(gqa, spread):
+    """Rows of 2^-60 to 2^60: the running max and the steps' common power are renewed again and again."""
+    q, kc, vc, ks, vs, tables, n = case([500, 129, 64], gqa, 2, 16, seed=gqa, spread=spread)
+    scale = 2.0 ** (-3.5 - spread)
+    check(both(q, kc, vc, ks, vs, tables, n, scale), q, kc, vc, ks, vs, tables, n, scale)
+
+
+@pytest.mark.parametrize("gqa", [1, 4])
+def test_rising_scores_and_rising_steps(gqa):
+    q, kc, vc, ks, vs, tables, n = case([640], gqa, 1, 16, seed=3)
+    at = torch.arange(640)
+    blk, off = tables[0].long()[at // 16], at % 16
+    up = torch.exp2(at / 40.0)[:, None, None]
+    kc[blk, :, off], ks[blk, :, off] = torch_ref.kv4_quantize(q[0, :1].float() * up / 2048)
+    vc[blk, :, off], vs[blk, :, off] = torch_ref.kv4_quantize(rows(640, 1, D, seed=5).float() * up)
+    check(both(q, kc, vc, ks, vs, tables, n, 0.1), q, kc, vc, ks, vs, tables, n, 0.1)
+
+
+def test_queries_of_any_size_scales_of_any_sign():
+    q, kc, vc, ks, vs, tables, n = case([100, 100, 100, 100], 4, 2, 16, seed=11)
+    q[0] = 0
+    q[1] = (q[1].float() * 2.0 ** 100).bfloat16()
+    q[2] = (q[2].float() * 2.0 ** -100).bfloat16()
+    scale = torch.tensor([1.0, 2.0 ** -104, 2.0 ** 96, -0.2])
+    for b in range(4):
+        one = (q[b:b + 1], kc, vc, ks, vs, tables[b:b + 1], n[b:b + 1])
+        check(both(*one, float(scale[b])), *one, float(scale[b]))
+
+
+def test_a_row_that_is_no_number_is_its_groups_alone():
+    q, kc, vc, ks, vs, tables, n = case([70, 200], 4, 2, 16, seed=12)
+    blk, off = int(tables[1, 3]), 5
+    vs[blk, 1, off, 1] = float("nan")                 # of kv head 1, values 64 to 127
+    out = both(q, kc, vc, ks, vs, tables, n, 0.1).cpu()
+    bad = torch.isnan(out)
+    assert bool(bad[1, 4:, 64:].all()) and int(bad.sum()) == 4 * 64
+    ks[blk, 0, off, 0] = float("nan")                 # a key: all of its heads
+    out = both(q, kc, vc, ks, vs, tables, n, 0.1).cpu()
+    assert bool(torch.isnan(out[1, :4]).all()) and int(torch.isnan(out).sum()) == 4 * 64 + 4 * 128
+
+
+def test_strided_queries_and_empty_calls():
+    q, kc, vc, ks, vs, tables, n = (t.to(DEV) for t in case([33, 65, 7], 4, 2, 16, seed=13))
+    want = ops.attn_decode_paged(q, kc, vc, tables, n, 0.1, ks, vs)
+    wide = torch.cat((q, q), 1)
+    assert torch.equal(ops.attn_decode_paged(wide[:, 8:], kc, vc, tables, n, 0.1, ks, vs), want)
+    odd = torch.empty(3 * 8 * D + 1, dtype=torch.bfloat16, device=DEV)[1:].view(3, 8, D).copy_(q)
+    assert torch.equal(ops.attn_decode_paged(odd, kc, vc, tables, n, 0.1, ks, vs), want)
+    assert ops.attn_decode_paged(q[:0], kc, vc, tables[:0], n[:0], 0.1, ks, vs).shape == (0, 8, D)
+    assert not bool(ops.attn_decode_paged(q, kc, vc, tables[:, :0].contiguous(), n * 0, 0.1, ks, vs).any())
+    assert not bool(ops.attn_decode_paged(q, kc, vc, tables, n * 0, 0.1, ks, vs).any())
+
+
+def test_caches_of_more_than_2_gb():
+    KVH, BS, NB = 8, 16, 300000                       # 2.5 GB of codes
+    q, kc, vc, ks, vs, tables, n = case([300], 4, KVH, BS, seed=14)
+    big = [torch.zeros(NB, *t.shape[1:], dtype=t.dtype, device=DEV) for t in (kc, vc, ks, vs)]
+    far = torch.arange(NB - kc.shape[0], NB)
+    for t, small in zip(big, (kc, vc, ks, vs)):
+        t[far[0]:] = small.to(DEV)
+    moved = (tables.long() + far[0]).int()
+    want = both(q, kc, vc, ks, vs, tables, n, 0.1)
+    out = ops.attn_decode_paged(q.to(DEV), big[0], big[1], moved.to(DEV), n.to(DEV), 0.1, big[2], big[3])
+    assert torch.equal(out, want)
+    slots = torch.tensor([NB * BS - 1, (NB - 5) * BS], device=DEV)
+    new = rows(2, KVH, D, seed=15).to(DEV)
+    ops.store_kv(new, new, big[0], big[1], slots, big[2], big[3])
+    a, b = ops.load_kv(big[0], big[1], slots, big[2], big[3])
+    assert torch.equal(a, b) and torch.equal(a.cpu(), torch_ref.kv4_values(*torch_ref.kv4_quantize(new.cpu())).bfloat16())
+
+
+def test_replayed_and_on_another_stream():
+    """Captured with the store, replayed with other work between; two graphs of one cache."""
+    q, kc, vc, ks, vs, tables, n = (t.to(DEV) for t in case([700, 20], 4, 2, 16, seed=16))
+    k_new, v_new = rows(2, 2, D, seed=17).to(DEV), rows(2, 2, D, seed=18).to(DEV)
+    slots = torch.stack([tables[b, (n[b] - 1) // 16].long() * 16 + (n[b] - 1) % 16 for b in range(2)])
+    arrived = torch.zeros(4, dtype=torch.int32, device=DEV)
+
+    def step():
+        ops.store_kv(k_new, v_new, kc, vc, slots, ks, vs)
+        return ops.attn_decode_paged(q, kc, vc, tables, n, 0.1, ks, vs, arrived)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graphs = []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = step()
+        graphs.append((g, out))
+    for i in range(4):
+        k_new.copy_(rows(2, 2, D, seed=20 + i))
+        q.copy_(rows(2, 8, D, seed=40 + i))
+        want = step().clone()
+        for g, out in graphs:
+            out.zero_()
+            g.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, want)
+
+
+def test_refusals():
+    q, kc, vc, ks, vs, tables, n = (t.to(DEV) for t in case([20], 4, 2, 16, seed=21))
+    call = lambda **o: ops.attn_decode_paged(*[o.get(k, v) for k, v in dict(q=q, kc=kc, vc=vc, tables=tables, n=n, scale=0.1, ks=ks, vs=vs).items()])
+    call()
+    for bad in (dict(ks=ks.float()), dict(vs=vs[:, :, :, :1].contiguous()), dict(kc=kc[..., :32].contiguous()), dict(tables=tables.long()),
+                dict(n=n.long()), dict(q=q.float()), dict(q=q[:, :6].contiguous()), dict(q=q[:, :, :64].contiguous()),
+                dict(kc=kc.transpose(1, 2)), dict(tables=tables.cpu()), dict(n=torch.cat((n, n))), dict(vc=vc[:1])):
+        with pytest.raises(RuntimeError):
+            call(**bad)
+    new, slots = rows(1, 2, D).to(DEV), torch.zeros(1, dtype=torch.long, device=DEV)
+    for bad in (dict(slots=slots.int()), dict(k=new.float()), dict(k=new[:, :1]), dict(ks=ks.float()), dict(slots=torch.zeros(2, dtype=torch.long, device=DEV))):
+        with pytest.raises(RuntimeError):
+            ops.store_kv(bad.get("k", new), new, kc, vc, bad.get("slots", slots), bad.get("ks", ks), vs)
