@@ -1155,8 +1155,10 @@ class EngineConfig(BaseModel):
     # traffic/footprint; OCP e4m3 with PER-ROW dequant scales — each
     # (token, head) row is stored as x/s with s = amax(|row|)/448 kept in a
     # parallel fp32 [NB, KVH, BS] tensor (~3% overhead), so outlier-heavy
-    # real checkpoints don't saturate e4m3's +-448 range)
-    kv_cache_dtype: Literal["bf16", "fp8_e4m3"] = "bf16"
+    # real checkpoints don't saturate e4m3's +-448 range), or "int4" (0.28 of
+    # the bf16 footprint: whole steps above the least value of each group of 64
+    # values, both kept in bf16; dense and mixture models, head size 128 on the GPU)
+    kv_cache_dtype: Literal["bf16", "fp8_e4m3", "int4"] = "bf16"
     # Fraction of free HBM given to the KV cache after weights are resident
     kv_memory_fraction: float = 0.70
     max_kv_blocks: Optional[int] = None  # explicit cap (used on CPU/tests)

@@ -22,6 +22,7 @@ import torch
 
 from ..models.llama import ForwardBatch
 from .config import EngineConfig, ModelArchConfig
+from ..ops.torch_ref import kv4_groups
 from .kvcache import PagedKVCache, SequenceKV
 from .sampling import SamplingParams
 from .tokenizer import BaseTokenizer, load_tokenizer
@@ -282,6 +283,8 @@ class LLMEngine:
 
     def _build_kv_cache(self) -> PagedKVCache:
         if self.stateful:
+            if self.config.kv_cache_dtype == "int4":
+                raise ValueError(f"kv_cache_dtype='int4' needs a model whose layers all keep plain keys and values: {self.arch.arch} does not")
             return self._build_state_cache()
         a = self.arch
         tp = self.ctx.world_size
@@ -292,8 +295,16 @@ class LLMEngine:
             elem = 1
             # per-row fp32 dequant scale sidecar: 4 B per (head_dim) row
             scale_bytes = 2 * a.num_layers * kv_heads_local * self.config.kv_block_size * 4
+        elif self.config.kv_cache_dtype == "int4":
+            if self.device.type == "cuda" and (a.head_dim_ != 128 or a.num_heads // a.num_kv_heads not in (1, 2, 4, 8)):
+                raise ValueError("kv_cache_dtype='int4' needs head size 128 and 1, 2, 4 or 8 heads to a kv head on the GPU: "
+                                 f"the model has {a.head_dim_} and {a.num_heads} to {a.num_kv_heads}")
+            elem = 0.5
+            # a bf16 step and least value for each group
+            scale_bytes = 2 * a.num_layers * kv_heads_local * self.config.kv_block_size * 4 * kv4_groups(a.head_dim_)
         block_bytes = (2 * a.num_layers * kv_heads_local * self.config.kv_block_size *
                        a.head_dim_ * elem + scale_bytes)
+        block_bytes = int(block_bytes)
         if self.config.max_kv_blocks is not None:
             num_blocks = self.config.max_kv_blocks
         elif self.device.type == "cuda":
@@ -306,6 +317,8 @@ class LLMEngine:
         cache_dtype = self.dtype
         if self.config.kv_cache_dtype == "fp8_e4m3":
             cache_dtype = torch.float8_e4m3fn
+        elif self.config.kv_cache_dtype == "int4":
+            cache_dtype = torch.uint8
         return PagedKVCache(
             a.num_layers, kv_heads_local, a.head_dim_, self.config.kv_block_size,
             int(num_blocks), self.device, cache_dtype,

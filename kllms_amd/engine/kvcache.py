@@ -7,7 +7,8 @@ copies a block only when it must write into a shared one (its last, partial
 block). Sized for 288 GB of HBM3E per MI355X: with an 8B bf16 model resident
 (~16 GB) the cache can hold ~2M tokens of KV.
 
-Layout per layer: k_cache/v_cache = [num_blocks, kv_heads, block_size, head_dim].
+Layout per layer: k_cache/v_cache = [num_blocks, kv_heads, block_size, head_dim],
+in 4 bits head_dim / 2 bytes.
 """
 
 from __future__ import annotations
@@ -19,6 +20,8 @@ from dataclasses import dataclass, field
 from typing import Callable, List, Optional, Tuple
 
 import torch
+
+from ..ops.torch_ref import kv4_groups
 
 
 class BlockAllocator:
@@ -84,9 +87,11 @@ class PagedKVCache:
         self.block_size = block_size
         self.num_blocks = num_blocks
         self.device = device
+        # uint8: four bits a value, two values a byte (ops.torch_ref.kv4_quantize)
+        self.kv4 = dtype == torch.uint8
         # One contiguous allocation for all layers keeps pointers stable for
         # hipGraph capture and makes block copies (COW) two device ops.
-        self.k_all = torch.zeros(num_layers, num_blocks, num_kv_heads, block_size, head_dim,
+        self.k_all = torch.zeros(num_layers, num_blocks, num_kv_heads, block_size, head_dim // 2 if self.kv4 else head_dim,
                                  device=device, dtype=dtype)
         self.v_all = torch.zeros_like(self.k_all)
         self.k_caches = [self.k_all[i] for i in range(num_layers)]
@@ -95,19 +100,25 @@ class PagedKVCache:
         # at store time): outlier rows in real checkpoints would otherwise
         # saturate e4m3's +-448 under a static scale. fp32 [NB, KVH, BS] per
         # layer per cache = 1/32 of the fp8 payload; init 1.0 (neutral for
-        # never-written slots). bf16 caches carry no scales (None).
+        # never-written slots). 4-bit caches carry the step and least value of
+        # each group of 64 values, bf16 [NB, KVH, BS, groups, 2] = 1/8 of the
+        # payload. bf16 caches carry no scales (None).
         self.fp8 = dtype == torch.float8_e4m3fn
         if self.fp8:
             self.k_scale_all = torch.ones(num_layers, num_blocks, num_kv_heads, block_size,
                                           device=device, dtype=torch.float32)
             self.v_scale_all = torch.ones_like(self.k_scale_all)
+        elif self.kv4:
+            self.k_scale_all = torch.zeros(num_layers, num_blocks, num_kv_heads, block_size, kv4_groups(head_dim), 2,
+                                           device=device, dtype=torch.bfloat16)
+            self.v_scale_all = torch.zeros_like(self.k_scale_all)
         else:
             self.k_scale_all = self.v_scale_all = None
         self.allocator = BlockAllocator(num_blocks)
 
     def layer_caches(self) -> List[Tuple[torch.Tensor, torch.Tensor, Optional[torch.Tensor], Optional[torch.Tensor]]]:
         """Per layer (k, v, k_scale, v_scale); scales are None for bf16."""
-        if self.fp8:
+        if self.k_scale_all is not None:
             return [(self.k_caches[i], self.v_caches[i], self.k_scale_all[i], self.v_scale_all[i])
                     for i in range(self.num_layers)]
         return [(self.k_caches[i], self.v_caches[i], None, None) for i in range(self.num_layers)]
@@ -149,7 +160,7 @@ class PagedKVCache:
         dst = self.allocator.alloc()
         self.k_all[:, dst].copy_(self.k_all[:, src])
         self.v_all[:, dst].copy_(self.v_all[:, src])
-        if self.fp8:
+        if self.k_scale_all is not None:
             self.k_scale_all[:, dst].copy_(self.k_scale_all[:, src])
             self.v_scale_all[:, dst].copy_(self.v_scale_all[:, src])
         return dst
@@ -303,7 +314,8 @@ class HybridStateCache(PagedKVCache):
         self.block_size = block_size
         self.num_blocks = num_blocks
         self.device = device
-        self.fp8 = False
+        self.fp8 = self.kv4 = False
+        self.k_scale_all = self.v_scale_all = None
         self.specs = specs
         self.layers: List[LayerState] = []
         for sp in specs:

@@ -35,7 +35,7 @@ class ForwardBatch:
     mode: Literal["prefill", "decode", "segments"]
     positions: torch.Tensor              # [T] long
     slot_mapping: torch.Tensor           # [T] long — flat KV slots to write
-    kv_caches: List[Tuple]  # per layer (k, v, k_scale|None, v_scale|None)
+    kv_caches: List[Tuple]  # per layer (k, v, k_scale|None, v_scale|None): bf16, or fp8 or 4-bit (uint8) with scales
     cu_seqlens: Optional[torch.Tensor] = None   # [n_seq+1] int32 (prefill)
     block_tables: Optional[torch.Tensor] = None  # [B, max_blocks] int32 (decode)
     context_lens: Optional[torch.Tensor] = None  # [B] int32 (decode)
@@ -105,10 +105,10 @@ class LlamaAttention(nn.Module):
         """Attention of decode-mode rows q [T, H, D] against the paged cache; ``arrived``: zeros of ops.attn_decode_paged."""
         k_cache, v_cache, k_scale, v_scale = batch.kv_caches[self.layer_idx]
         paged = (batch.plans or {}).get("paged")
-        if paged is not None and k_scale is None:
+        if paged is not None:
             plan, short = paged
             return ops.attn_segments_paged(q, k_cache, v_cache, batch.block_tables, batch.context_lens, self.scale,
-                                           plan, short, batch.seg_tables, batch.seg_start)
+                                           plan, short, batch.seg_tables, batch.seg_start, k_scale, v_scale)
         return ops.attn_decode_paged(
             q, k_cache, v_cache, batch.block_tables, batch.context_lens, self.scale,
             k_scale, v_scale, arrived,
@@ -417,11 +417,10 @@ class LlamaForCausalLM(nn.Module):
                                     input_ids.shape[0])
             return replace(batch, plans={**(batch.plans or {}), "prefill": plan})
         if (batch.host_segs is not None and batch.seg_tables is not None and self.dtype == torch.bfloat16
-                and self.layers and self.layers[0].self_attn.head_dim == 128
-                and ops.paged_prefill_pays(batch.host_segs, self.layers[0].self_attn.num_kv_heads)):
+                and self.layers and self.layers[0].self_attn.head_dim == 128):
             at = self.layers[0].self_attn
-            rows = 64 if ops.paged_prefill_few(batch.host_segs, at.num_heads) else 256
-            plan, short = ops.paged_prefill_plan(batch.host_segs, input_ids.device, rows)
+            plan, short = ops.paged_plan(batch.host_segs, at.num_heads, at.num_kv_heads, input_ids.device,
+                                         batch.kv_caches[0][0].dtype if batch.kv_caches else torch.bfloat16)
             if plan is not None:
                 return replace(batch, plans={**(batch.plans or {}), "paged": (plan, short)})
         return batch

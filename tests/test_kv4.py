@@ -93,3 +93,85 @@ def test_decode_against_64_bits(D, gqa):
     out = ops.attn_decode_paged(q, kc, vc, tables, n, D ** -0.5, ks, vs)
     want, off = attention64(q, kc, vc, ks, vs, tables, n, D ** -0.5)
     assert bool(((out.double() - want).abs() <= off).all())
+
+
+def engine(**more):
+    from kllms_amd.engine.config import EngineConfig
+    from kllms_amd.engine.engine import LLMEngine
+
+    return LLMEngine(EngineConfig(**{**dict(model="tiny-llama", max_kv_blocks=256, use_hip_graphs=False, device="cpu", seed=0,
+                                            kv_cache_dtype="int4"), **more}))
+
+
+def greedy(n):
+    from kllms_amd.engine.sampling import SamplingParams
+
+    return SamplingParams(temperature=0.0, max_new_tokens=n)
+
+
+@pytest.mark.parametrize("model", ["tiny-llama", "tiny-mixtral"])
+def test_engine_generates(model):
+    from kllms_amd.engine.engine import GenRequest
+
+    eng = engine(model=model)
+    assert eng.kv.k_all.dtype == torch.uint8 and eng.kv.k_all.shape[-1] * 2 == eng.arch.head_dim_
+    outs = eng.generate([GenRequest(prompt_ids=list(range(1, 30)), n=3, sampling=greedy(8)),
+                         GenRequest(prompt_ids=[5], n=1, sampling=greedy(4))])
+    first = outs[0].streams[0].token_ids
+    assert len(first) >= 1 and all(s.token_ids == first for s in outs[0].streams)      # one prompt, no drawing: all alike
+
+
+def test_step_logits_are_those_of_the_values_the_cache_holds():
+    """A decode step over the 4-bit cache equals one over a plain cache that holds the same values."""
+    from kllms_amd.engine.engine import GenRequest
+
+    eng, plain = engine(), engine(kv_cache_dtype="bf16")
+    ids = list(range(1, 40))
+    outs = {}
+    for name, e in (("int4", eng), ("bf16", plain)):
+        seqs, streams = [], []
+        with torch.inference_mode():
+            e.begin_requests([GenRequest(prompt_ids=ids, n=1, sampling=greedy(4))], seqs, streams)
+        outs[name] = streams[0]
+    a, b = outs["int4"].seq, outs["bf16"].seq
+    assert a.blocks == b.blocks
+    for layer in range(eng.kv.num_layers):
+        for c4, s4, c in ((eng.kv.k_caches, eng.kv.k_scale_all, plain.kv.k_caches), (eng.kv.v_caches, eng.kv.v_scale_all, plain.kv.v_caches)):
+            held = torch_ref.kv4_values(c4[layer][a.blocks], s4[layer][a.blocks])
+            had = c[layer][a.blocks].bfloat16().float()
+            step = s4[layer][a.blocks][..., 0].float().amax()
+            assert bool(((held - had).abs() <= 0.53 * step).all())
+            c[layer][a.blocks] = held
+    from kllms_amd.models.llama import ForwardBatch
+
+    def step(e, seq):
+        slot = e.kv.append_slot(seq)
+        n = seq.num_tokens
+        batch = ForwardBatch(mode="decode", positions=torch.tensor([n - 1]), slot_mapping=torch.tensor([slot]),
+                             kv_caches=e.kv.layer_caches(), block_tables=torch.tensor([seq.blocks], dtype=torch.int32),
+                             context_lens=torch.tensor([n], dtype=torch.int32))
+        with torch.inference_mode():
+            return e.model.forward_decode(torch.tensor([7]), batch)
+
+    got, want = step(eng, a), step(plain, b)
+    # one position of 40 is rounded to 4 bits in one of them: the logits move by a small part of their spread
+    assert float((got - want).abs().max()) < 0.1 * float(want.std())
+
+
+def test_a_copied_block_takes_its_scales_along():
+    eng = engine()
+    kv = eng.kv
+    src = kv.allocator.alloc()
+    for t in (kv.k_all, kv.v_all):
+        t[:, src] = torch.randint(0, 256, t[:, src].shape, dtype=torch.uint8)
+    for t in (kv.k_scale_all, kv.v_scale_all):
+        t[:, src] = torch.randn(t[:, src].shape).bfloat16()
+    dst = kv._copy_block(src)
+    for t in (kv.k_all, kv.v_all, kv.k_scale_all, kv.v_scale_all):
+        assert torch.equal(t[:, src], t[:, dst]) and dst != src
+    assert all(len(c) == 4 and c[2].dtype == torch.bfloat16 for c in kv.layer_caches())
+
+
+def test_models_with_states_are_refused():
+    with pytest.raises(ValueError, match="int4"):
+        engine(model="tiny-zutalix")
