@@ -457,6 +457,58 @@ def linear_clamped_glu(x: torch.Tensor, w: torch.Tensor, limit: float, alpha: fl
     return _try_tiles(x, w, None, 2, limit, alpha)
 
 
+# --- products in 8-bit integers -----------------------------------------------------
+
+def _check_int8(x: torch.Tensor, w: torch.Tensor) -> None:
+    if w.dtype != torch.int8 or w.dim() != 2 or x.dim() != 2 or x.shape[1] != w.shape[1]:
+        raise ValueError(f"x [M, K] with int8 weights [N, K]: got {list(x.shape)} with {w.dtype} {list(w.shape)}")
+    if x.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError("products in 8-bit integers have no gradient: call them under torch.no_grad()")
+
+
+def quantize_rows(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(codes int8 [M, K], scales fp32 [M]) of rows: x / scale to the nearest whole number, scale = max |x| / 127 of the
+    row. A row with a value that is no finite number has the scale NaN. On the GPU x is bf16, K a multiple of 16."""
+    if x.dim() != 2:
+        raise ValueError(f"rows [M, K]: got {list(x.shape)}")
+    if x.is_cuda and not _force_torch():
+        return _hip_or_raise().quantize_rows(x)
+    return torch_ref.quantize_rows(x)
+
+
+def quantize_weights(w: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(int8 [N, K], scales fp32 [N]) of a weight matrix [N, K] of any float type, for linear_int8."""
+    if w.dim() != 2:
+        raise ValueError(f"weights [N, K]: got {list(w.shape)}")
+    return torch_ref.quantize_weights(w)
+
+
+def linear_int8(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, bias: Optional[torch.Tensor] = None,
+                once: bool = False) -> torch.Tensor:
+    """x @ w^T (+ bias) in 8-bit integers, in x's dtype: x [M, K] quantized row by row (quantize_rows), w int8 [N, K] with a
+    scale for each row (quantize_weights), exact 32-bit sums. On the GPU x is bf16, K a multiple of 16 up to 131072, N one of 16.
+    ``once``: weights_once of the caller's model."""
+    _check_int8(x, w)
+    if x.is_cuda and not _force_torch():
+        return _hip_or_raise().linear_int8(x, w, w_scale, bias, 0, once)
+    return torch_ref.linear_int8(x, w, w_scale, bias)
+
+
+def linear_silu_int8(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, once: bool = False) -> torch.Tensor:
+    """silu(gate) * up of linear_int8 with a fused [gate; up] matrix (N a multiple of 32 on the GPU)."""
+    _check_int8(x, w)
+    if w.shape[0] % 2:
+        raise ValueError("gate and up have the same rows")
+    if x.is_cuda and not _force_torch():
+        return _hip_or_raise().linear_int8(x, w, w_scale, None, 1, once)
+    return torch_ref.linear_silu_int8(x, w, w_scale)
+
+
+def linear_part_int8(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, once: bool = False) -> torch.Tensor:
+    """linear_int8 of up to LINEAR_ROWS_MAX rows as fp32 sums [S, M, N] over S shares of K, like linear_part (GPU only)."""
+    return _hip_or_raise().linear_int8(x, w, w_scale, None, 2, once)
+
+
 def embed_norm_rows(ids, table, weight, eps, unknown=None, clear=None):
     """(rms(table[ids]) * weight, table[ids]). An id outside the table gives a row of NaN and sets ``unknown``, one int32
     of pinned host memory, to 1. ``clear``: int32 values on the GPU that the launch zeroes."""

@@ -554,6 +554,90 @@ torch::Tensor linear_tiles(torch::Tensor x, torch::Tensor w, torch::Tensor bias,
   return out;
 }
 
+// --- products in 8-bit integers (linear_int8.hip) --------------------------------
+extern "C" int int8_rows_padded(int K);
+extern "C" void launch_int8_rows(int8_t* codes, float* scales, const bf16_t* x, int64_t x_stride, int M, int K, int* clear, int clears,
+                                 hipStream_t stream);
+extern "C" int64_t linear_int8_room(int M, int N, int K, int form, int* zeros);
+extern "C" int linear_int8_splits(int M, int N, int K);
+extern "C" int launch_linear_int8(void* out, const int8_t* x, const float* xs, const int8_t* w, const float* ws, const bf16_t* bias,
+                                  float* part, int* count, int M, int N, int K, int form, bool once, hipStream_t stream);
+
+static bool on_16_bytes_at(const torch::Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0; }
+
+static void check_int8_rows(const torch::Tensor& x, const char* who) {
+  TORCH_CHECK(x.is_cuda() && x.scalar_type() == at::kBFloat16 && x.dim() == 2, who, ": rows are bf16 [M, K] on the GPU");
+  TORCH_CHECK(x.size(1) % 16 == 0 && x.size(1) >= 16 && x.size(1) <= 131072 && x.size(0) < (1LL << 30),
+              who, ": K is a multiple of 16, up to 131072 (a sum of more products does not fit 32 bits)");
+}
+
+// rows that 16-byte loads can read
+static torch::Tensor int8_readable(const torch::Tensor& x) {
+  const bool fine = x.stride(1) == 1 && on_16_bytes_at(x) && (x.size(0) <= 1 || (x.stride(0) % 8 == 0 && x.stride(0) >= 0));
+  return fine ? x : x.clone(at::MemoryFormat::Contiguous);
+}
+
+// (codes int8 [M, K], a view of rows filled up with zeros; scales fp32 [M]) of bf16 rows
+std::tuple<torch::Tensor, torch::Tensor> quantize_rows(torch::Tensor x) {
+  check_int8_rows(x, "quantize_rows");
+  const c10::DeviceGuard device(x.device());
+  const int64_t M = x.size(0), K = x.size(1);
+  auto codes = torch::empty({M, int8_rows_padded((int)K)}, x.options().dtype(torch::kChar));
+  auto scales = torch::empty({M}, x.options().dtype(torch::kFloat));
+  if (M > 0) {
+    x = int8_readable(x);
+    launch_int8_rows(codes.data_ptr<int8_t>(), scales.data_ptr<float>(), cbf(x), x.stride(0), (int)M, (int)K, nullptr, 0, cur_stream());
+  }
+  return {codes.narrow(1, 0, K), scales};
+}
+
+static void check_int8_weights(const torch::Tensor& w, const torch::Tensor& w_scale, int64_t K, const torch::Tensor& like, int64_t form) {
+  TORCH_CHECK(w.scalar_type() == at::kChar && w.dim() == 2 && w.is_contiguous() && w.size(1) == K && w.device() == like.device() &&
+                  on_16_bytes_at(w), "linear_int8: weights are contiguous int8 [N, K] on x's device, on 16 bytes");
+  TORCH_CHECK(w.size(0) % (form == 1 ? 32 : 16) == 0 && w.size(0) > 0 && w.size(0) < (1LL << 30),
+              "linear_int8: N is a multiple of 16 (of 32 for gate and up)");
+  TORCH_CHECK(w_scale.scalar_type() == at::kFloat && w_scale.is_contiguous() && w_scale.numel() == w.size(0) &&
+                  w_scale.device() == like.device() && on_16_bytes_at(w_scale), "linear_int8: a contiguous fp32 scale for each row of the weights");
+}
+
+// form 0: x [M, K] w^T (+ bias) in bf16, 1: silu(gate) * up of a fused [gate; up], 2: fp32 sums [S, M, N] of up to 128 rows.
+// once: the weights of the caller's step do not stay in the caches until its next
+torch::Tensor linear_int8(torch::Tensor x, torch::Tensor w, torch::Tensor w_scale, std::optional<torch::Tensor> bias, int64_t form,
+                          bool once) {
+  check_int8_rows(x, "linear_int8");
+  TORCH_CHECK(form >= 0 && form <= 2, "linear_int8: form 0 to 2");
+  const int64_t M = x.size(0), K = x.size(1);
+  check_int8_weights(w, w_scale, K, x, form);
+  const int64_t N = w.size(0);
+  TORCH_CHECK(form != 2 || (M >= 1 && M <= 128), "linear_int8: sums of 1 to 128 rows");
+  TORCH_CHECK(((M + 63) / 64) * ((N + 127) / 128) < (1 << 27), "linear_int8: too many tiles");
+  if (bias) {
+    TORCH_CHECK(form == 0 && bias->scalar_type() == at::kBFloat16 && bias->is_contiguous() && bias->numel() == N &&
+                    bias->device() == x.device(), "linear_int8: bias bf16 [N] of a plain product");
+    if (reinterpret_cast<uintptr_t>(bias->data_ptr()) % 8) bias = bias->clone();
+  }
+  const c10::DeviceGuard device(x.device());
+  const int S = form == 2 ? linear_int8_splits((int)M, (int)N, (int)K) : 1;
+  auto out = form == 2 ? torch::empty({S, M, N}, x.options().dtype(torch::kFloat)) : torch::empty({M, form == 1 ? N / 2 : N}, x.options());
+  if (M == 0) return out;
+  x = int8_readable(x);
+  int zeros = 0;
+  const int64_t room = form == 2 ? 0 : linear_int8_room((int)M, (int)N, (int)K, (int)form, &zeros);
+  const int64_t padded = int8_rows_padded((int)K);
+  // codes, scales and counters in one allocation
+  const int64_t scales_at = M * padded, count_at = scales_at + (M + 3) / 4 * 16;
+  auto work = torch::empty({count_at + 4 * zeros}, x.options().dtype(torch::kByte));
+  auto part = room ? torch::empty({room}, x.options().dtype(torch::kFloat)) : torch::Tensor();
+  char* at = reinterpret_cast<char*>(work.data_ptr());
+  launch_int8_rows(reinterpret_cast<int8_t*>(at), reinterpret_cast<float*>(at + scales_at), cbf(x), x.stride(0), (int)M, (int)K,
+                   reinterpret_cast<int*>(at + count_at), zeros, cur_stream());
+  TORCH_CHECK(launch_linear_int8(out.data_ptr(), reinterpret_cast<int8_t*>(at), reinterpret_cast<float*>(at + scales_at), w.data_ptr<int8_t>(),
+                                 w_scale.data_ptr<float>(), bias ? cbf(*bias) : nullptr, room ? part.data_ptr<float>() : nullptr,
+                                 reinterpret_cast<int*>(at + count_at), (int)M, (int)N, (int)K, (int)form, once, cur_stream()) == 0,
+              "linear_int8: 160 KB of LDS are not available");
+  return out;
+}
+
 // Whether nothing but the values of a tensor is wanted: no subclass, transform or gradient looks on
 static bool plain_values(const torch::Tensor& t) {
   static const c10::DispatchKeySet others({c10::DispatchKey::Python, c10::DispatchKey::PythonTLSSnapshot,
@@ -852,6 +936,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("unknown"), py::arg("clear") = py::none());
   m.def("rope_store_rows", &rope_store_rows);
   m.def("decode_inputs", &decode_inputs);
+  m.def("quantize_rows", &quantize_rows);
+  m.def("linear_int8", &linear_int8, py::arg("x"), py::arg("w"), py::arg("w_scale"), py::arg("bias"), py::arg("form"),
+        py::arg("once") = false);
+  m.def("linear_int8_splits", &linear_int8_splits);
   m.def("linear_tiles", &linear_tiles);
   m.def("linear_tiles_rows", &linear_tiles_rows);
   m.def("linear_tiles_pick", &linear_tiles_pick);

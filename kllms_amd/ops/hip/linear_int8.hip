@@ -1,0 +1,415 @@
+// Products of rows in 8-bit integers, a scale for each row, with a weight matrix in 8-bit integers, a scale for each of its
+// rows (output channels), for gfx950:
+//
+//   s_m = max |x_m| / 127,  c_m = x_m / s_m to the nearest whole number, halves to even
+//   y_mn = (sum_k c_mk w_nk) s_m t_n (+ b_n),  or silu(gate) * up of such sums in fp32, rounded once
+//
+// The sums are of 32 bits and exact: 127 * 127 * K stays below 2^31 up to K = 131072. So shares of K add up to the same
+// whoever is last. 127 x and its quotient by max |x| decide between two whole numbers as the exact quotient does: both are bf16
+// values, of 8 bits, so a quotient that is no half itself is 2^-17 of it away from one.
+//
+// On the ring and tiles of tile_product.h, to which a row of K integers is one of K / 2 bf16: as many bytes and
+// matrix instructions of twice the products. Up to 128 rows the stream of W is the bound, in tiles of 64 or 128 rows of W
+// (linear_rows.hip has the reasons); above, tiles of 256 and the matrix units (linear_tiles.hip). A product of few tiles is shared out
+// over K; each workgroup leaves its sums past the L2 and the last one to arrive adds them up. The counters for that are zeroed by the
+// launch that makes the codes, which comes before anyway.
+//
+// K is a multiple of 16; the codes' rows are filled up to whole stages with zeros, which what W has behind a row meets.
+
+#include <atomic>
+
+#include "tile_product.h"
+
+typedef unsigned short u16x8 __attribute__((ext_vector_type(8)));
+typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
+
+#define LI_STAGE 128       // bytes of a row in a stage
+enum Int8Form { LI_BF16 = 0, LI_SILU = 1, LI_PART = 2 };
+
+// ---- codes ---------------------------------------------------------------------------------------
+
+// What rows are multiplied with before they are rounded: 127 / most by an inverse and what it leaves, both taken near one
+struct Int8Row {
+  float up, most, inverse, scale;
+  __device__ __forceinline__ explicit Int8Row(uint32_t bits) {       // of the largest magnitude, as bf16
+    const float m = __uint_as_float(bits << 16);
+    const bool sound = bits < 0x7f80u;                               // neither infinite nor NaN
+    const int e = max((int)(bits >> 7) - 127, -120);
+    const float f = ldexpf(1.0f, -e);
+    up = 127.0f * f;
+    most = m * f;
+    inverse = sound && m > 0.0f ? 1.0f / most : 0.0f;
+    scale = sound ? m / 127.0f : __uint_as_float(0x7fc00000u);       // such a row is NaN as a whole
+  }
+  __device__ __forceinline__ uint32_t code(float x) const {          // one byte
+    const float t = x * up, q = t * inverse;
+    const float n = __builtin_rintf(__builtin_fmaf(__builtin_fmaf(-q, most, t), inverse, q));
+    return (uint32_t)(int)fminf(fmaxf(n, -127.0f), 127.0f) & 0xffu;
+  }
+};
+
+// LANES threads a row, R vectors of 8 of each (R 0: any number, read twice). codes [M, padded], zeros behind K; clears
+// ``clear`` beside.
+template <int LANES, int R>
+__global__ void __launch_bounds__(256) int8_rows_kernel(int8_t* __restrict__ codes, float* __restrict__ scales,
+                                                        const bf16_t* __restrict__ x, int64_t x_stride, int M, int K, int padded,
+                                                        int* __restrict__ clear, int clears) {
+  __shared__ uint32_t red[4];
+  const int tid = threadIdx.x, lane = tid % LANES;
+  for (int i = blockIdx.x * 256 + tid; i < clears; i += gridDim.x * 256) clear[i] = 0;
+  const int m = blockIdx.x * (256 / LANES) + tid / LANES;
+  if (LANES == 64 && m >= M) return;
+  const int vecs = K / 8, all = padded / 8;
+  const u16x8* row = reinterpret_cast<const u16x8*>((const short*)x + (int64_t)m * x_stride);
+  u32x2* to = reinterpret_cast<u32x2*>(codes + (int64_t)m * padded);
+  u16x8 v[R > 0 ? R : 1];
+  u16x8 top = {};
+  if constexpr (R > 0) {
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const int i = lane + r * LANES;
+      v[r] = i < vecs ? row[i] : u16x8{};
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r) top = __builtin_elementwise_max(top, v[r] & (u16x8)(unsigned short)0x7fff);
+  } else {
+    for (int i = lane; i < vecs; i += LANES) top = __builtin_elementwise_max(top, row[i] & (u16x8)(unsigned short)0x7fff);
+  }
+  uint32_t most = 0;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) most = max(most, (uint32_t)top[j]);
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) most = max(most, (uint32_t)__shfl_xor((int)most, off));
+  if constexpr (LANES == 256) {
+    if ((tid & 63) == 0) red[tid >> 6] = most;
+    __syncthreads();
+    most = max(max(red[0], red[1]), max(red[2], red[3]));
+  }
+  const Int8Row by(most);
+  if (lane == 0) scales[m] = by.scale;
+  auto put = [&](int i, const u16x8& a) {
+    uint32_t w[2] = {0u, 0u};
+#pragma unroll
+    for (int j = 0; j < 8; ++j) w[j >> 2] |= by.code(bf16_to_f32((short)a[j])) << ((j & 3) * 8);
+    to[i] = u32x2{w[0], w[1]};
+  };
+  if constexpr (R > 0) {
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+      if (lane + r * LANES < all) put(lane + r * LANES, v[r]);
+  } else {
+    for (int i = lane; i < all; i += LANES) put(i, i < vecs ? row[i] : u16x8{});
+  }
+}
+
+extern "C" int int8_rows_padded(int K) { return (K + LI_STAGE - 1) / LI_STAGE * LI_STAGE; }
+
+extern "C" void launch_int8_rows(int8_t* codes, float* scales, const bf16_t* x, int64_t x_stride, int M, int K, int* clear, int clears,
+                                 hipStream_t stream) {
+  const int padded = int8_rows_padded(K);
+#define LI_ROWS(LANES, R)                                                                                                    \
+  hipLaunchKernelGGL((int8_rows_kernel<LANES, R>), dim3((M + 256 / LANES - 1) / (256 / LANES)), dim3(256), 0, stream, codes, scales, \
+                     x, x_stride, M, K, padded, clear, clears)
+  if (padded <= 512) LI_ROWS(64, 1);
+  else if (padded <= 1024) LI_ROWS(64, 2);
+  else if (padded <= 2048) LI_ROWS(256, 1);
+  else if (padded <= 4096) LI_ROWS(256, 2);
+  else if (padded <= 8192) LI_ROWS(256, 4);
+  else if (padded <= 16384) LI_ROWS(256, 8);
+  else LI_ROWS(256, 0);
+#undef LI_ROWS
+}
+
+// ---- up to 128 rows ------------------------------------------------------------------------------
+
+// linear_rows_kernel of whole numbers. K, padded: bytes of a row of w and of x. PART leaves fp32 sums [splits, M, N], the
+// others add their shares up (part, count) and write bf16.
+template <int NI, int MJ, int FORM, int KB, bool ONCE>
+__global__ void __launch_bounds__(TP_THREADS, 1) linear_int8_rows_kernel(
+    void* __restrict__ out, const int8_t* __restrict__ x, const float* __restrict__ xs, const int8_t* __restrict__ w,
+    const float* __restrict__ ws, const bf16_t* __restrict__ bias, float* __restrict__ part, int* __restrict__ count, int M, int N,
+    int K, int padded, int m_tiles, int splits) {
+  extern __shared__ __attribute__((aligned(1024))) char smem[];
+  constexpr bool GATED = FORM == LI_SILU;
+  constexpr int BN = GATED ? 16 * NI : 32 * NI;    // columns of the result
+  const int columns = GATED ? N / 2 : N;
+  const int n_tiles = (columns + BN - 1) / BN, all = n_tiles * splits * m_tiles, xcd = blockIdx.x & 7;
+  const int begin = (int)((int64_t)all * xcd >> 3), items = (int)((int64_t)all * (xcd + 1) >> 3) - begin;
+  const int at = blockIdx.x >> 3;
+  if (at >= items) return;
+  const int item = begin + at, rest = item / m_tiles, share = rest / n_tiles, n0 = rest % n_tiles * BN;
+  const int rows = (M + m_tiles - 1) / m_tiles;    // even parts
+  const int m0 = item % m_tiles * rows, m_end = min(M, m0 + rows);
+  const int stages_all = padded / LI_STAGE, first = (int)((int64_t)stages_all * share / splits);
+  const int stages = (int)((int64_t)stages_all * (share + 1) / splits) - first, k0 = first * LI_STAGE;
+  const int lane = threadIdx.x & 63, col = lane & 15, grp = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  i32x4 acc[NI][MJ];
+#pragma unroll
+  for (int i = 0; i < NI; ++i)
+#pragma unroll
+    for (int j = 0; j < MJ; ++j) acc[i][j] = i32x4{0, 0, 0, 0};
+  // W rows of a gated tile: 8 * NI gate, the same of up, the next gate, their up
+  const int n_put = GATED ? n0 + (wave >> 1) * (8 * NI) : n0 + wave * (8 * NI);
+  const bf16_t* wk = reinterpret_cast<const bf16_t*>(w + (GATED ? (int64_t)(wave & 1) * columns : 0) * K + k0);
+  const TileRows xr(reinterpret_cast<const bf16_t*>(x + k0), m0 + wave * MJ * 8, m_end, MJ * 8, padded / 2, (padded - k0) / 2, lane);
+  const TileRowsOf<ONCE> wr(wk, n_put, columns, 8 * NI, K / 2, (K - k0) / 2, lane);
+  tile_product<MJ, NI, KB * 1024>(acc, wr, xr, stages, stages * xcd / 8, smem);
+  if constexpr (FORM != LI_PART) {
+    if (splits > 1) {
+      const int tile = rest % n_tiles * m_tiles + item % m_tiles;
+      if (!tile_fold<MJ>(acc, part + (int64_t)tile * splits * (NI * MJ * TP_THREADS * 4), share, splits, count + tile, smem)) return;
+    }
+  }
+  const int m = m0 + (wave & 1) * MJ * 16 + col, n = n0 + (wave >> 1) * (BN / 2) + grp * 4;
+#pragma unroll
+  for (int j = 0; j < MJ; ++j) {
+    const int mr = m + j * 16;
+    if (mr >= m_end) continue;
+    const float s = xs[mr];
+#pragma unroll
+    for (int i = 0; i < (GATED ? NI / 2 : NI); ++i) {
+      const int nc = n + i * 16;
+      if (nc >= columns) continue;
+      const f32x4 t = *reinterpret_cast<const f32x4*>(ws + nc);
+      f32x4 v;
+      if constexpr (GATED) {
+        const f32x4 tu = *reinterpret_cast<const f32x4*>(ws + columns + nc);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float g = (float)acc[i][j][r] * s * t[r], u = (float)acc[i + NI / 2][j][r] * s * tu[r];
+          v[r] = g / (1.0f + __expf(-g)) * u;
+        }
+      } else {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) v[r] = (float)acc[i][j][r] * s * t[r];
+      }
+      if constexpr (FORM == LI_PART) {
+        *reinterpret_cast<f32x4*>((float*)out + ((int64_t)share * M + mr) * N + nc) = v;
+      } else {
+        if (FORM == LI_BF16 && bias) {
+          const bf16x4_vec b = *reinterpret_cast<const bf16x4_vec*>((const short*)bias + nc);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) v[r] += bf16_to_f32(b[r]);
+        }
+        *reinterpret_cast<bf16x4_vec*>((short*)out + (int64_t)mr * columns + nc) = tp_pack(v[0], v[1], v[2], v[3]);
+      }
+    }
+  }
+}
+
+#define LI_UNITS 256       // compute units
+
+struct Int8Plan {
+  int ni, mj, m_tiles, splits;
+};
+
+// Tiles of up to 128 rows, as linear_plan has them for K / 2 bf16, and shares of K: one workgroup for each compute unit, four
+// stages at least
+static Int8Plan int8_plan(int M, int N, int K, int form) {
+  Int8Plan p;
+  p.m_tiles = 1;
+  p.mj = (M + 31) / 32;
+  if (form == LI_SILU) p.ni = N <= 256 * 64 || (N > 256 * 128 && p.mj == 1) ? 2 : 4;
+  else p.ni = N <= 8448 && !(p.mj == 4 && N >= 4096 && K >= 16384) ? 2 : 4;
+  const int tiles = ((form == LI_SILU ? N / 2 : N) + (form == LI_SILU ? 16 : 32) * p.ni - 1) / ((form == LI_SILU ? 16 : 32) * p.ni);
+  const int most = int8_rows_padded(K) / LI_STAGE / 4, s = (LI_UNITS + 8) / tiles;
+  p.splits = s < 1 || most < 1 ? 1 : s < most ? s : most;
+  return p;
+}
+
+extern "C" int linear_int8_splits(int M, int N, int K) { return int8_plan(M, N, K, LI_PART).splits; }
+
+#define LI_ONCE (8 << 20)
+#define LI_ONCE_ALONE ((int64_t)320 << 20)
+
+template <int NI, int MJ, int FORM, bool ONCE>
+static int linear_int8_rows_go(const Int8Plan& p, void* out, const int8_t* x, const float* xs, const int8_t* w, const float* ws,
+                               const bf16_t* bias, float* part, int* count, int M, int N, int K, hipStream_t stream) {
+  constexpr int KB = NI == 2 || MJ <= 2 ? 80 : 160, BN = (FORM == LI_SILU ? 16 : 32) * NI;
+  if (!tp_lds_ready(reinterpret_cast<const void*>(linear_int8_rows_kernel<NI, MJ, FORM, KB, ONCE>))) return -1;
+  constexpr int LDS = TileRing<MJ, NI, KB * 1024>::STRIDE * TileRing<MJ, NI, KB * 1024>::RING;
+  const int64_t all = (int64_t)(((FORM == LI_SILU ? N / 2 : N) + BN - 1) / BN) * p.splits * p.m_tiles;
+  hipLaunchKernelGGL((linear_int8_rows_kernel<NI, MJ, FORM, KB, ONCE>), dim3((all + 7) / 8 * 8), dim3(TP_THREADS), LDS, stream, out, x, xs,
+                     w, ws, bias, part, count, M, N, K, int8_rows_padded(K), p.m_tiles, p.splits);
+  return 0;
+}
+
+template <int FORM>
+static int linear_int8_rows_form(const Int8Plan& p, void* out, const int8_t* x, const float* xs, const int8_t* w, const float* ws,
+                                 const bf16_t* bias, float* part, int* count, int M, int N, int K, bool once, hipStream_t stream) {
+  const int64_t bytes = (int64_t)N * K;
+  once = once ? bytes >= LI_ONCE : bytes >= LI_ONCE_ALONE;
+#define LI_CASE(NI, MJ)                                                                                                           \
+  if (p.ni == NI && p.mj == MJ)                                                                                                   \
+    return once ? linear_int8_rows_go<NI, MJ, FORM, true>(p, out, x, xs, w, ws, bias, part, count, M, N, K, stream)               \
+                : linear_int8_rows_go<NI, MJ, FORM, false>(p, out, x, xs, w, ws, bias, part, count, M, N, K, stream)
+  LI_CASE(2, 1);
+  LI_CASE(2, 2);
+  LI_CASE(2, 3);
+  LI_CASE(2, 4);
+  LI_CASE(4, 1);
+  LI_CASE(4, 2);
+  LI_CASE(4, 3);
+  LI_CASE(4, 4);
+#undef LI_CASE
+  return -1;
+}
+
+// ---- more rows -----------------------------------------------------------------------------------
+
+#define LI_BAND 8          // row tiles of a band
+
+template <int ACT, int MJ>
+__global__ void __launch_bounds__(TP_THREADS, 1) linear_int8_tiles_kernel(
+    bf16_t* __restrict__ out, const int8_t* __restrict__ x, const float* __restrict__ xs, const int8_t* __restrict__ w,
+    const float* __restrict__ ws, const bf16_t* __restrict__ bias, float* __restrict__ part, int* __restrict__ count, int M, int N, int K,
+    int padded, int m_tiles) {
+  extern __shared__ __attribute__((aligned(1024))) char smem[];
+  constexpr int BN = ACT ? 128 : 256;              // output columns of a workgroup
+  const int n_tiles = (N + BN - 1) / BN;
+  // an XCD's tiles are neighbours, in bands of rows and column by column in them
+  const int xcd = blockIdx.x & 7;
+  const int all = m_tiles * n_tiles;
+  const int begin = (int)((int64_t)all * xcd / 8), tiles = (int)((int64_t)all * (xcd + 1) / 8) - begin;
+  const int stages_all = padded / LI_STAGE;
+  const TileShare sh(blockIdx.x >> 3, tiles, stages_all, part, count, xcd, 256 * 32 * MJ);
+  if (sh.tile >= tiles) return;
+  const int tile = begin + sh.tile;
+  const int bands = (m_tiles + LI_BAND - 1) / LI_BAND, deep = (m_tiles + bands - 1) / bands;
+  const int band = tile / (deep * n_tiles), in = tile % (deep * n_tiles);
+  const int high = min(deep, m_tiles - band * deep);
+  const int rows = (M + m_tiles - 1) / m_tiles;    // even parts
+  const int m0 = (band * deep + in % high) * rows, m_end = min(M, m0 + rows);
+  const int n0 = in / high * BN;
+  const int lane = threadIdx.x & 63, col = lane & 15, grp = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  i32x4 acc[8][MJ];
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+#pragma unroll
+    for (int j = 0; j < MJ; ++j) acc[i][j] = i32x4{0, 0, 0, 0};
+  const int stages = sh.length(stages_all), k0 = sh.first(stages_all) * LI_STAGE;
+  const int m = m0 + (wave & 1) * MJ * 16;         // first row of this wave's results
+  const TileRows xr(reinterpret_cast<const bf16_t*>(x + k0), m0 + wave * MJ * 8, m_end, MJ * 8, padded / 2, (padded - k0) / 2, lane);
+  // W rows of a gated tile: 64 gate, 64 up, the next 64 gate, 64 up
+  const int n_put = ACT ? n0 + (wave >> 1) * 64 : n0 + wave * 64;
+  const TileRows wr(reinterpret_cast<const bf16_t*>(w + (ACT ? (int64_t)(wave & 1) * N : 0) * K + k0), n_put, N, 64, K / 2, (K - k0) / 2, lane);
+  tile_product<MJ>(acc, wr, xr, stages, stages * xcd / 8, smem);
+  if (sh.shares > 1 && !tile_fold<MJ>(acc, sh.part, sh.share, sh.shares, sh.count, smem)) return;
+  float s[MJ];
+#pragma unroll
+  for (int j = 0; j < MJ; ++j) s[j] = xs[min(m + j * 16 + col, M - 1)];
+  const int n = n0 + (wave >> 1) * (ACT ? 64 : 128);
+  // scales and bias of 4 columns: N is a multiple of 16, what is behind it is not stored
+  auto of = [&](int at) { return *reinterpret_cast<const f32x4*>(ws + (ACT && at >= 2 * N ? 0 : !ACT && at >= N ? 0 : at)); };
+  if constexpr (ACT) {
+    tile_store<4, MJ>(out + (int64_t)m * N + n, N, m_end - m, N - n, smem, [&](int i, int j) {
+      const int c = min(n + i * 16 + grp * 4, N - 4);
+      const f32x4 tg = of(c), tu = of(N + c);
+      float v[4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const float g = (float)acc[i][j][r] * s[j] * tg[r], u = (float)acc[i + 4][j][r] * s[j] * tu[r];
+        v[r] = g / (1.0f + __expf(-g)) * u;
+      }
+      return tp_pack(v[0], v[1], v[2], v[3]);
+    });
+  } else {
+    tile_store<8, MJ>(out + (int64_t)m * N + n, N, m_end - m, N - n, smem, [&](int i, int j) {
+      const int c = min(n + i * 16 + grp * 4, N - 4);
+      const f32x4 t = of(c);
+      bf16x4_vec b = {0, 0, 0, 0};
+      if (bias) b = *reinterpret_cast<const bf16x4_vec*>((const short*)bias + c);
+      float v[4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) v[r] = (float)acc[i][j][r] * s[j] * t[r] + bf16_to_f32(b[r]);
+      return tp_pack(v[0], v[1], v[2], v[3]);
+    });
+  }
+}
+
+// us of a round of tiles of 32 * MJ rows by 256 columns and 64 stages, with all compute units at work
+static const int LI_COST[9] = {0, 0, 44, 49, 60, 68, 77, 88, 97};
+
+// MJ of the tiles of more than 128 rows, + 16 where the last round is shared out over K
+static int int8_tiles_pick(int64_t M, int64_t N, int64_t K, bool gated) {
+  const int64_t n_tiles = gated ? (N + 127) / 128 : (N + 255) / 256, stages = int8_rows_padded((int)K) / LI_STAGE;
+  int best = 8;
+  double least = 1e30;
+  for (int mj = 8; mj >= 2; --mj) {
+    const int64_t tiles = (M + 32 * mj - 1) / (32 * mj) * n_tiles;
+    const double round = LI_COST[mj] * (stages / 64.0);
+    const double whole = (tiles + LI_UNITS - 1) / LI_UNITS * round;
+    if (whole < least) least = whole, best = mj;
+    const int64_t unit = (tiles + 7) / 8, rest = unit % TP_SLOTS;
+    if (stages < 16 || rest == 0 || rest > TP_SLOTS / 2) continue;
+    int64_t shares = TP_SLOTS / rest < TP_SHARES ? TP_SLOTS / rest : TP_SHARES;
+    shares = shares < stages / 8 ? shares : stages / 8;
+    // the sums' way through memory: 16 us for four shares of 64 rows, 28 for three of 256
+    const double shared = unit / TP_SLOTS * round + round / shares + 10 + 0.75 * mj * shares;
+    if (shared < least) least = shared, best = mj + 16;
+  }
+  return best;
+}
+
+template <int ACT, int MJ>
+static int linear_int8_tiles_go(void* out, const int8_t* x, const float* xs, const int8_t* w, const float* ws, const bf16_t* bias,
+                                float* part, int* count, int M, int N, int K, hipStream_t stream) {
+  if (!tp_lds_ready(reinterpret_cast<const void*>(linear_int8_tiles_kernel<ACT, MJ>))) return -1;
+  constexpr int BN = ACT ? 128 : 256;
+  const int m_tiles = (M + 32 * MJ - 1) / (32 * MJ);
+  const int64_t all = (int64_t)m_tiles * ((N + BN - 1) / BN);
+  hipLaunchKernelGGL((linear_int8_tiles_kernel<ACT, MJ>), dim3(((all + 7) / 8 + (part ? TP_SLOTS : 0)) * 8), dim3(TP_THREADS), TP_LDS, stream,
+                     (bf16_t*)out, x, xs, w, ws, bias, part, count, M, N, K, int8_rows_padded(K), m_tiles);
+  return 0;
+}
+
+// ---- the calls -----------------------------------------------------------------------------------
+
+#define LI_ROWS_MOST 128
+
+// floats of part and zeros of count that a product (form 0 or 1; N: rows of w) takes, 0 where it has no shares
+extern "C" int64_t linear_int8_room(int M, int N, int K, int form, int* zeros) {
+  *zeros = 0;
+  if (M <= LI_ROWS_MOST) {
+    const Int8Plan p = int8_plan(M, N, K, form);
+    if (p.splits == 1) return 0;
+    const int64_t tiles = ((form == LI_SILU ? N / 2 : N) + (form == LI_SILU ? 16 : 32) * p.ni - 1) / ((form == LI_SILU ? 16 : 32) * p.ni);
+    *zeros = (int)(tiles * p.m_tiles);
+    return tiles * p.m_tiles * p.splits * (p.ni * p.mj * TP_THREADS * 4);
+  }
+  const int mj = int8_tiles_pick(M, form == LI_SILU ? N / 2 : N, K, form == LI_SILU);
+  if (mj < 16) return 0;
+  *zeros = LI_UNITS;
+  return (int64_t)LI_UNITS * 256 * 32 * (mj & 15);
+}
+
+// form 0: bf16 [M, N] (+ bias), 1: silu(gate) * up bf16 [M, N / 2]; 2: fp32 sums [splits, M, N] of up to 128 rows. part and
+// count (zeroed): of linear_int8_room. 0, or -1 where the LDS cannot be had.
+extern "C" int launch_linear_int8(void* out, const int8_t* x, const float* xs, const int8_t* w, const float* ws, const bf16_t* bias,
+                                  float* part, int* count, int M, int N, int K, int form, bool once, hipStream_t stream) {
+  if (M <= LI_ROWS_MOST) {
+    const Int8Plan p = int8_plan(M, N, K, form);
+    return form == LI_SILU   ? linear_int8_rows_form<LI_SILU>(p, out, x, xs, w, ws, bias, part, count, M, N, K, once, stream)
+           : form == LI_PART ? linear_int8_rows_form<LI_PART>(p, out, x, xs, w, ws, bias, part, count, M, N, K, once, stream)
+                             : linear_int8_rows_form<LI_BF16>(p, out, x, xs, w, ws, bias, part, count, M, N, K, once, stream);
+  }
+  const bool gated = form == LI_SILU;
+  const int n = gated ? N / 2 : N;
+#define LI_CASE(MJ)                                                                                                 \
+  case MJ:                                                                                                          \
+    return gated ? linear_int8_tiles_go<1, MJ>(out, x, xs, w, ws, bias, part, count, M, n, K, stream)               \
+                 : linear_int8_tiles_go<0, MJ>(out, x, xs, w, ws, bias, part, count, M, n, K, stream)
+  switch (int8_tiles_pick(M, n, K, gated) & 15) {
+    LI_CASE(2);
+    LI_CASE(3);
+    LI_CASE(4);
+    LI_CASE(5);
+    LI_CASE(6);
+    LI_CASE(7);
+    LI_CASE(8);
+    default: return -1;
+  }
+#undef LI_CASE
+}

@@ -1,7 +1,9 @@
-// The inner loop of the large bf16 products, for gfx950: a workgroup of 4 waves, one on
+// The inner loop of the large bf16 and int8 products, for gfx950: a workgroup of 4 waves, one on
 // each SIMD of a compute unit, multiplies 256 rows of W (columns of the result) with 32 * MJ rows of X,
 // acc[i][j] of a wave = 16 columns i by 16 rows j of its 128 columns x 16 * MJ rows, in
-// v_mfma_f32_16x16x32_bf16 (W the A operand, so that a lane ends with 4 neighbouring columns of a row).
+// v_mfma_f32_16x16x32_bf16 (W the A operand, so that a lane ends with 4 neighbouring columns of a row). Whole numbers of
+// 8 bits go the same way in v_mfma_i32_16x16x64_i8, whose fragments are the same 16 bytes: a row of 2 n of them is one of n
+// bf16 everywhere below, and the sums' type says which it is.
 //
 // K goes by 64 ("stages") through a ring of LDS buffers, copied there straight from
 // memory (no registers in between). Rows of 128 bytes; the copy writes LDS in lane
@@ -39,6 +41,7 @@
 typedef __bf16 bf16x8_mfma __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x4_cvt __attribute__((ext_vector_type(4)));
 typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
 
 #define TP_N 256           // rows of W of a workgroup
 #define TP_K 64            // k of a stage
@@ -151,8 +154,8 @@ struct TileRing {
 
 // acc += W X^T over K; w: this wave's 8 * NI of the 32 * NI rows (64 of 256), x: its 8 * MJ of the 32 * MJ. Ends with all
 // waves past their last LDS read. NI 4, tiles of 128 columns, is for few rows: half the sums, more buffers in flight.
-template <int MJ, int NI = 8, int BYTES = TP_LDS, class W, class X>
-__device__ __forceinline__ void tile_product(f32x4 (&acc)[NI][MJ], const W& w, const X& x, int stages, int start,
+template <int MJ, int NI = 8, int BYTES = TP_LDS, class W, class X, class A>
+__device__ __forceinline__ void tile_product(A (&acc)[NI][MJ], const W& w, const X& x, int stages, int start,
                                              char* smem) {
   constexpr int STRIDE = TileRing<MJ, NI, BYTES>::STRIDE, RING = TileRing<MJ, NI, BYTES>::RING;
   constexpr int G = NI * MJ;             // matrix instructions of a half
@@ -204,7 +207,11 @@ __device__ __forceinline__ void tile_product(f32x4 (&acc)[NI][MJ], const W& w, c
   auto multiply = [&](int ks, int f) {
     if (f >= G) return;
     const int i = f / MJ, j = f % MJ;
-    acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[ks][i], b[ks][j], acc[i][j], 0, 0, 0);
+    if constexpr (std::is_same<A, i32x4>::value)
+      acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, a[ks][i]), __builtin_bit_cast(i32x4, b[ks][j]),
+                                                        acc[i][j], 0, 0, 0);
+    else
+      acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[ks][i], b[ks][j], acc[i][j], 0, 0, 0);
     if (f & 1) TP_HOLD;
   };
 
@@ -256,19 +263,19 @@ __device__ __forceinline__ void tile_product(f32x4 (&acc)[NI][MJ], const W& w, c
 }
 
 // Sums of a tile whose K is shared by ``shares`` workgroups: each leaves its own in part
-// [shares][8 * MJ][threads][4]; the last one to arrive adds them all up, in the order
+// [shares][NI * MJ][threads][4]; the last one to arrive adds them all up, in the order
 // of the shares whoever it is, and goes on (true) with the whole. count: 0 before.
 //
 // The sums are stored past the XCD's L2 and read past it (sc1), and each wave waits for its stores before the count. A
 // fence of the device's scope instead writes back and invalidates that whole L2, under everybody who works on it. 2048
 // columns, K 8192, in up to four shares of 64-row tiles: 150 rows 52 us with the fences, 33 without; 700 rows 70 and 47.
-template <int MJ>
-__device__ __forceinline__ bool tile_fold(f32x4 (&acc)[8][MJ], float* part, int share, int shares, int* count, char* smem) {
-  constexpr int SIZE = 8 * MJ * TP_THREADS * 16, SC1 = 16;
+template <int MJ, int NI, class A>
+__device__ __forceinline__ bool tile_fold(A (&acc)[NI][MJ], float* part, int share, int shares, int* count, char* smem) {
+  constexpr int SIZE = NI * MJ * TP_THREADS * 16, SC1 = 16;
   const int tid = threadIdx.x;
   const auto all = __builtin_amdgcn_make_buffer_rsrc(part, 0, shares * SIZE, 0x00020000);
 #pragma unroll
-  for (int i = 0; i < 8; ++i)
+  for (int i = 0; i < NI; ++i)
 #pragma unroll
     for (int j = 0; j < MJ; ++j)
       __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, acc[i][j]), all, tid * 16,
@@ -282,12 +289,12 @@ __device__ __forceinline__ bool tile_fold(f32x4 (&acc)[8][MJ], float* part, int 
   __syncthreads();                       // smem is free again
   // 32 loads of a thread at a time
 #pragma unroll
-  for (int i0 = 0; i0 < 8; i0 += 2) {
-    f32x4 sum[2][MJ];
+  for (int i0 = 0; i0 < NI; i0 += 2) {
+    A sum[2][MJ];
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
-      for (int j = 0; j < MJ; ++j) sum[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int j = 0; j < MJ; ++j) sum[i][j] = A{0, 0, 0, 0};
 #pragma unroll 1
     for (int s0 = 0; s0 < shares; s0 += 2) {
       u32x4 v[2][2][MJ];
@@ -313,7 +320,7 @@ __device__ __forceinline__ bool tile_fold(f32x4 (&acc)[8][MJ], float* part, int 
         for (int i = 0; i < 2; ++i)
 #pragma unroll
           for (int j = 0; j < MJ; ++j) {
-            const f32x4 x = __builtin_bit_cast(f32x4, v[e][i][j]);
+            const A x = __builtin_bit_cast(A, v[e][i][j]);
 #pragma unroll
             for (int r = 0; r < 4; ++r) sum[i][j][r] += x[r];
           }

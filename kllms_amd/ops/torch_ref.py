@@ -92,6 +92,43 @@ def silu_mul(gate: torch.Tensor, up: torch.Tensor) -> torch.Tensor:
     return (torch.nn.functional.silu(gate.float()) * up.float()).to(gate.dtype)
 
 
+# --- products in 8-bit integers -------------------------------------------------
+
+def quantize_rows(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Rows x [M, K] as whole numbers of -127..127, int8, and their scales fp32 [M]: x / scale to the nearest, halves to
+    even, scale = max |x| / 127. A row with a value that is no finite number has the scale NaN."""
+    x = x.float()
+    most = x.abs().amax(-1, keepdim=True) if x.shape[-1] else x.new_zeros(x.shape[0], 1)
+    sound = torch.isfinite(x).all(-1, keepdim=True)
+    e = torch.frexp(torch.where(sound, most, torch.ones_like(most))).exponent.clamp(min=-119) - 1
+    near = torch.ldexp(x, -e)                             # the largest one is near 1: 127 times it is a number
+    codes = torch.where((most > 0) & sound, torch.round(127 * near / torch.ldexp(most, -e)), torch.zeros_like(x))
+    return codes.to(torch.int8), torch.where(sound, most / 127, torch.full_like(most, float("nan"))).squeeze(-1)
+
+
+def quantize_weights(w: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Weights [N, K] as (int8 [N, K], fp32 [N]): a scale for each output channel, as quantize_rows has one for each row."""
+    return quantize_rows(w)
+
+
+def linear_int8(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, bias=None) -> torch.Tensor:
+    """(quantized x) w^T with both scales (+ bias), fp32 before the rounding to x's dtype; w int8 [N, K], w_scale fp32 [N]."""
+    return _linear_int8(x, w, w_scale, bias).to(x.dtype)
+
+
+def _linear_int8(x, w, w_scale, bias=None) -> torch.Tensor:
+    codes, scales = quantize_rows(x)
+    sums = codes.double() @ w.double().t()                # whole numbers, exact
+    y = sums.float() * scales[:, None] * w_scale
+    return y if bias is None else y + bias.float()
+
+
+def linear_silu_int8(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor) -> torch.Tensor:
+    """silu(gate) * up of a fused [gate; up] int8 matrix."""
+    gate, up = _linear_int8(x, w, w_scale).chunk(2, -1)
+    return (torch.nn.functional.silu(gate) * up).to(x.dtype)
+
+
 # --- paged KV cache -----------------------------------------------------------
 
 KV4_GROUP = 64

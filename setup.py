@@ -33,6 +33,7 @@ SOURCES = [
         "moe.hip",
         "linear_rows.hip",
         "linear_tiles.hip",
+        "linear_int8.hip",
         "decode_rows.hip",
         "levenshtein.hip",
     )

@@ -1,0 +1,67 @@
+"""Products in 8-bit integers on the CPU: the form of the codes, refusals."""
+
+import pytest
+import torch
+
+from kllms_amd import ops
+
+
+def test_rows_are_rounded_to_the_nearest_of_255():
+    x = (torch.randn(40, 96) * torch.exp(torch.randn(40, 1) * 5)).bfloat16()
+    x[3] = 0
+    codes, scales = ops.quantize_rows(x)
+    assert codes.dtype == torch.int8 and int(codes.max()) == 127 or int(codes.min()) == -127
+    back = codes.double() * scales.double()[:, None]
+    # half a scale, and the scale's own rounding (2^-24 of it) 127 times
+    assert bool(((back - x.double()).abs() <= scales.double()[:, None] * (0.5 + 127 * 2 ** -24)).all())
+    assert bool((codes[3] == 0).all()) and float(scales[3]) == 0
+
+
+def test_halves_go_to_the_even_number():
+    x = torch.zeros(1, 16, dtype=torch.bfloat16)
+    x[0, :3] = torch.tensor([254.0, 1.0, 3.0])               # 127 / 254: 0.5 and 1.5
+    codes, _ = ops.quantize_rows(x)
+    assert codes[0, :3].tolist() == [127, 0, 2]
+
+
+def test_rows_of_any_size_and_rows_that_are_none():
+    x = torch.randn(5, 32).bfloat16()
+    x[0], x[1] = x[0] * 2.0 ** -130, x[1] * 2.0 ** 120
+    x[0, 0], x[1, 0] = 2.0 ** -127, 3e38
+    x[2, 7], x[3, 9] = float("nan"), float("inf")
+    codes, scales = ops.quantize_rows(x)
+    assert torch.isnan(scales).tolist() == [False, False, True, True, False]
+    for r in (0, 1, 4):
+        want = torch.round(127 * x[r].double() / x[r].double().abs().max())
+        assert torch.equal(codes[r].double(), want)
+
+
+@pytest.mark.parametrize("gated", [False, True])
+def test_product_against_64_bits(gated):
+    x, w = torch.randn(7, 80).bfloat16(), torch.randn(64, 80)
+    wc, ws = ops.quantize_weights(w)
+    xc, xs = ops.quantize_rows(x)
+    y = (xc.double() @ wc.double().t()) * xs.double()[:, None] * ws.double()
+    if gated:
+        got, y = ops.linear_silu_int8(x, wc, ws), torch.sigmoid(y[:, :32]) * y[:, :32] * y[:, 32:]
+    else:
+        b = torch.randn(64).bfloat16()
+        got, y = ops.linear_int8(x, wc, ws, b), y + b.double()
+    assert got.dtype == x.dtype
+    # rounded to bf16 once (half of 2^-7), fp32 before
+    assert bool(((got.double() - y).abs() <= 2 ** -8 * y.abs() + 1e-5).all())
+    # and the quantization itself stays near the product of what was there
+    if not gated:
+        full = x.double() @ w.double().t() + b.double()
+        err = 0.5 * xs.double()[:, None] * w.double().abs().sum(1) + 0.5 * (x.double().abs().sum(1)[:, None] + 40 * xs.double()[:, None]) * ws.double()
+        assert bool(((got.double() - full).abs() <= err * 1.01 + 2 ** -7 * full.abs()).all())
+
+
+def test_refusals():
+    x, w, s = torch.zeros(2, 16), torch.zeros(6, 16, dtype=torch.int8), torch.ones(6)
+    for call in (lambda: ops.linear_int8(x, w.float(), s), lambda: ops.linear_int8(x[:, :8], w, s), lambda: ops.linear_int8(x[0], w, s),
+                 lambda: ops.linear_silu_int8(x, w[:5], s[:5]), lambda: ops.quantize_rows(x[0]), lambda: ops.quantize_weights(x[0])):
+        with pytest.raises(ValueError):
+            call()
+    with pytest.raises(RuntimeError, match="no gradient"):
+        ops.linear_int8(x.requires_grad_(), w, s)
