@@ -1145,6 +1145,11 @@ class EngineConfig(BaseModel):
     weights_path: Optional[str] = None  # safetensors dir; None = random init
     dtype: Literal["bfloat16", "float32", "float16"] = "bfloat16"
     seed: int = 0
+    # "bf16" (the compute dtype) or "int8": the projections of attention and
+    # feed-forward in 8-bit integers with a scale for each output channel, their
+    # inputs with one for each token (dense models, and a mixture's attention;
+    # embedding, head, norms and experts keep their type)
+    weight_dtype: Literal["bf16", "int8"] = "bf16"
 
     # Parallelism: TP over RCCL/xGMI (one process per GPU)
     tp_size: int = 1

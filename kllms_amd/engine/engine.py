@@ -252,6 +252,10 @@ class LLMEngine:
             model.to_device(self.device)
             model.random_init_(self.config.seed)
         model.eval()
+        if self.config.weight_dtype == "int8":
+            if not hasattr(model, "quantize_weights_"):
+                raise ValueError(f"weight_dtype='int8' is for dense and mixture models: {self.arch.arch} is another")
+            model.quantize_weights_()
         return model
 
     def _build_state_cache(self) -> PagedKVCache:

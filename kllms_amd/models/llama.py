@@ -132,6 +132,8 @@ class LlamaMLP(nn.Module):
         """silu(gate) * up."""
         p = self.gate_up_proj
         plain = ops.only_weights(p, ColumnParallelLinear) and ops.no_global_hooks()
+        if plain and p.bias is None and p.weight.dtype == torch.int8:
+            return ops.linear_silu_int8(x, p.weight, p.weight_scale, p.once)
         act = ops.linear_silu(x, p.weight) if plain and p.bias is None else None
         if act is not None:
             return act
@@ -356,6 +358,27 @@ class LlamaForCausalLM(nn.Module):
                 read += (up.weight, down.weight)
         return ops.rows_weights_ok(read, input_ids)
 
+    def quantize_weights_(self) -> None:
+        """Holds the projections of attention and feed-forward in 8-bit integers (ops.linear_int8); embedding, norms, head
+        and experts keep their type."""
+        kinds = (ColumnParallelLinear, RowParallelLinear)
+        layers = [m for m in self.modules() if isinstance(m, kinds)]
+        for m in layers:
+            if m.weight.is_cuda and (m.weight.shape[1] % 16 or m.weight.shape[0] % 32):
+                raise ValueError(f"int8 weights on the GPU have a multiple of 32 rows of a multiple of 16: {list(m.weight.shape)}")
+        for m in layers:
+            m.quantize_()
+        self._once = ops.weights_once(self)
+        for m in layers:
+            m.quantize_(self._once)
+
+    @staticmethod
+    def _sums(x: torch.Tensor, p, once: bool) -> torch.Tensor:
+        """fp32 sums [S, M, N] of a few rows with a projection's weights."""
+        if p.weight.dtype == torch.int8:
+            return ops.linear_part_int8(x, p.weight, p.weight_scale, once)
+        return ops.linear_part(x, p.weight, once)
+
     _unknown: Optional[torch.Tensor] = None
 
     def _unknown_ids(self) -> torch.Tensor:
@@ -394,16 +417,17 @@ class LlamaForCausalLM(nn.Module):
             if batch.mode == "prefill":
                 att = at.attend(x, batch, self.cos_sin)
             else:
-                q = ops.rope_store_rows(ops.linear_part(x, at.qkv_proj.weight, once), at.qkv_proj.bias, at.num_heads,
+                q = ops.rope_store_rows(self._sums(x, at.qkv_proj, once), at.qkv_proj.bias, at.num_heads,
                                         batch.positions, self.cos_sin, k_cache, v_cache, batch.slot_mapping, k_scale, v_scale)
                 att = at.attend_cache(q, batch, arrived)
-            x = ops.add_norm_rows(ops.linear_part(att.view(T, -1), at.o_proj.weight, once), residual, norm.weight, norm.eps)
+            x = ops.add_norm_rows(self._sums(att.view(T, -1), at.o_proj, once), residual, norm.weight, norm.eps)
             norm = layers[i + 1].input_layernorm if i + 1 < len(layers) else self.norm
             mlp = layer.mlp
             if isinstance(mlp, LlamaMLP):
                 w = mlp.gate_up_proj.weight
-                act = (ops.linear_silu_rows(x, w, once) if self._silu_rows(T, w) or self._silu_streams(T, w) else mlp.activate(x))
-                x = ops.add_norm_rows(ops.linear_part(act, mlp.down_proj.weight, once), residual, norm.weight, norm.eps)
+                act = (ops.linear_silu_rows(x, w, once) if w.dtype == torch.bfloat16 and (self._silu_rows(T, w) or self._silu_streams(T, w))
+                       else mlp.activate(x))
+                x = ops.add_norm_rows(self._sums(act, mlp.down_proj, once), residual, norm.weight, norm.eps)
             else:
                 x, residual = ops.fused_add_rmsnorm(mlp(x), residual, norm.weight, norm.eps)
         return x

@@ -480,7 +480,8 @@ def quantize_weights(w: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     """(int8 [N, K], scales fp32 [N]) of a weight matrix [N, K] of any float type, for linear_int8."""
     if w.dim() != 2:
         raise ValueError(f"weights [N, K]: got {list(w.shape)}")
-    return torch_ref.quantize_weights(w)
+    parts = [torch_ref.quantize_weights(p) for p in w.split(4096)]       # their fp32 copies are not all there at once
+    return torch.cat([p[0] for p in parts]), torch.cat([p[1] for p in parts])
 
 
 def linear_int8(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, bias: Optional[torch.Tensor] = None,

@@ -58,7 +58,32 @@ class ParallelContext:
         return torch.cat(parts, dim=dim)
 
 
-class ColumnParallelLinear(nn.Module):
+class _QuantizableLinear(nn.Module):
+    """A linear layer whose weight can be held in 8-bit integers with a scale for each output channel of this rank's
+    shard; its input rows are then quantized as they come (ops.linear_int8)."""
+
+    once = False
+
+    def __init__(self):
+        super().__init__()
+        self.register_parameter("weight_scale", None)      # fp32 [N] of an int8 weight
+
+    @torch.no_grad()
+    def quantize_(self, once: bool = False) -> None:
+        """Replaces the weight by its int8 form. ``once``: ops.weights_once of the model that it belongs to."""
+        if self.weight.dtype != torch.int8:
+            codes, scales = ops.quantize_weights(self.weight)
+            self.weight = nn.Parameter(codes, requires_grad=False)
+            self.weight_scale = nn.Parameter(scales, requires_grad=False)
+        self.once = once
+
+    def _product(self, x: torch.Tensor, bias: Optional[torch.Tensor]) -> torch.Tensor:
+        if self.weight.dtype == torch.int8:
+            return ops.linear_int8(x, self.weight, self.weight_scale, bias, self.once)
+        return ops.linear(x, self.weight, bias)
+
+
+class ColumnParallelLinear(_QuantizableLinear):
     """Y = X W^T with W row-sharded over ranks (output features split).
 
     No communication on forward; the sharded output feeds a row-parallel
@@ -105,10 +130,10 @@ class ColumnParallelLinear(nn.Module):
         return torch.cat(pieces, dim=0)
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
-        return ops.linear(x, self.weight, self.bias)
+        return self._product(x, self.bias)
 
 
-class RowParallelLinear(nn.Module):
+class RowParallelLinear(_QuantizableLinear):
     """Y = X W^T with W column-sharded over ranks (input features split);
     forward ends with one RCCL all-reduce (the per-layer TP boundary)."""
 
@@ -123,7 +148,7 @@ class RowParallelLinear(nn.Module):
         )
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
-        y = ops.linear(x, self.weight)
+        y = self._product(x, None)
         return self.ctx.all_reduce(y)
 
 

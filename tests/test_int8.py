@@ -65,3 +65,47 @@ def test_refusals():
             call()
     with pytest.raises(RuntimeError, match="no gradient"):
         ops.linear_int8(x.requires_grad_(), w, s)
+
+
+def engine(**more):
+    from kllms_amd.engine.config import EngineConfig
+    from kllms_amd.engine.engine import LLMEngine
+
+    return LLMEngine(EngineConfig(**{**dict(model="tiny-llama", max_kv_blocks=256, use_hip_graphs=False, device="cpu", seed=0,
+                                            weight_dtype="int8"), **more}))
+
+
+@pytest.mark.parametrize("model", ["tiny-llama", "tiny-mixtral", "tiny-qwen2"])
+def test_engine_generates(model):
+    from kllms_amd.engine.config import MODEL_PRESETS
+    from kllms_amd.engine.engine import GenRequest
+    from kllms_amd.engine.sampling import SamplingParams
+
+    if model not in MODEL_PRESETS:
+        pytest.skip("no such preset")
+    eng = engine(model=model, kv_cache_dtype="int4")
+    at = eng.model.layers[0].self_attn
+    assert at.qkv_proj.weight.dtype == at.o_proj.weight.dtype == torch.int8 and eng.model.embed_tokens.weight.dtype != torch.int8
+    out = eng.generate([GenRequest(prompt_ids=list(range(1, 30)), n=2, sampling=SamplingParams(temperature=0.0, max_new_tokens=6))])[0]
+    assert out.streams[0].token_ids == out.streams[1].token_ids and len(out.streams[0].token_ids) >= 1
+
+
+def test_layers_are_the_operator():
+    eng, plain = engine(), engine(weight_dtype="bf16")
+    p, q = eng.model.layers[0].mlp.down_proj, plain.model.layers[0].mlp.down_proj
+    codes, scales = ops.quantize_weights(q.weight)
+    assert torch.equal(p.weight, codes) and torch.equal(p.weight_scale, scales)
+    x = torch.randn(3, p.weight.shape[1])
+    assert torch.equal(p(x), ops.linear_int8(x, codes, scales))
+    eng.model.quantize_weights_()                        # once is enough
+    assert torch.equal(p.weight, codes)
+    mlp, plain_mlp = eng.model.layers[0].mlp, plain.model.layers[0].mlp
+    x = torch.randn(3, plain_mlp.gate_up_proj.weight.shape[1])
+    got, want = mlp(x), plain_mlp(x)
+    # rounded to 255 steps twice: each product's terms are off by 1/127 of the largest at most, near 0.3 % of it on average
+    assert float((got - want).norm()) < 0.05 * float(want.norm())
+
+
+def test_other_families_are_refused():
+    with pytest.raises(ValueError, match="int8"):
+        engine(model="tiny-zutalix")
