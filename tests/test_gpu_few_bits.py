@@ -1,0 +1,87 @@
+"""The engine on the GPU with weights in 8-bit integers and a 4-bit cache: whole runs of the operators together."""
+
+import pytest
+import torch
+
+from kllms_amd import ops
+from kllms_amd.engine.config import EngineConfig
+from kllms_amd.engine.engine import GenRequest, LLMEngine
+from kllms_amd.engine.sampling import SamplingParams
+from kllms_amd.models.llama import ForwardBatch
+from kllms_amd.ops import torch_ref
+
+pytestmark = pytest.mark.gpu
+
+
+def engine(**more):
+    return LLMEngine(EngineConfig(**{**dict(model="mid-llama", max_kv_blocks=512, use_hip_graphs=False, device="cuda:0", seed=0), **more}))
+
+
+def requests(n=3, tokens=12):
+    g = torch.Generator().manual_seed(0)
+    return [GenRequest(prompt_ids=torch.randint(1, 400, (k,), generator=g).tolist(), n=n,
+                       sampling=SamplingParams(temperature=0.0, max_new_tokens=tokens)) for k in (40, 3, 170)]
+
+
+@pytest.mark.parametrize("weight,cache", [("bf16", "int4"), ("int8", "bf16"), ("int8", "fp8_e4m3"), ("int8", "int4")])
+@pytest.mark.parametrize("model", ["mid-llama", "mid-mixtral"])
+def test_graphs_give_what_eager_steps_give(model, weight, cache):
+    runs = []
+    for graphs in (False, True):
+        eng = engine(model=model, weight_dtype=weight, kv_cache_dtype=cache, use_hip_graphs=graphs, hip_graph_batch_sizes=[9, 16])
+        runs.append([[s.token_ids for s in o.streams] for o in eng.generate(requests())])
+        if graphs:
+            assert eng._graph_runner._enabled and eng._graph_runner.graphs
+    assert runs[0] == runs[1]
+    assert all(len(t) > 0 for o in runs[0] for t in o)
+
+
+def test_a_step_on_the_few_row_kernels_is_one_of_the_modules():
+    """The step's sums in shares against the layers' own calls: the same whole numbers, rounded at other places."""
+    eng = engine(weight_dtype="int8", kv_cache_dtype="int4")
+    model, kv = eng.model, eng.kv
+    B, ctx = 5, 70
+    g = torch.Generator().manual_seed(1)
+    per = -(-ctx // 16)
+    tables = torch.arange(B * per, dtype=torch.int32).view(B, per).cuda()
+    slots = torch.arange(B * per * 16).view(B, -1)[:, :ctx].reshape(-1).cuda()
+    for k, v, ks, vs in kv.layer_caches():
+        rows = torch.randn(2, B * ctx, k.shape[1], 128, generator=g).bfloat16().cuda()
+        ops.store_kv(rows[0], rows[1], k, v, slots, ks, vs)
+    batch = ForwardBatch(mode="decode", positions=torch.full((B,), ctx - 1, device="cuda"), kv_caches=kv.layer_caches(), block_tables=tables,
+                         slot_mapping=slots.view(B, ctx)[:, -1].contiguous(), context_lens=torch.full((B,), ctx, dtype=torch.int32, device="cuda"))
+    ids = torch.arange(3, 3 + B, device="cuda")
+    with torch.inference_mode():
+        assert model._takes_rows(ids, batch)
+        got = model.forward_hidden(ids, batch).float()
+        hidden, residual = model.embed_tokens(ids), None
+        for layer in model.layers:
+            hidden, residual = layer(hidden, residual, batch, model.cos_sin)
+        want = ops.fused_add_rmsnorm(hidden, residual, model.norm.weight, model.norm.eps)[0].float()
+    # a bf16 rounding that falls differently moves a row's codes by one of 127 steps here and there
+    assert float((got - want).norm()) < 0.03 * float(want.norm())
+
+
+@pytest.mark.parametrize("cache", ["int4"])
+def test_prompts_behind_a_cached_prefix(cache):
+    """Whole prompts, then others with the same head, whose tails attend over the 4-bit cache."""
+    eng = engine(kv_cache_dtype=cache, weight_dtype="int8", prefix_cache_min_tokens=32, max_seq_len=1024)
+    head = list(range(5, 5 + 160))
+    first = [GenRequest(prompt_ids=head + [7] * 40, n=1, sampling=SamplingParams(temperature=0.0, max_new_tokens=4))]
+    eng.generate(first)
+    g = torch.Generator().manual_seed(2)
+    tails = [GenRequest(prompt_ids=head + torch.randint(1, 400, (k,), generator=g).tolist(), n=2,
+                        sampling=SamplingParams(temperature=0.0, max_new_tokens=5)) for k in (1, 33, 90, 300)]
+    outs = eng.generate(tails)
+    alone = [eng.generate([t])[0] for t in tails]
+    for o, a in zip(outs, alone):
+        assert o.streams[0].token_ids == o.streams[1].token_ids and len(o.streams[0].token_ids) > 0
+        assert len(a.streams[0].token_ids) > 0
+
+
+def test_int8_weights_hold_half_the_bytes():
+    eng = engine(weight_dtype="int8")
+    at = eng.model.layers[0].self_attn
+    assert at.qkv_proj.weight.dtype == torch.int8 and at.qkv_proj.weight.is_cuda
+    codes, scales = torch_ref.quantize_weights(at.qkv_proj.weight.float().cpu() * at.qkv_proj.weight_scale.cpu()[:, None])
+    assert torch.equal(codes, at.qkv_proj.weight.cpu())
