@@ -20,8 +20,11 @@
 //   max      renewed only when a score passes it by more than 8 (in powers of two), which leaves p s below fp16's end
 //   steps    p s is scaled by the power of two above the largest step of V so far, renewed like the max
 //
-// Nothing goes through LDS before the end. Key 4 r + c of 16 is row 4 c + r of a score tile: the rows that an instruction
-// loads of V, four of 64 bytes, are neighbours in memory then.
+// A wave's tile goes to a strip of LDS that is its own, straight from memory and as it lies there: nine loads of whole lines
+// for 64 keys, without registers in between or barriers; the next K is on its way as soon as this one's fragments are read, the next V
+// behind P V. (Loaded to registers by the fragments' own pattern, 4 + 16 + 16 loads whose lanes lie in many rows, the address
+// unit was the bound: 16 streams of 6100 33 us, one of 131071 with eight heads to a kv head 48.) A row's 16-byte units are
+// XORed with its key: both kinds of reads are free of bank conflicts. Key 4 r + c of 16 is row 4 c + r of a score tile.
 //
 // What bounds it: the cache's bytes where contexts are many or long, else the chain of loads of one tile.
 
@@ -33,6 +36,7 @@ typedef _Float16 f16x8_mfma __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x2_cvt __attribute__((ext_vector_type(2)));
 typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
 typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 
 #define NTHREADS 256
@@ -131,7 +135,7 @@ __device__ __forceinline__ void merge4(bf16_t* __restrict__ out, const float* al
 
 // WHOLE: blocks of a multiple of 16 keys
 template <int GQA, bool WHOLE>
-__global__ __launch_bounds__(NTHREADS, 3) void attn_decode4_kernel(
+__global__ __launch_bounds__(NTHREADS, GQA == 8 || !WHOLE ? 3 : 4) void attn_decode4_kernel(
     float* __restrict__ partials,          // [B, KVH, Z, GQA, PART_STRIDE]
     bf16_t* __restrict__ out,              // written where one workgroup has the context, or by the last one with ``arrived``
     const bf16_t* __restrict__ q,          // [B, H, 128], row stride q_stride
@@ -140,7 +144,10 @@ __global__ __launch_bounds__(NTHREADS, 3) void attn_decode4_kernel(
     const int* __restrict__ block_tables, const int* __restrict__ context_lens, int* __restrict__ arrived, int apart,
     float scale, int block_size, uint32_t block_inverse, int max_blocks, int64_t q_stride, Decode4Shares shares) {
   constexpr int SETS = 16 / GQA;
-  __shared__ __attribute__((aligned(16))) float o_lds[4][16][PART_STRIDE];
+  constexpr int STRIP = 2 * TKEYS * KV4_BYTES + 2 * TKEYS * 8;
+  static_assert(STRIP >= 16 * PART_STRIDE * 4);
+  __shared__ __attribute__((aligned(1024))) char strips[4][STRIP];
+  float (&o_lds)[4][STRIP / 4] = reinterpret_cast<float(&)[4][STRIP / 4]>(strips);      // at the end: a wave's sums, [16][PART_STRIDE]
   __shared__ float m_lds[4][16], l_lds[4][16];
   __shared__ int last_lds;
   const int g_kv = blockIdx.x, num_kv_heads = gridDim.x, b = blockIdx.y, z = blockIdx.z;
@@ -211,9 +218,32 @@ __global__ __launch_bounds__(NTHREADS, 3) void attn_decode4_kernel(
     return n - (rest < 0) + (rest >= block_size);
   };
 
-  u32x4 kraw[4];
-  uint32_t vraw[4][4];
-  u32x2 ks[GQA], vs[GQA];
+  // ---- the strip: K of a tile, V, (step, least) of both -----------------------------------------
+  char* const strip = strips[wave];
+  typedef __attribute__((address_space(3))) char* lds_t;
+  typedef __attribute__((address_space(3))) const u32x4* lds_v4;
+  typedef __attribute__((address_space(3))) const u32x2* lds_v2;
+  typedef __attribute__((address_space(3))) const uint32_t* lds_v1;
+  const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_t)strip);
+  constexpr int V_AT = TKEYS * KV4_BYTES, S_AT = 2 * V_AT, VS_AT = S_AT + TKEYS * 8;
+  // a load's lane has 16 bytes of row lane / 4 of sixteen
+  const int put_row = lane >> 2;
+  const uint32_t put_off = put_row * KV4_BYTES + (((lane & 3) ^ (put_row >> 2)) << 4);
+  const int k_key = 4 * (col & 3) + (col >> 2);        // key of row ``col`` of a score tile
+  uint32_t k_get = lds0 + k_key * KV4_BYTES + ((grp ^ (k_key >> 2)) << 4);
+  uint32_t v_get = lds0 + V_AT + grp * KV4_BYTES + col * 4;          // word col of key grp, the unit XORed with the key's r
+  uint32_t s_get = lds0 + S_AT + key_in_tile(0) * 8;
+  auto put = [&](const char* rows, uint32_t lane_off, uint32_t at) {
+    const uint64_t r = (uint64_t)rows;
+    const u32x2 from = {(uint32_t)__builtin_amdgcn_readfirstlane((int)r), (uint32_t)__builtin_amdgcn_readfirstlane((int)(r >> 32))};
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(lane_off), "s"(from), "s"(at) : "memory");
+  };
+  auto put_at = [&](const char* from, uint32_t at) {
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(from), "s"(at) : "memory");
+  };
+  auto put_word = [&](const uint32_t* from, uint32_t at) {
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(from), "s"(at) : "memory");
+  };
   constexpr int IDS = WHOLE ? 4 : 1;
   int ids[IDS];                            // WHOLE: blocks of a tile's four sixteens; else the block of this lane's key
   auto ask = [&](int t) {
@@ -223,54 +253,40 @@ __global__ __launch_bounds__(NTHREADS, 3) void attn_decode4_kernel(
       ids[i] = bt[block_of(key)];
     }
   };
-  const int k_row = 4 * (col & 3) + (col >> 2);        // key of row ``col`` of a score tile
-  auto load_k = [&](int t, const int64_t (&base)[4], int row) {
-    if constexpr (WHOLE) {
+  auto load_rows = [&](const uint32_t* cache, uint32_t to, const i32x4& base, int row) {    // 4 loads
 #pragma unroll
-      for (int tt = 0; tt < 4; ++tt) kraw[tt] = *reinterpret_cast<const u32x4*>(k_cache + base[tt] * 16 + (k_row * 16 + grp * 4));
-#pragma unroll
-      for (int i = 0; i < GQA; ++i) {
-        const int key = key_in_tile(i), tt = key >> 4;
-        int64_t at = base[0];
-        if constexpr (GQA >= 4) {
-          at = base[GQA == 8 ? i >> 1 : i];
-        } else {
-#pragma unroll
-          for (int e = 1; e < 4; ++e) at = tt == e ? base[e] : at;
-        }
-        ks[i] = *reinterpret_cast<const u32x2*>(k_scale + (at + (key & 15)) * 2);
-        vs[i] = *reinterpret_cast<const u32x2*>(v_scale + (at + (key & 15)) * 2);
-      }
-    } else {
-#pragma unroll
-      for (int tt = 0; tt < 4; ++tt) {
-        const int64_t r = __shfl(row, 16 * tt + k_row);
-        kraw[tt] = *reinterpret_cast<const u32x4*>(k_cache + r * 16 + grp * 4);
-      }
-#pragma unroll
-      for (int i = 0; i < GQA; ++i) {
-        const int64_t r = __shfl(row, key_in_tile(i));
-        ks[i] = *reinterpret_cast<const u32x2*>(k_scale + r * 2);
-        vs[i] = *reinterpret_cast<const u32x2*>(v_scale + r * 2);
+    for (int tt = 0; tt < 4; ++tt) {
+      if constexpr (WHOLE) {
+        put((const char*)cache + (int64_t)base[tt] * KV4_BYTES, put_off, to + tt * 16 * KV4_BYTES);
+      } else {
+        const int64_t r = __shfl(row, 16 * tt + put_row);
+        put_at((const char*)cache + r * KV4_BYTES + (((lane & 3) ^ (put_row >> 2)) << 4), to + tt * 16 * KV4_BYTES);
       }
     }
   };
-  auto load_v = [&](const int64_t (&base)[4], int row) {
+  constexpr int SCALE_LOADS = WHOLE ? 1 : 4;
+  auto load_scales = [&](const i32x4& base, int row) {
+    if constexpr (WHOLE) {                 // two keys a lane, K's in the lower half of the wave
+      const int at = lane & 31, tt = at >> 3;
+      int r = base[0];
 #pragma unroll
-    for (int tt = 0; tt < 4; ++tt)
+      for (int e = 1; e < 4; ++e) r = tt == e ? base[e] : r;
+      put_at((const char*)(lane < 32 ? k_scale : v_scale) + ((int64_t)r * 8 + (at & 7) * 16), lds0 + S_AT);
+    } else {                               // a word a lane
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        if constexpr (WHOLE) vraw[tt][r] = v_cache[base[tt] * 16 + ((4 * r + grp) * 16 + col)];
-        else vraw[tt][r] = v_cache[(int64_t)__shfl(row, 16 * tt + 4 * r + grp) * 16 + col];
+      for (int e = 0; e < 4; ++e) {
+        const int64_t r = __shfl(row, (e & 1) * 32 + (lane >> 1));
+        put_word((e < 2 ? k_scale : v_scale) + r * KV4_GROUPS + (lane & 1), lds0 + S_AT + e * 256);
       }
+    }
   };
   // rows of the cache: of the four sixteens' first keys, or of this lane's key; those behind the context repeat what is in it
-  auto rows_of = [&](int t, int64_t (&base)[4], int& row) {
+  auto rows_of = [&](int t, i32x4& base, int& row) {
     if constexpr (WHOLE) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int key = min(t * TKEYS + i * 16, (L - 1) & ~15);
-        base[i] = ((int64_t)ids[i] * num_kv_heads + g_kv) * block_size + (key - block_of(key) * block_size);
+        base[i] = __builtin_amdgcn_readfirstlane((ids[i] * num_kv_heads + g_kv) * block_size + (key - block_of(key) * block_size));
       }
     } else {
       const int key = min(t * TKEYS + lane, L - 1);
@@ -286,13 +302,14 @@ __global__ __launch_bounds__(NTHREADS, 3) void attn_decode4_kernel(
 
   const int step = Z * 4;
   int t = z * 4 + wave;
-  int64_t base[4];
+  i32x4 base = {0, 0, 0, 0};
   int row = 0;
   if (t < tiles) {
     ask(t);
     rows_of(t, base, row);
-    load_k(t, base, row);
-    load_v(base, row);
+    load_rows(k_cache, lds0, base, row);
+    load_scales(base, row);
+    load_rows(v_cache, lds0 + V_AT, base, row);
     ask(min(t + step, tiles - 1));
   }
 #pragma unroll 1
@@ -302,10 +319,28 @@ __global__ __launch_bounds__(NTHREADS, 3) void attn_decode4_kernel(
       rows_of(t + step, base, row);
       ask(min(t + 2 * step, tiles - 1));
     }
+    // ---- K's fragments and the scales are there (V is not): to registers, and the next ones on their way -------
+    u32x4 kraw[4];
+    u32x2 ks[GQA], vs[GQA];
+    asm volatile("s_waitcnt vmcnt(4)" : "+v"(k_get), "+v"(v_get), "+v"(s_get)::"memory");      // not all their addresses for the whole loop
+#pragma unroll
+    for (int tt = 0; tt < 4; ++tt) kraw[tt] = *(lds_v4)(uintptr_t)(k_get + tt * 16 * KV4_BYTES);
+#pragma unroll
+    for (int i = 0; i < GQA; ++i) {
+      const int more_keys = GQA == 8 ? 16 * (i >> 1) + 4 * (i & 1) : 16 * i;     // key_in_tile(i) - key_in_tile(0)
+      ks[i] = *(lds_v2)(uintptr_t)(s_get + more_keys * 8);
+      vs[i] = *(lds_v2)(uintptr_t)(s_get + (VS_AT - S_AT) + more_keys * 8);
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    if (more) {
+      load_rows(k_cache, lds0, base, row);
+      load_scales(base, row);
+    }
+    __builtin_amdgcn_sched_barrier(0);
     // ---- scores of whole numbers, a group at a time ---------------------------------------
     float x[GQA];
     {
-      f32x4 acc[4][2];
+      float sums[2][GQA];                  // of this lane's keys: of the registers of all sets, this one's
 #pragma unroll
       for (int tt = 0; tt < 4; ++tt) {
         Frag4 f[4];
@@ -320,53 +355,41 @@ __global__ __launch_bounds__(NTHREADS, 3) void attn_decode4_kernel(
         const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int g = 0; g < 2; ++g) {
-          acc[tt][g] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f[2 * g].m, qf[2 * g].m, zero, 0, 0, 0);
-          acc[tt][g] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f[2 * g + 1].m, qf[2 * g + 1].m, acc[tt][g], 0, 0, 0);
+          f32x4 acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(f[2 * g].m, qf[2 * g].m, zero, 0, 0, 0);
+          acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(f[2 * g + 1].m, qf[2 * g + 1].m, acc, 0, 0, 0);
+          if constexpr (GQA == 8) {
+            sums[g][2 * tt] = set ? acc[2] : acc[0];
+            sums[g][2 * tt + 1] = set ? acc[3] : acc[1];
+          } else {
+            const float lo = set & 1 ? acc[1] : acc[0], hi = set & 1 ? acc[3] : acc[2], mine = set & 2 ? hi : lo;
+            const int i = GQA == 4 ? tt : GQA == 2 ? tt & 1 : 0;
+            if (GQA == 4 || tt < GQA) sums[g][i] = mine;
+            else sums[g][i] = (GQA == 2 ? set >> 2 == tt >> 1 : set >> 2 == tt) ? mine : sums[g][i];
+          }
         }
+        __builtin_amdgcn_sched_barrier(0);
       }
-      auto mine = [&](int i, int g) {      // of the registers of all sets, this one's
-        if constexpr (GQA == 8) return set ? acc[i >> 1][g][2 + (i & 1)] : acc[i >> 1][g][i & 1];
-        auto of = [&](int tt) {
-          const f32x4 a = acc[tt][g];
-          const float lo = set & 1 ? a[1] : a[0], hi = set & 1 ? a[3] : a[2];
-          return set & 2 ? hi : lo;
-        };
-        if constexpr (GQA == 4) return of(i);
-        if constexpr (GQA == 2) return set & 4 ? of(2 + i) : of(i);
-        const float lo = set & 4 ? of(1) : of(0), hi = set & 4 ? of(3) : of(2);
-        return set & 8 ? hi : lo;
-      };
 #pragma unroll
       for (int i = 0; i < GQA; ++i) {
-        const float whole = __builtin_fmaf(kv4_step(ks[i][1]), mine(i, 1), kv4_step(ks[i][0]) * mine(i, 0));
+        const float whole = __builtin_fmaf(kv4_step(ks[i][1]), sums[1][i], kv4_step(ks[i][0]) * sums[0][i]);
         const float low = __builtin_fmaf(kv4_least(ks[i][1]), q_sum[1], kv4_least(ks[i][0]) * q_sum[0]);
         x[i] = __builtin_fmaf(whole, q_back, low);
       }
     }
-    float v_step[GQA][2], v_low[GQA][2];
-#pragma unroll
-    for (int i = 0; i < GQA; ++i)
-#pragma unroll
-      for (int g = 0; g < 2; ++g) {
-        v_step[i][g] = kv4_step(vs[i][g]);
-        v_low[i][g] = kv4_least(vs[i][g]);
-      }
     if (t * TKEYS + TKEYS > L) {           // what lies behind the context is another's
 #pragma unroll
       for (int i = 0; i < GQA; ++i)
         if (t * TKEYS + key_in_tile(i) >= L) {
           x[i] = -INFINITY;
-#pragma unroll
-          for (int g = 0; g < 2; ++g) v_step[i][g] = v_low[i][g] = 0.0f;
+          vs[i] = u32x2{0u, 0u};
         }
     }
-    if (more) load_k(t + step, base, row);
     // ---- the max and the largest step, renewed when they have to be ---------------------------
-    float top = x[0], wide = fmaxf(v_step[0][0], v_step[0][1]);
+    float top = x[0], wide = 0.0f;
 #pragma unroll
-    for (int i = 1; i < GQA; ++i) {
+    for (int i = 0; i < GQA; ++i) {
       top = fmaxf(top, x[i]);
-      wide = fmaxf(wide, fmaxf(v_step[i][0], v_step[i][1]));
+      wide = fmaxf(wide, fmaxf(kv4_step(vs[i][0]), kv4_step(vs[i][1])));
     }
     if (__any(top > m_run + LAG || wide > cap)) {
 #pragma unroll
@@ -394,7 +417,6 @@ __global__ __launch_bounds__(NTHREADS, 3) void attn_decode4_kernel(
     const float m_use = m_run == -INFINITY ? 0.0f : m_run;
     Frag4 pf[2][2];                        // [32 keys][group]
     {
-      uint32_t w[GQA][2];
       float ps[GQA][2];
 #pragma unroll
       for (int i = 0; i < GQA; ++i) {
@@ -402,9 +424,8 @@ __global__ __launch_bounds__(NTHREADS, 3) void attn_decode4_kernel(
         l_run += p;
 #pragma unroll
         for (int g = 0; g < 2; ++g) {
-          ps[i][g] = p * (v_step[i][g] * to_cap);
-          low_run[g] = __builtin_fmaf(p, v_low[i][g], low_run[g]);
-          if constexpr (GQA < 8) w[i][g] = pack_f16(ps[i][g], ps[i][g]);
+          ps[i][g] = p * (kv4_step(vs[i][g]) * to_cap);
+          low_run[g] = __builtin_fmaf(p, kv4_least(vs[i][g]), low_run[g]);
         }
       }
 #pragma unroll
@@ -412,36 +433,50 @@ __global__ __launch_bounds__(NTHREADS, 3) void attn_decode4_kernel(
 #pragma unroll
         for (int g = 0; g < 2; ++g) {
           uint32_t v;
-          if constexpr (GQA == 8) v = pack_f16(ps[2 * tt][g], ps[2 * tt + 1][g]);
-          else if constexpr (GQA == 4) v = w[tt][g];
-          else if constexpr (GQA == 2) v = set >> 2 == tt >> 1 ? w[tt & 1][g] : 0u;
-          else v = set >> 2 == tt ? w[0][g] : 0u;
+          if constexpr (GQA == 8) {
+            v = pack_f16(ps[2 * tt][g], ps[2 * tt + 1][g]);
+          } else {
+            const float one = ps[GQA == 4 ? tt : GQA == 2 ? tt & 1 : 0][g];
+            v = pack_f16(one, one);
+            if constexpr (GQA == 2) v = set >> 2 == tt >> 1 ? v : 0u;
+            if constexpr (GQA == 1) v = set >> 2 == tt ? v : 0u;
+          }
 #pragma unroll
           for (int e = 0; e < 2; ++e) pf[tt >> 1][g].u[(tt & 1) * 2 + e] = v & keep[e];
         }
     }
-    // ---- P V: 32 keys at a time, a nibble a column tile -----------------------------------------
+    // ---- P V: 32 keys at a time, a nibble a column tile, those of a word's lower half first -------
+    if (more) asm volatile("s_waitcnt vmcnt(%0)" ::"i"(4 + SCALE_LOADS) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
-      Frag4 f[8];
+      uint32_t vraw[2][4];                 // word col of key 4 r + grp
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const uint32_t a = vraw[2 * s + (e >> 1)][(e & 1) * 2], c = vraw[2 * s + (e >> 1)][(e & 1) * 2 + 1];
-        const uint32_t lo = __builtin_amdgcn_perm(c, a, 0x05040100), hi = __builtin_amdgcn_perm(c, a, 0x07060302);
-        const uint32_t lo8 = lo >> 8, hi8 = hi >> 8;
-        f[0].u[e] = lo & 0x000f000fu;
-        f[1].u[e] = lo & 0x00f000f0u;
-        f[2].u[e] = lo8 & 0x000f000fu;
-        f[3].u[e] = lo8 & 0x00f000f0u;
-        f[4].u[e] = hi & 0x000f000fu;
-        f[5].u[e] = hi & 0x00f000f0u;
-        f[6].u[e] = hi8 & 0x000f000fu;
-        f[7].u[e] = hi8 & 0x00f000f0u;
+      for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          vraw[tt][r] = *(lds_v1)(uintptr_t)((v_get ^ (r << 4)) + ((2 * s + tt) * 16 + 4 * r) * KV4_BYTES);
+#pragma unroll
+      for (int up = 0; up < 2; ++up) {
+        __builtin_amdgcn_sched_barrier(0);
+        Frag4 f[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t a = vraw[e >> 1][(e & 1) * 2], c = vraw[e >> 1][(e & 1) * 2 + 1];
+          const uint32_t w = __builtin_amdgcn_perm(c, a, up ? 0x07060302 : 0x05040100), w8 = w >> 8;
+          f[0].u[e] = w & 0x000f000fu;
+          f[1].u[e] = w & 0x00f000f0u;
+          f[2].u[e] = w8 & 0x000f000fu;
+          f[3].u[e] = w8 & 0x00f000f0u;
+        }
+#pragma unroll
+        for (int p = 0; p < 4; ++p)
+          o[up * 4 + p] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f[p].m, pf[s][p >> 1].m, o[up * 4 + p], 0, 0, 0);
       }
-#pragma unroll
-      for (int p = 0; p < 8; ++p) o[p] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f[p].m, pf[s][(p & 3) >> 1].m, o[p], 0, 0, 0);
     }
-    if (more) load_v(base, row);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    if (more) load_rows(v_cache, lds0 + V_AT, base, row);
+    __builtin_amdgcn_sched_barrier(0);
   }
 
   // ---- this wave's sums, then the sets' and the waves' ------------------------------------------
@@ -458,7 +493,7 @@ __global__ __launch_bounds__(NTHREADS, 3) void attn_decode4_kernel(
     f32x4 v;
 #pragma unroll
     for (int r = 0; r < 4; ++r) v[r] = __builtin_fmaf(o[p][r], p & 1 ? back * 0.0625f : back, low_run[g]);
-    *reinterpret_cast<f32x4*>(&o_lds[wave][col][32 * (p & 3) + 16 * (p >> 2) + 4 * grp]) = v;
+    *reinterpret_cast<f32x4*>(&o_lds[wave][col * PART_STRIDE + 32 * (p & 3) + 16 * (p >> 2) + 4 * grp]) = v;
   }
   if (lane < 16) {
     m_lds[wave][lane] = m_run;
@@ -481,7 +516,7 @@ __global__ __launch_bounds__(NTHREADS, 3) void attn_decode4_kernel(
       for (int j = 0; j < SETS; ++j) {
         l += l_lds[w][h + GQA * j] * e;
 #pragma unroll
-        for (int r = 0; r < VEC; ++r) acc[r] += o_lds[w][h + GQA * j][d + r] * e;
+        for (int r = 0; r < VEC; ++r) acc[r] += o_lds[w][(h + GQA * j) * PART_STRIDE + d + r] * e;
       }
     }
     if (Z == 1) {
