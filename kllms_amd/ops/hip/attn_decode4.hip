@@ -45,6 +45,10 @@ typedef float f32x2 __attribute__((ext_vector_type(2)));
 #define FAR 16             // loads and stores past the L2, from and to other XCDs' workgroups
 #define LAG 8.0f           // how far a score may pass the running max, in powers of two
 #define ROOM 128.0f        // 2^15 / 2^LAG
+// Bytes of a layer's keys and values from which on they are loaded with the streaming hint (nt), where no neighbour shares the
+// prompt. us without and with: 16 streams of 6144, 32 / 8 heads 31.9, 27.7; one of 131072, 64 / 8 heads 46.2, 44.7
+#define ONCE (16 << 20)
+#define ROW_BYTES 144      // of a key and its value
 #define LOG2E 1.44269504088896340736f
 
 union Frag4 {
@@ -57,27 +61,89 @@ __device__ __forceinline__ uint32_t pack_f16(float a, float b) {
   return __builtin_bit_cast(uint32_t, __builtin_convertvector(x, f16x2_cvt));
 }
 
-// How many workgroups share a context: one for every ``per`` rounds of four tiles, ``most`` at most, and of those as many as
-// are all equally long.
-struct Decode4Shares {
-  int per, most;
+// Who works on what: a kv head's ``slots`` workgroups are dealt out, a context having one for every so many of its tiles, so that
+// contexts of different lengths keep the chip equally busy. Of the three numbers of tiles that come of all slots, of half a slot less for
+// each row and of one less, the least that keeps to the slots; the third one always does. Every wave counts for itself, by
+// register moves, up to four rows a lane; more rows than that have one workgroup each. (With the same number for all contexts, and idle
+// workgroups between those at work, compute units had one to three of them: 16 streams of 4500 to 7777 32.9 us, of 6144 28.0.)
+#define DEAL_ROWS 256
+struct Deal {
+  int row, length, share, shares, start;   // workgroups of the row, from slot ``start`` on; row -1: nobody's slot
 };
-__host__ __device__ __forceinline__ int shares4_of(int tiles, const Decode4Shares& s) {
-  const int rounds = (tiles + 3) / 4;
-  int z = (rounds + s.per - 1) / s.per;
-  z = z < s.most ? z : s.most;
-  if (z <= 1) return 1;
-  const int each = (rounds + z - 1) / z;
-  return (rounds + each - 1) / each;
+__device__ __forceinline__ int tiles_of(int length) { return (int)(((int64_t)length + TKEYS - 1) / TKEYS); }
+// any number does, as long as all agree: the tiles go round
+__device__ __forceinline__ int shares_of(int tiles, float inverse) { return max((int)ceilf(tiles * inverse - 1e-3f), 1); }
+template <int CTRL, int ROWS = 0xf>
+__device__ __forceinline__ int lane_moved(int x) { return __builtin_amdgcn_update_dpp(0, x, CTRL, ROWS, 0xf, false); }
+__device__ __forceinline__ int scan(int x) {             // of this lane's and those before it
+  x += lane_moved<0x111>(x);               // row_shr 1
+  x += lane_moved<0x112>(x);               // 2
+  x += lane_moved<0x114>(x);               // 4
+  x += lane_moved<0x118>(x);               // 8
+  x += lane_moved<0x142, 0xa>(x);          // row_bcast 15
+  x += lane_moved<0x143, 0xc>(x);          // row_bcast 31
+  return x;
+}
+__device__ __forceinline__ int last_lane(int x) { return __builtin_amdgcn_readlane(x, 63); }
+// BY_ROW: of row ``at``; else of slot ``at``. EACH: rows of a lane
+template <bool BY_ROW, int EACH>
+__device__ __forceinline__ Deal deal_rows(const int* __restrict__ lengths, int B, int64_t limit, int slots, int at) {
+  const int lane = threadIdx.x & 63;
+  int length[EACH], z[EACH], n = 0;
+#pragma unroll
+  for (int e = 0; e < EACH; ++e) {
+    const int row = lane * EACH + e;
+    length[e] = row < B ? (int)min((int64_t)max(lengths[row], 0), limit) : 0;
+    n += tiles_of(length[e]);
+  }
+  // not more workgroups than there are four tiles for
+  const float all = (float)max(last_lane(scan(n)), 1);
+  auto inverse = [&](float of) { return fminf(__builtin_amdgcn_rcpf(all) * of, 0.25f); };
+  const float per0 = inverse(slots), per1 = inverse(slots - 0.5f * B);
+  n = 0;                                   // slots by the first and by the second, 16 bits each
+#pragma unroll
+  for (int e = 0; e < EACH; ++e)
+    if (lane * EACH + e < B)
+      n += shares_of(tiles_of(length[e]), per0) + (shares_of(tiles_of(length[e]), per1) << 16);      // both below slots + B
+  n = last_lane(scan(n));
+  const float per = (n & 0xffff) <= slots ? per0 : n >> 16 <= slots ? per1 : inverse(slots - B);
+  n = 0;
+#pragma unroll
+  for (int e = 0; e < EACH; ++e) {
+    z[e] = lane * EACH + e < B ? shares_of(tiles_of(length[e]), per) : 0;
+    n += z[e];
+  }
+  const int until = scan(n);               // slots of this lane's rows end here
+  const int who = BY_ROW ? at / EACH : __popcll(__ballot(until <= at));
+  Deal d = {-1, 0, 0, 1, 0};
+  if (who >= 64) return d;
+  int from = __builtin_amdgcn_readlane(until, who) - __builtin_amdgcn_readlane(n, who);
+#pragma unroll
+  for (int e = 0; e < EACH; ++e) {
+    const int m = __builtin_amdgcn_readlane(z[e], who), l = __builtin_amdgcn_readlane(length[e], who);
+    if (BY_ROW ? who * EACH + e == at : at >= from && at < from + m) d = Deal{who * EACH + e, l, at - from, m, from};
+    from += m;
+  }
+  return d;
+}
+template <bool BY_ROW>
+__device__ __forceinline__ Deal deal(const int* __restrict__ lengths, int B, int64_t limit, int slots, int at) {
+  if (slots <= B) return Deal{at, (int)min((int64_t)max(lengths[at], 0), limit), 0, 1, at};
+  if (B == 1) {
+    const int length = (int)min((int64_t)max(lengths[0], 0), limit), n = min(shares_of(tiles_of(length), 0.25f), slots);
+    return Deal{BY_ROW || at < n ? 0 : -1, length, at, n, 0};
+  }
+  return B <= 64 ? deal_rows<BY_ROW, 1>(lengths, B, limit, slots, at) : deal_rows<BY_ROW, DEAL_ROWS / 64>(lengths, B, limit, slots, at);
 }
 
-// The partials [Z, GQA, PART_STRIDE] of a (stream, kv head), in their order, to its rows of the result, by all threads
+// The partials [GQA, PART_STRIDE] of Z workgroups, ``apart`` floats from each other, in their order, to rows of the result,
+// by all threads
 template <int GQA>
-__device__ __forceinline__ void merge4(bf16_t* __restrict__ out, const float* all, int Z, float (&sums)[NTHREADS][4],
+__device__ __forceinline__ void merge4(bf16_t* __restrict__ out, const float* all, int Z, int apart, float (&sums)[NTHREADS][4],
                                        float (&ml)[NTHREADS][2]) {
-  constexpr int SETS = NTHREADS / (32 * GQA), DEEP = 8;
+  constexpr int SETS = NTHREADS / (32 * GQA), DEEP = 16;
   const int tid = threadIdx.x, h = (tid >> 5) % GQA, d = (tid & 31) * 4, set = tid / (32 * GQA);
-  const auto far = __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(all), 0, Z * GQA * PART_STRIDE * 4, 0x00020000);
+  const auto far = __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(all), 0, ((Z - 1) * apart + GQA * PART_STRIDE) * 4, 0x00020000);
   float M = -INFINITY, sum = 0.0f;
   f32x4 acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 1
@@ -86,7 +152,7 @@ __device__ __forceinline__ void merge4(bf16_t* __restrict__ out, const float* al
     f32x2 of[DEEP];
 #pragma unroll
     for (int e = 0; e < DEEP; ++e) {       // behind the last one zeros
-      const int at = ((z0 + e * SETS) * GQA + h) * PART_STRIDE * 4;
+      const int at = ((z0 + e * SETS) * apart + h * PART_STRIDE) * 4;
       of[e] = __builtin_bit_cast(f32x2, __builtin_amdgcn_raw_buffer_load_b64(far, at + 512, 0, FAR));
       part[e] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(far, at + d * 4, 0, FAR));
     }
@@ -136,13 +202,13 @@ __device__ __forceinline__ void merge4(bf16_t* __restrict__ out, const float* al
 // WHOLE: blocks of a multiple of 16 keys
 template <int GQA, bool WHOLE>
 __global__ __launch_bounds__(NTHREADS, GQA == 8 || !WHOLE ? 3 : 4) void attn_decode4_kernel(
-    float* __restrict__ partials,          // [B, KVH, Z, GQA, PART_STRIDE]
+    float* __restrict__ partials,          // [slots, KVH, GQA, PART_STRIDE]
     bf16_t* __restrict__ out,              // written where one workgroup has the context, or by the last one with ``arrived``
     const bf16_t* __restrict__ q,          // [B, H, 128], row stride q_stride
     const uint32_t* __restrict__ k_cache, const uint32_t* __restrict__ v_cache,    // [NB, KVH, BS, 16] words
     const uint32_t* __restrict__ k_scale, const uint32_t* __restrict__ v_scale,    // [NB, KVH, BS, 2] words (step, least)
     const int* __restrict__ block_tables, const int* __restrict__ context_lens, int* __restrict__ arrived, int apart,
-    float scale, int block_size, uint32_t block_inverse, int max_blocks, int64_t q_stride, Decode4Shares shares) {
+    float scale, int block_size, uint32_t block_inverse, int max_blocks, int64_t q_stride, int B, int slots) {
   constexpr int SETS = 16 / GQA;
   constexpr int STRIP = 2 * TKEYS * KV4_BYTES + 2 * TKEYS * 8;
   static_assert(STRIP >= 16 * PART_STRIDE * 4);
@@ -150,11 +216,12 @@ __global__ __launch_bounds__(NTHREADS, GQA == 8 || !WHOLE ? 3 : 4) void attn_dec
   float (&o_lds)[4][STRIP / 4] = reinterpret_cast<float(&)[4][STRIP / 4]>(strips);      // at the end: a wave's sums, [16][PART_STRIDE]
   __shared__ float m_lds[4][16], l_lds[4][16];
   __shared__ int last_lds;
-  const int g_kv = blockIdx.x, num_kv_heads = gridDim.x, b = blockIdx.y, z = blockIdx.z;
-  const int L = (int)min((int64_t)context_lens[b], (int64_t)max_blocks * block_size);
-  const int tiles = (max(L, 0) + TKEYS - 1) / TKEYS;
-  const int Z = shares4_of(tiles, shares);
-  if (z >= Z) return;
+  const int g_kv = blockIdx.x, num_kv_heads = gridDim.x;
+  const Deal mine = deal<false>(context_lens, B, (int64_t)max_blocks * block_size, slots, blockIdx.y);
+  const int b = __builtin_amdgcn_readfirstlane(mine.row), z = __builtin_amdgcn_readfirstlane(mine.share);
+  const int Z = __builtin_amdgcn_readfirstlane(mine.shares), L = __builtin_amdgcn_readfirstlane(mine.length);
+  if (b < 0) return;
+  const int tiles = tiles_of(L);
   const int tid = threadIdx.x, lane = tid & 63, col = lane & 15, grp = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int head = col % GQA, set = col / GQA;
@@ -213,6 +280,9 @@ __global__ __launch_bounds__(NTHREADS, GQA == 8 || !WHOLE ? 3 : 4) void attn_dec
   const uint32_t keep[2] = {r_mine < 2 ? half : 0u, r_mine < 2 ? 0u : half};
 
   const int* bt = block_tables + (int64_t)b * max_blocks;
+  // the neighbours' first blocks are this context's: so are more, and lie in the L2
+  const bool once = (int64_t)L * B * num_kv_heads * ROW_BYTES >= ONCE &&
+                    !((b > 0 && bt[-max_blocks] == bt[0]) || (b + 1 < B && bt[max_blocks] == bt[0]));
   auto block_of = [&](int key) {           // key / block_size by its reciprocal, which is off by one at most
     const int n = (int)__umulhi((uint32_t)key, block_inverse), rest = key - n * block_size;
     return n - (rest < 0) + (rest >= block_size);
@@ -236,10 +306,14 @@ __global__ __launch_bounds__(NTHREADS, GQA == 8 || !WHOLE ? 3 : 4) void attn_dec
   auto put = [&](const char* rows, uint32_t lane_off, uint32_t at) {
     const uint64_t r = (uint64_t)rows;
     const u32x2 from = {(uint32_t)__builtin_amdgcn_readfirstlane((int)r), (uint32_t)__builtin_amdgcn_readfirstlane((int)(r >> 32))};
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(lane_off), "s"(from), "s"(at) : "memory");
+    if (once)
+      asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1 nt" ::"v"(lane_off), "s"(from), "s"(at) : "memory");
+    else
+      asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(lane_off), "s"(from), "s"(at) : "memory");
   };
   auto put_at = [&](const char* from, uint32_t at) {
-    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(from), "s"(at) : "memory");
+    if (once) asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off nt" ::"v"(from), "s"(at) : "memory");
+    else asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(from), "s"(at) : "memory");
   };
   auto put_word = [&](const uint32_t* from, uint32_t at) {
     asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(from), "s"(at) : "memory");
@@ -500,7 +574,7 @@ __global__ __launch_bounds__(NTHREADS, GQA == 8 || !WHOLE ? 3 : 4) void attn_dec
     l_lds[wave][lane] = l_run;
   }
   __syncthreads();
-  float* const part = partials + (((int64_t)b * num_kv_heads + g_kv) * gridDim.z + z) * (GQA * PART_STRIDE);
+  float* const part = partials + ((int64_t)blockIdx.y * num_kv_heads + g_kv) * (GQA * PART_STRIDE);
   bf16_t* const to = out + ((int64_t)b * num_kv_heads + g_kv) * GQA * 128;
   constexpr int VEC = GQA > 2 ? GQA / 2 : 1;
   if (tid * VEC < GQA * 128) {
@@ -540,70 +614,69 @@ __global__ __launch_bounds__(NTHREADS, GQA == 8 || !WHOLE ? 3 : 4) void attn_dec
   }
   __syncthreads();
   if (!last_lds) return;
-  merge4<GQA>(to, part - (int64_t)z * (GQA * PART_STRIDE), Z, reinterpret_cast<float(&)[NTHREADS][4]>(o_lds[0]),
+  merge4<GQA>(to, part - (int64_t)z * num_kv_heads * (GQA * PART_STRIDE), Z, num_kv_heads * (GQA * PART_STRIDE), reinterpret_cast<float(&)[NTHREADS][4]>(o_lds[0]),
               reinterpret_cast<float(&)[NTHREADS][2]>(o_lds[1]));
 }
 
-// the same for callers without counters
-template <int GQA>
+// the same in a launch of its own, a workgroup for each head
 __global__ __launch_bounds__(NTHREADS) void attn_decode4_merge_kernel(bf16_t* __restrict__ out, const float* __restrict__ partials,
-                                                                     const int* __restrict__ context_lens, int grid_z, int64_t most,
-                                                                     Decode4Shares shares) {
+                                                                     const int* __restrict__ context_lens, int64_t limit, int B,
+                                                                     int slots) {
   __shared__ float sums[NTHREADS][4], ml[NTHREADS][2];
-  const int g_kv = blockIdx.x, num_kv_heads = gridDim.x, b = blockIdx.y;
-  const int L = (int)min((int64_t)context_lens[b], most);
-  const int Z = shares4_of((max(L, 0) + TKEYS - 1) / TKEYS, shares);
-  if (Z == 1) return;
-  const int64_t pair = (int64_t)b * num_kv_heads + g_kv;
-  merge4<GQA>(out + pair * GQA * 128, partials + pair * grid_z * (GQA * PART_STRIDE), Z, sums, ml);
+  const int h = blockIdx.x, num_q_heads = gridDim.x, b = blockIdx.y;
+  const Deal mine = deal<true>(context_lens, B, limit, slots, b);
+  const int Z = __builtin_amdgcn_readfirstlane(mine.shares);
+  if (Z == 1) return;                      // its one workgroup has written the result
+  merge4<1>(out + ((int64_t)b * num_q_heads + h) * 128,
+            partials + ((int64_t)__builtin_amdgcn_readfirstlane(mine.start) * num_q_heads + h) * PART_STRIDE, Z, num_q_heads * PART_STRIDE,
+            sums, ml);
 }
 
 // rows of a launch: they lie on the grid's y, which ends at 65535
 #define MAX_ROWS 65535
 
-static Decode4Shares attn_decode4_shares(int B, int num_kv_heads) {
-  const int64_t pairs = (int64_t)B * num_kv_heads;
-  Decode4Shares s;
-  s.per = 1;
-  s.most = (int)std::max<int64_t>(1, std::min<int64_t>(768 / pairs, 128));
-  return s;
+// Workgroups of a kv head: two for each compute unit, a workgroup's beginning and end being 5 us of its own; of more rows than
+// units one for each, and some for contexts that are much longer than the others. us in all of 256, 512, 768 and 1024 workgroups: 16
+// streams of 6144, 32 / 8 heads 27.1, 25.6, 27.8, 27.7; one of 131072, 64 / 8 heads 40.9, 33.9, 38.9, 38.1; 40 of 1500 (320 pairs) 18.5 with
+// a workgroup each, 22.2 with two. max_ctx: positions of the table
+static int attn_decode4_slots(int B, int num_kv_heads, int64_t max_ctx) {
+  const int slots = std::max(1, 512 / num_kv_heads);
+  // contexts of a few rounds at most are as they are where they fill the chip
+  if (B > DEAL_ROWS || max_ctx <= 4 * TKEYS || (2 * B > slots && max_ctx <= 16 * TKEYS)) return B;
+  if (B == 1) return (int)std::min<int64_t>(slots, (max_ctx + 4 * TKEYS - 1) / (4 * TKEYS));
+  return 2 * B <= slots ? slots : B + std::max(1, 256 / num_kv_heads);
 }
 
-// workgroups per context of a launch; max_ctx: positions of the table
-extern "C" int attn_decode4_splits(int B, int num_kv_heads, int max_ctx) {
-  const int tiles = (int)(((int64_t)max_ctx + TKEYS - 1) / TKEYS), rounds = (tiles + 3) / 4;
-  const Decode4Shares s = attn_decode4_shares(B < MAX_ROWS ? B : MAX_ROWS, num_kv_heads);
-  return std::max(1, std::min(rounds, s.most));
+// floats of a launch's partials: 0 where every row has one workgroup
+extern "C" int64_t attn_decode4_room(int B, int num_kv_heads, int gqa, int64_t max_ctx) {
+  const int slots = attn_decode4_slots(B, num_kv_heads, max_ctx);
+  return slots > B ? (int64_t)slots * num_kv_heads * gqa * PART_STRIDE : 0;
 }
-
-// floats of a launch's partials for each (row, kv head, workgroup, head of it)
-extern "C" int attn_decode4_part() { return PART_STRIDE; }
 
 extern "C" void launch_attn_decode4(bf16_t* out, float* partials, int* arrived, int apart, const bf16_t* q, const void* k_cache,
                                     const void* v_cache, const void* k_scale, const void* v_scale, const int* block_tables,
                                     const int* context_lens, float scale, int num_q_heads, int num_kv_heads, int block_size,
-                                    int max_blocks, int max_ctx, int64_t q_stride, int B, hipStream_t stream) {
-  const int gqa = num_q_heads / num_kv_heads, splits = attn_decode4_splits(B, num_kv_heads, max_ctx);
-  const Decode4Shares sh = attn_decode4_shares(B < MAX_ROWS ? B : MAX_ROWS, num_kv_heads);
+                                    int max_blocks, int64_t q_stride, int B, hipStream_t stream) {
+  const int gqa = num_q_heads / num_kv_heads;
+  const int64_t limit = (int64_t)max_blocks * block_size;
+  const int slots = attn_decode4_slots(B, num_kv_heads, limit);
+  // merged by the last workgroup, unless its work alone is more than a launch: heads times shares of a context
+  if ((int64_t)(slots / B) * gqa > 192) arrived = nullptr;
   const uint32_t inverse = block_size > 1 ? (uint32_t)(((1ull << 32) + block_size - 1) / block_size) : ~0u;
   for (int b0 = 0; b0 < B; b0 += MAX_ROWS) {
     const int rows = B - b0 < MAX_ROWS ? B - b0 : MAX_ROWS;
-    const dim3 grid(num_kv_heads, rows, splits);
+    const dim3 grid(num_kv_heads, std::max(rows, slots));
     bf16_t* o = out + (int64_t)b0 * num_q_heads * 128;
     const bf16_t* q0 = q + (int64_t)b0 * q_stride;
     const int* bt = block_tables + (int64_t)b0 * max_blocks;
-    int* a0 = arrived ? arrived + (int64_t)b0 * num_kv_heads * apart : nullptr;
 #define LAUNCH(G, W)                                                                                                    \
   hipLaunchKernelGGL((attn_decode4_kernel<G, W>), grid, dim3(NTHREADS), 0, stream, partials, o, q0, (const uint32_t*)k_cache, \
-                     (const uint32_t*)v_cache, (const uint32_t*)k_scale, (const uint32_t*)v_scale, bt, context_lens + b0, a0,  \
-                     apart, scale, block_size, inverse, max_blocks, q_stride, sh)
+                     (const uint32_t*)v_cache, (const uint32_t*)k_scale, (const uint32_t*)v_scale, bt, context_lens + b0, arrived,  \
+                     apart, scale, block_size, inverse, max_blocks, q_stride, rows, slots)
 #define DISPATCH(G)                                                                                                       \
   do {                                                                                                                    \
     if (block_size % 16 == 0) LAUNCH(G, true);                                                                            \
     else LAUNCH(G, false);                                                                                                \
-    if (splits > 1 && !arrived)                                                                                           \
-      hipLaunchKernelGGL(attn_decode4_merge_kernel<G>, dim3(num_kv_heads, rows), dim3(NTHREADS), 0, stream, o, partials,  \
-                         context_lens + b0, splits, (int64_t)max_blocks * block_size, sh);                                \
   } while (0)
     switch (gqa) {
       case 1: DISPATCH(1); break;
@@ -613,5 +686,8 @@ extern "C" void launch_attn_decode4(bf16_t* out, float* partials, int* arrived, 
     }
 #undef DISPATCH
 #undef LAUNCH
+    if (slots > B && !arrived)
+      hipLaunchKernelGGL(attn_decode4_merge_kernel, dim3(num_q_heads, rows), dim3(NTHREADS), 0, stream, o, partials, context_lens + b0, limit,
+                         rows, slots);
   }
 }

@@ -148,10 +148,9 @@ std::tuple<torch::Tensor, torch::Tensor> load_kv4(torch::Tensor k_cache, torch::
   return {k, v};
 }
 
-extern "C" int attn_decode4_splits(int B, int num_kv_heads, int max_ctx);
-extern "C" int attn_decode4_part();
+extern "C" int64_t attn_decode4_room(int B, int num_kv_heads, int gqa, int64_t max_ctx);
 extern "C" void launch_attn_decode4(bf16_t*, float*, int*, int, const bf16_t*, const void*, const void*, const void*, const void*,
-                                    const int*, const int*, float, int, int, int, int, int, int64_t, int, hipStream_t);
+                                    const int*, const int*, float, int, int, int, int, int64_t, int, hipStream_t);
 
 // Rows of tables int32 [B, MAXB] and lengths int32 [B] beside q [B, H, 128]
 static void check_contexts(const torch::Tensor& q, const torch::Tensor& tables, const torch::Tensor& lens, const char* who) {
@@ -180,20 +179,17 @@ torch::Tensor attn_decode4(torch::Tensor q, torch::Tensor k_cache, torch::Tensor
   if (B == 0) return out;
   if (max_blocks == 0 || k_cache.numel() == 0) return out.zero_();     // every context is empty
   if (!rows_aligned(q)) q = q.clone(at::MemoryFormat::Contiguous);
-  const int longest = (int)std::min<int64_t>(max_blocks * BS, INT32_MAX);
-  const int splits = attn_decode4_splits((int)B, (int)KVH, longest);
   int apart = 1;
   if (arrived) {
     TORCH_CHECK(arrived->is_contiguous() && arrived->scalar_type() == at::kInt && arrived->numel() >= B * KVH &&
                     arrived->device() == q.device(), "arrived: an int32 zero for each row and kv head");
     apart = (int)std::min<int64_t>(arrived->numel() / (B * KVH), 32);
   }
-  auto partials = torch::empty({splits > 1 ? std::min<int64_t>(B, 65535) * KVH * splits * gqa * attn_decode4_part() : 0},
-                               q.options().dtype(torch::kFloat));
+  auto partials = torch::empty({attn_decode4_room((int)B, (int)KVH, (int)gqa, max_blocks * BS)}, q.options().dtype(torch::kFloat));
   launch_attn_decode4(bf(out), partials.data_ptr<float>(), arrived ? arrived->data_ptr<int>() : nullptr, apart, cbf(q),
                       k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), block_tables.data_ptr<int>(),
-                      context_lens.data_ptr<int>(), (float)scale, (int)H, (int)KVH, (int)BS, (int)max_blocks, longest, q.stride(0),
-                      (int)B, cur_stream());
+                      context_lens.data_ptr<int>(), (float)scale, (int)H, (int)KVH, (int)BS, (int)max_blocks, q.stride(0), (int)B,
+                      cur_stream());
   return out;
 }
 
@@ -964,7 +960,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("attn_decode4", &attn_decode4, py::arg("q"), py::arg("k_cache"), py::arg("v_cache"), py::arg("block_tables"),
         py::arg("context_lens"), py::arg("scale"), py::arg("k_scale"), py::arg("v_scale"), py::arg("arrived") = py::none(),
         py::arg("into") = py::none());
-  m.def("attn_decode4_splits", &attn_decode4_splits);
   // workgroups of a context at most, by rows, kv heads, heads of each, positions of the table, fp8, block-local, counters
   m.def("attn_decode_splits", &attn_decode_splits);
   m.def("attn_decode_paged", &attn_decode_paged, py::arg("out"), py::arg("q"), py::arg("k_cache"),

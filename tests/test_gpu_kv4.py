@@ -128,22 +128,23 @@ def case(ctx, gqa, KVH, BS, seed=0, width=None, shared=0, spread=0.0, behind=Tru
     return rows(B, KVH * gqa, D, seed=seed + 99), kc, vc, ks, vs, tables, torch.tensor(ctx, dtype=torch.int32)
 
 
-def check(out, q, kc, vc, ks, vs, tables, n, scale):
+def check(outs, q, kc, vc, ks, vs, tables, n, scale):
     want, off = attention64(q, kc, vc, ks, vs, tables, n, scale)
-    far = (out.double().cpu() - want).abs()
-    assert bool((far <= off).all()), f"{float((far / off).max())} of what is allowed, at {torch.nonzero(far > off)[:3].tolist()}"
+    for out in outs:
+        far = (out.double().cpu() - want).abs()
+        assert bool((far <= off).all()), f"{float((far / off).max())} of what is allowed, at {torch.nonzero(far > off)[:3].tolist()}"
 
 
 def both(q, kc, vc, ks, vs, tables, n, scale):
-    """The result, the same with counters and without."""
+    """The results without counters and with them, whose shares are added up in another order."""
     dev = [t.to(DEV) for t in (q, kc, vc, tables, n, ks, vs)]
     q, kc, vc, tables, n, ks, vs = dev
     out = ops.attn_decode_paged(q, kc, vc, tables, n, scale, ks, vs)
     arrived = torch.zeros(q.shape[0] * kc.shape[1] * ops.ATTN_COUNTER_GAP, dtype=torch.int32, device=DEV)
     joined = ops.attn_decode_paged(q, kc, vc, tables, n, scale, ks, vs, arrived)
-    assert torch.equal(joined.nan_to_num(7e37), out.nan_to_num(7e37))
+    assert torch.equal(ops.attn_decode_paged(q, kc, vc, tables, n, scale, ks, vs, arrived).nan_to_num(7e37), joined.nan_to_num(7e37))
     assert not bool(arrived.any())
-    return out
+    return out, joined
 
 
 @pytest.mark.parametrize("gqa,KVH,BS", [(1, 2, 16), (2, 1, 8), (4, 8, 16), (8, 2, 32), (4, 3, 5), (1, 1, 1), (2, 2, 48), (8, 1, 7)])
@@ -160,6 +161,14 @@ def test_decode(gqa, KVH, BS, ctx, width):
 @pytest.mark.parametrize("gqa,KVH,BS", [(4, 8, 16), (8, 1, 16), (1, 2, 6), (2, 1, 32)])
 def test_long_contexts_in_shares(gqa, KVH, BS):
     args = case([9000, 5], gqa, KVH, BS, seed=gqa)
+    check(both(*args, D ** -0.5), *args, D ** -0.5)
+
+
+@pytest.mark.parametrize("ctx", [[40000, 3, 0], [9000, 30000], [0, 20000], [17000] + [40] * 20, [100] * 70 + [9000], [300 + 7 * i for i in range(200)],
+                                 [5] * 300, [0, 0, 0, 700]])
+@pytest.mark.parametrize("KVH,BS", [(1, 16), (4, 6)])
+def test_one_context_much_longer_than_the_others(ctx, KVH, BS):
+    args = case(ctx, 4, KVH, BS, seed=len(ctx))
     check(both(*args, D ** -0.5), *args, D ** -0.5)
 
 
@@ -198,12 +207,12 @@ def test_a_row_that_is_no_number_is_its_groups_alone():
     q, kc, vc, ks, vs, tables, n = case([70, 200], 4, 2, 16, seed=12)
     blk, off = int(tables[1, 3]), 5
     vs[blk, 1, off, 1] = float("nan")                 # of kv head 1, values 64 to 127
-    out = both(q, kc, vc, ks, vs, tables, n, 0.1).cpu()
-    bad = torch.isnan(out)
-    assert bool(bad[1, 4:, 64:].all()) and int(bad.sum()) == 4 * 64
+    for out in both(q, kc, vc, ks, vs, tables, n, 0.1):
+        bad = torch.isnan(out)
+        assert bool(bad[1, 4:, 64:].all()) and int(bad.sum()) == 4 * 64
     ks[blk, 0, off, 0] = float("nan")                 # a key: all of its heads
-    out = both(q, kc, vc, ks, vs, tables, n, 0.1).cpu()
-    assert bool(torch.isnan(out[1, :4]).all()) and int(torch.isnan(out).sum()) == 4 * 64 + 4 * 128
+    for out in both(q, kc, vc, ks, vs, tables, n, 0.1):
+        assert bool(torch.isnan(out[1, :4]).all()) and int(torch.isnan(out).sum()) == 4 * 64 + 4 * 128
 
 
 def test_strided_queries_and_empty_calls():
@@ -226,7 +235,7 @@ def test_caches_of_more_than_2_gb():
     for t, small in zip(big, (kc, vc, ks, vs)):
         t[far[0]:] = small.to(DEV)
     moved = (tables.long() + far[0]).int()
-    want = both(q, kc, vc, ks, vs, tables, n, 0.1)
+    want = both(q, kc, vc, ks, vs, tables, n, 0.1)[0]
     out = ops.attn_decode_paged(q.to(DEV), big[0], big[1], moved.to(DEV), n.to(DEV), 0.1, big[2], big[3])
     assert torch.equal(out, want)
     slots = torch.tensor([NB * BS - 1, (NB - 5) * BS], device=DEV)
