@@ -252,27 +252,97 @@ def paged_prefill_plan(segs, device, rows: int = 256) -> tuple:
     return PagedGroups(upload(torch.tensor(groups, dtype=torch.int32).t().contiguous(), device), rows), short
 
 
+class Kv4Groups(NamedTuple):
+    """Groups of a segment's rows that attend over the 4-bit cache together: ``items`` int32 [n, 8] (first packed row and rows of
+    the segment, first row of the group, segment, first and last key, where its sums go, 0) and ``cuts`` [m, 4] (first packed
+    row, rows, first part, parts) of groups whose keys are cut into ``parts`` altogether."""
+    items: torch.Tensor
+    cuts: torch.Tensor
+    parts: int
+
+
+KV4_GROUP_ROWS = 8           # segments shorter than this attend row by row
+_KV4_UNITS = 256
+_KV4_ITEM = (8.0, 0.027)     # us of an item, and of each of its keys
+
+
+def _kv4_cuts(keys, kv_heads: int) -> int:
+    """How many keys an item of groups of so many keys each has at most: what makes the rounds of all compute units
+    shortest, sums' way through memory and the second launch included."""
+    total, longest = sum(keys), max(keys)
+
+    def cost(most):
+        items = kv_heads * sum(-(-k // most) for k in keys)
+        parts = items - kv_heads * sum(k <= most for k in keys)
+        at, key = _KV4_ITEM
+        return -(-items // _KV4_UNITS) * (at + min(most, longest) * key) + (5.0 + parts * 0.06 if parts else 0.0)
+
+    tries = {-(-longest // 128) * 128}
+    for waves in (1, 2, 3, 4, 6):
+        tries.add(max(256, -(-total * kv_heads // (_KV4_UNITS * waves * 128)) * 128))
+        tries.add(max(256, -(-total * kv_heads // ((_KV4_UNITS - min(255, kv_heads * len(keys) // 2)) * waves * 128)) * 128))
+    return min(sorted(tries, reverse=True), key=cost)
+
+
+def kv4_plan(segs, heads: int, kv_heads: int, device) -> tuple:
+    """paged_plan of the 4-bit cache."""
+    rows = 256 // (heads // kv_heads)
+    groups, short, row = [], [], 0
+    for i, (start, n) in enumerate(segs):
+        if n >= KV4_GROUP_ROWS:
+            groups.extend((row, n, r, i, start + min(n, r + rows)) for r in range(0, n, rows))
+        elif n and short and short[-1][0] + short[-1][1] == row:
+            short[-1] = (short[-1][0], short[-1][1] + n)
+        elif n:
+            short.append((row, n))
+        row += n
+    if not groups:
+        return None, short
+    most = _kv4_cuts([g[4] for g in groups], kv_heads)
+    items, cuts, parts = [], [], 0
+    for row, n, r, i, keys in groups:
+        pieces = -(-keys // most)
+        if pieces == 1:
+            items.append((row, n, r, i, 0, keys, -1, 0))
+            continue
+        each = -(-keys // (pieces * 128)) * 128
+        pieces = -(-keys // each)
+        cuts.append((row + r, min(n - r, rows), parts, pieces))
+        items.extend((row, n, r, i, e * each, min(keys, (e + 1) * each), parts + e, 0) for e in range(pieces))
+        parts += pieces
+    items.sort(key=lambda g: g[4] - g[5])                # longest first
+    flat = upload(torch.tensor([x for g in items for x in g] + [x for c in cuts for x in c], dtype=torch.int32), device)
+    return Kv4Groups(flat[:8 * len(items)].view(-1, 8), flat[8 * len(items):].view(-1, 4), parts), short
+
+
 def paged_plan(segs, heads: int, kv_heads: int, device, cache_dtype=torch.bfloat16) -> tuple:
     """What attn_segments_paged takes of segments [(start position, rows)]: (groups of rows that attend together, or None,
     [(first row, rows)] of those that attend row by row). Made once for all layers of a pass."""
-    rows = sum(n for _, n in segs)
+    if cache_dtype == torch.uint8 and heads // kv_heads in (1, 2, 4, 8) and heads % kv_heads == 0:
+        return kv4_plan(segs, heads, kv_heads, device)
     if cache_dtype == torch.bfloat16 and paged_prefill_pays(segs, kv_heads):
         return paged_prefill_plan(segs, device, 64 if paged_prefill_few(segs, heads) else 256)
+    rows = sum(n for _, n in segs)
     return None, [(0, rows)] if rows else []
 
 
 def attn_segments_paged(q, k_cache, v_cache, block_tables, context_lens, scale, plan, short, seg_tables, seg_start,
                         k_scale=None, v_scale=None):
     """Rows of long segments on the matrix cores against the paged bf16 or 4-bit cache, the others row by row (GPU only).
-    ``plan`` and ``short``: of paged_plan for this cache's type."""
+    ``plan`` and ``short``: of paged_plan for this cache's type. A 4-bit value row that is no number makes the rows that
+    attend together and see it none as a whole."""
     _check_kv4(k_cache, k_scale, v_scale)
     out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     if k_cache.dtype == torch.uint8:
+        if plan is not None:
+            _hip_or_raise().attn_prefill4(out, q, k_cache, v_cache, plan.items, plan.cuts, plan.parts, seg_tables, seg_start, scale,
+                                          k_scale, v_scale)
         for r, n in short:
             _hip_or_raise().attn_decode4(q[r:r + n], k_cache, v_cache, block_tables[r:r + n], context_lens[r:r + n], scale,
                                          k_scale, v_scale, None, out[r:r + n])
         return out
-    _hip_or_raise().attn_prefill_paged(out, q, k_cache, v_cache, plan.groups, seg_tables, seg_start, scale, plan.rows)
+    if plan is not None:
+        _hip_or_raise().attn_prefill_paged(out, q, k_cache, v_cache, plan.groups, seg_tables, seg_start, scale, plan.rows)
     f = _none(q, torch.float32)
     for r, n in short:
         _hip_or_raise().attn_decode_paged(out[r:r + n], q[r:r + n], k_cache, v_cache, block_tables[r:r + n],

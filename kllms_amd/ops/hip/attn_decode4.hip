@@ -17,8 +17,8 @@
 //   scores   S[key][column] (16x16x32), column n is head n % GQA in set n / GQA. All sets hold the same scores; set j
 //            works on GQA of a lane's 16 alone: no exponential is computed twice, a lane loads the scales of GQA keys
 //   P V      O^T = V^T P^T: P's columns have the keys of their set and zeros for the others, sets are added up at the end
-//   max      renewed only when a score passes it by more than 8 (in powers of two), which leaves p s below fp16's end
-//   steps    p s is scaled by the power of two above the largest step of V so far, renewed like the max
+//   max      renewed only when a score passes it by more than 8 (in powers of two)
+//   p s      is scaled to fp16's range by its own largest so far, of each head and group, renewed in the same way
 //
 // A wave's tile goes to a strip of LDS that is its own, straight from memory and as it lies there: nine loads of whole lines
 // for 64 keys, without registers in between or barriers; the next K is on its way as soon as this one's fragments are read, the next V
@@ -44,7 +44,8 @@ typedef float f32x2 __attribute__((ext_vector_type(2)));
 #define PART_STRIDE 132    // of a head's partial: 128 sums, max, sum of exponentials
 #define FAR 16             // loads and stores past the L2, from and to other XCDs' workgroups
 #define LAG 8.0f           // how far a score may pass the running max, in powers of two
-#define ROOM 128.0f        // 2^15 / 2^LAG
+#define ROOM 32768.0f      // largest p s in fp16
+#define SPARE 4            // powers of two that p s may grow by before it is scaled anew
 // Bytes of a layer's keys and values from which on they are loaded with the streaming hint (nt), where no neighbour shares the
 // prompt. us without and with: 16 streams of 6144, 32 / 8 heads 31.9, 27.7; one of 131072, 64 / 8 heads 46.2, 44.7
 #define ONCE (16 << 20)
@@ -372,7 +373,7 @@ __global__ __launch_bounds__(NTHREADS, GQA == 8 || !WHOLE ? 3 : 4) void attn_dec
 #pragma unroll
   for (int p = 0; p < 8; ++p) o[p] = f32x4{0.f, 0.f, 0.f, 0.f};
   float m_run = -INFINITY, l_run = 0.0f, low_run[2] = {0.0f, 0.0f};      // of this lane's head and keys
-  float cap = 0.0f, to_cap = 0.0f;         // power of two from V's largest step so far on; what p s is multiplied by
+  float cap[2] = {0.0f, 0.0f}, to_cap[2] = {0.0f, 0.0f};       // what p s of a group stays below, and what it is multiplied by
 
   const int step = Z * 4;
   int t = z * 4 + wave;
@@ -458,50 +459,63 @@ __global__ __launch_bounds__(NTHREADS, GQA == 8 || !WHOLE ? 3 : 4) void attn_dec
           vs[i] = u32x2{0u, 0u};
         }
     }
-    // ---- the max and the largest step, renewed when they have to be ---------------------------
-    float top = x[0], wide = 0.0f;
+    // ---- the max, renewed when it has to be ----------------------------------------------------
+    float top = x[0];
 #pragma unroll
-    for (int i = 0; i < GQA; ++i) {
-      top = fmaxf(top, x[i]);
-      wide = fmaxf(wide, fmaxf(kv4_step(vs[i][0]), kv4_step(vs[i][1])));
-    }
-    if (__any(top > m_run + LAG || wide > cap)) {
+    for (int i = 1; i < GQA; ++i) top = fmaxf(top, x[i]);
+    if (__any(top > m_run + LAG)) {
 #pragma unroll
       for (int off = GQA; off <= 32; off <<= 1) top = fmaxf(top, __shfl_xor(top, off));
-#pragma unroll
-      for (int off = 1; off <= 32; off <<= 1) wide = fmaxf(wide, __shfl_xor(wide, off));
       const float m_new = fmaxf(m_run, top);
       const float alpha = m_run == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m_run - m_new);
       m_run = m_new;
-      float shrink = 1.0f;
-      if (wide > cap) {                    // 2^(e + 1), within what its inverse times ROOM can be
-        const int e = min(max((int)(__float_as_uint(wide) >> 23) - 126, -110), 127);
-        const float cap_new = ldexpf(1.0f, e);
-        shrink = cap > 0.0f ? cap / cap_new : 0.0f;
-        cap = cap_new;
-        to_cap = ROOM / cap;
-      }
       l_run *= alpha;
-      low_run[0] *= alpha;
-      low_run[1] *= alpha;
 #pragma unroll
-      for (int p = 0; p < 8; ++p) o[p] *= alpha * shrink;
+      for (int g = 0; g < 2; ++g) {
+        low_run[g] *= alpha;
+        cap[g] *= alpha;                   // the sums stay as they are, in a smaller unit
+        cap[g] = cap[g] < 1e-30f ? 0.0f : cap[g];
+        to_cap[g] = cap[g] > 0.0f ? ROOM / cap[g] : 0.0f;
+      }
     }
     // ---- P, and P times V's steps to fragments ------------------------------------------------
     const float m_use = m_run == -INFINITY ? 0.0f : m_run;
     Frag4 pf[2][2];                        // [32 keys][group]
     {
-      float ps[GQA][2];
+      float ps[GQA][2], wide[2] = {0.0f, 0.0f};
 #pragma unroll
       for (int i = 0; i < GQA; ++i) {
         const float p = __builtin_amdgcn_exp2f(x[i] - m_use);
         l_run += p;
 #pragma unroll
         for (int g = 0; g < 2; ++g) {
-          ps[i][g] = p * (kv4_step(vs[i][g]) * to_cap);
+          ps[i][g] = p * kv4_step(vs[i][g]);
+          wide[g] = fmaxf(wide[g], ps[i][g]);
           low_run[g] = __builtin_fmaf(p, kv4_least(vs[i][g]), low_run[g]);
         }
       }
+      if (__any(wide[0] > cap[0] || wide[1] > cap[1])) {
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+#pragma unroll
+          for (int off = GQA; off <= 32; off <<= 1) wide[g] = fmaxf(wide[g], __shfl_xor(wide[g], off));
+          float shrink = 1.0f;
+          if (wide[g] > cap[g]) {
+            const int e = min(max((int)(__float_as_uint(wide[g]) >> 23) - 126 + SPARE, -100), 127);
+            const float cap_new = ldexpf(1.0f, e);
+            shrink = cap[g] / cap_new;
+            cap[g] = cap_new;
+            to_cap[g] = ROOM / cap_new;
+          }
+#pragma unroll
+          for (int p = 0; p < 8; ++p)
+            if ((p & 3) >> 1 == g) o[p] *= shrink;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < GQA; ++i)
+#pragma unroll
+        for (int g = 0; g < 2; ++g) ps[i][g] *= to_cap[g];
 #pragma unroll
       for (int tt = 0; tt < 4; ++tt)
 #pragma unroll
@@ -560,13 +574,13 @@ __global__ __launch_bounds__(NTHREADS, GQA == 8 || !WHOLE ? 3 : 4) void attn_dec
     low_run[0] += __shfl_xor(low_run[0], off);
     low_run[1] += __shfl_xor(low_run[1], off);
   }
-  const float back = cap * (16777216.0f / ROOM);       // 2^24: the nibbles'
+  const float back[2] = {cap[0] * (16777216.0f / ROOM), cap[1] * (16777216.0f / ROOM)};       // 2^24: the nibbles'
 #pragma unroll
   for (int p = 0; p < 8; ++p) {
     const int g = (p & 3) >> 1;
     f32x4 v;
 #pragma unroll
-    for (int r = 0; r < 4; ++r) v[r] = __builtin_fmaf(o[p][r], p & 1 ? back * 0.0625f : back, low_run[g]);
+    for (int r = 0; r < 4; ++r) v[r] = __builtin_fmaf(o[p][r], p & 1 ? back[g] * 0.0625f : back[g], low_run[g]);
     *reinterpret_cast<f32x4*>(&o_lds[wave][col * PART_STRIDE + 32 * (p & 3) + 16 * (p >> 2) + 4 * grp]) = v;
   }
   if (lane < 16) {

@@ -1,0 +1,472 @@
+// Attention of prompt portions (rows behind a cached prefix, causal among themselves) against a paged cache held in 4 bits
+// (kv4.h), for gfx950.
+//
+//   - an 8-wave workgroup serves 32-row tiles of all query heads of ONE kv head of a segment: 256 / GQA rows, a wave for
+//     each tile and head. So the keys are made once for all heads, and a short tail still has eight waves at work
+//   - 128 keys at a time: each thread has a quarter of a K row and of a V row on their way in registers, makes fp16 of them
+//     and puts them to LDS, double-buffered, while the stage before is multiplied
+//   - fp16 holds what the cache stands for to 2^-12 (with K in bf16 the result is three times further off than its own
+//     rounding makes it, behind 9000 keys). 16 keys that a wave makes have a power of 2^16 taken out, such that their largest is between
+//     2^-4 and 2^13: none, in a model, and then nothing is multiplied back. q's rows are scaled into fp16's range exactly
+//   - scores and softmax as in attn_prefill.hip: S = K Q^T, a lane has one row's scores, base-2 exponentials of one fma, the
+//     running max renewed when it grows by more than 8; P is fp16 in one part, 2^-12 of it, where bf16 would need two
+//   - few or long groups are cut along the keys (the plan says where); their sums meet in a second launch
+//
+// A nibble becomes fp16 in three half instructions of two each: masked into 1024 + n, less 1024, times step plus least
+// value, which is rounded once.
+//
+// What bounds it: the vector units, with the softmax's exponentials before all; making the keys is a sixth of their work.
+//
+// Fragment maps and ds_read_b64_tr_b16: attn_prefill.hip.
+
+#include <algorithm>
+#include <type_traits>
+
+#include "kv4.h"
+
+typedef _Float16 f16x8_mfma __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
+typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+
+#define QBLK 32
+#define STAGE 128                  // keys staged per barrier round
+#define NWAVES 8
+#define STAGE_BYTES (STAGE * 256)  // K or V of a stage
+#define CLASSES (2 * STAGE)        // bytes of a stage's: K's and V's of each key
+#define LDS_BYTES (4 * STAGE_BYTES + 2 * CLASSES + 2 * NWAVES)
+#define PART_STRIDE 132            // of a row and head's partial: 128 sums, max, sum of exponentials
+#define PART_ROWS (NWAVES * QBLK)  // rows and heads of an item and kv head
+
+__device__ __forceinline__ int acc_row(int r, int half) { return (r & 3) + 8 * (r >> 2) + 4 * half; }   // C/D row map
+// V's 32-byte slots of a row are XORed with this: the rows of a turned read, 4 by 2 slots, lie in all banks
+__device__ __forceinline__ int v_turn(int row) { return (row & 3) * 2 + (row >> 2 & 1); }
+__device__ __forceinline__ uint32_t pack_f16(float a, float b) {
+  const f32x2 x = {a, b};
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector(x, f16x2));
+}
+__device__ __forceinline__ f16x2 as_f16(uint32_t w) { return __builtin_bit_cast(f16x2, w); }
+
+// An item of the plan: rows r0.. of a segment (first packed row, rows, its number), keys from..to of it, where its sums go (-1:
+// nobody else has these rows)
+struct Item {
+  int row, len, r0, seg, from, to, part, unused;
+};
+
+// A row's class: the power of 2^16 that is taken out of it, after the largest exponent of a group's least value and step. A
+// group that is no number does not count.
+__device__ __forceinline__ int row_class(const u32x2& scales) {
+  int e = 0;
+#pragma unroll
+  for (int g = 0; g < 2; ++g) {
+    const int l = (int)(scales[g] >> 23 & 0xff), s = (int)(scales[g] >> 7 & 0xff);
+    e = max(e, l == 255 || s == 255 ? 0 : max(l, s ? s + 4 : 0));        // all values are below 2^(e - 127 + 2)
+  }
+  if (e == 0) return 0;
+  e -= 127;
+  return e > 12 ? (e - 13 >> 4) + 1 : e < -10 ? max(-(-11 - e >> 4) - 1, -7) : 0;
+}
+
+// Four words of a row (32 values) to fp16: put(p, two words) takes those of nibble p, four neighbouring values
+template <class P>
+__device__ __forceinline__ void kv4_to_f16(const u32x4& w, const u32x2& scales, float down, P put) {
+  f16x2 step[2], least[2];
+#pragma unroll
+  for (int g = 0; g < 2; ++g) {
+    const float s = kv4_step(scales[g]) * down, l = kv4_least(scales[g]) * down;
+    step[g] = as_f16(pack_f16(s, s));
+    least[g] = as_f16(pack_f16(l, l));
+  }
+  const f16x2 base = as_f16(0x64006400u);
+#pragma unroll
+  for (int up = 0; up < 2; ++up) {         // lower halves of the words, nibbles 0 to 3, then the upper ones
+    uint32_t m[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) m[i] = __builtin_amdgcn_perm(w[2 * i + 1], w[2 * i], up ? 0x07060302 : 0x05040100);
+#pragma unroll
+    for (int p = 0; p < 4; ++p) {
+      u32x2 v;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const f16x2 n = as_f16((m[i] >> 4 * p & 0x000f000fu) | 0x64006400u) - base;
+        v[i] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(n, step[p >> 1], least[p >> 1]));
+      }
+      put(up * 4 + p, v);
+    }
+  }
+}
+
+template <int GQA>
+__global__ void __launch_bounds__(64 * NWAVES) attn_prefill4_kernel(
+    bf16_t* __restrict__ out,              // [T, H, 128] contiguous
+    float* __restrict__ parts,             // [parts, KVH, PART_ROWS, PART_STRIDE]
+    const bf16_t* __restrict__ q,          // [T, H, 128], row stride q_stride
+    const char* __restrict__ k_cache, const char* __restrict__ v_cache,            // [NB, KVH, BS, 64] bytes
+    const uint32_t* __restrict__ k_scale, const uint32_t* __restrict__ v_scale,    // [NB, KVH, BS, 2] words (step, least)
+    const Item* __restrict__ items, const int* __restrict__ block_tables, const int* __restrict__ seg_pos, float scale,
+    int64_t q_stride, int block_size, uint32_t block_inverse, int max_blocks) {
+  const int g_kv = blockIdx.x, num_kv_heads = gridDim.x;
+  const Item it = items[blockIdx.y];
+  const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, col = lane & 31;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int h = g_kv * GQA + wave % GQA;
+  const int qrow0 = it.r0 + wave / GQA * QBLK, rows_end = min(it.len, it.r0 + NWAVES / GQA * QBLK);
+  const int pos0 = seg_pos[it.seg];                      // keys before the segment's first row
+  const bool active = qrow0 < rows_end;
+  const int my_pos = pos0 + qrow0 + col;
+  const int64_t held = (int64_t)max_blocks * block_size;
+  // keys of this item that the group's last row sees, and this wave's
+  const int end_grp = (int)min((int64_t)min(it.to, pos0 + rows_end), held);
+  const int end_me = active ? min(end_grp, pos0 + min(rows_end, qrow0 + QBLK)) : 0;
+
+  extern __shared__ __attribute__((aligned(1024))) char smem[];          // [buffer][K | V], classes [buffer][key][K, V], [buffer][wave] has any
+  signed char* const classes = (signed char*)smem + 4 * STAGE_BYTES;
+  signed char* const has_class = classes + 2 * CLASSES;
+
+  // ---- Q fragments (B-operand), the row's largest element to 2^14 -------------------------------
+  union Frag { u32x4 u; f16x8_mfma m; };
+  Frag q_frag[8];
+  float c2;                                // scores to base-2 exponents
+  {
+    const int row = active ? min(qrow0 + col, it.len - 1) : it.r0;
+    const short* qp = (const short*)q + (int64_t)(it.row + row) * q_stride + h * 128 + half * 8;
+    bf16x8_vec raw[8];
+    float most = 0.0f;
+#pragma unroll
+    for (int s = 0; s < 8; ++s) {
+      raw[s] = *reinterpret_cast<const bf16x8_vec*>(qp + s * 16);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) most = fmaxf(most, fabsf(bf16_to_f32(raw[s][j])));
+    }
+    const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(most), __float_as_uint(most), false, false);
+    most = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
+    const int e = max((int)(__float_as_uint(most) >> 23) - 127, -90);
+    // a negative scale goes into Q's signs: the max below is taken before scaling
+    const float up = ldexpf(scale < 0.0f ? -1.0f : 1.0f, 14 - e);
+#pragma unroll
+    for (int s = 0; s < 8; ++s)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) q_frag[s].u[j] = pack_f16(bf16_to_f32(raw[s][2 * j]) * up, bf16_to_f32(raw[s][2 * j + 1]) * up);
+    // above zero, so that a masked score stays -inf
+    c2 = fmaxf(ldexpf(fabsf(scale) * 1.44269504088896340736f, e - 14), 1e-37f);
+  }
+  const float THR2 = 8.0f * 1.44269504088896340736f;
+
+  // ---- staging: a thread has 32 values of K row tid / 4 and of V's ------------------------------
+  const int st_row = tid >> 2, st_part = tid & 3;
+  const int* bt = block_tables + (int64_t)it.seg * max_blocks;
+  auto block_of = [&](int key) {           // key / block_size by its reciprocal, which is off by one at most
+    const int n = (int)__umulhi((uint32_t)key, block_inverse), rest = key - n * block_size;
+    return n - (rest < 0) + (rest >= block_size);
+  };
+  auto key_at = [&](int ks) { return min(ks + st_row, end_grp - 1); };
+  u32x4 kr, vr;
+  u32x2 ksc, vsc;
+  int block = 0;
+  auto ask = [&](int ks) { block = bt[block_of(key_at(ks))]; };
+  auto load = [&](int ks) {
+    const int key = key_at(ks);
+    const int64_t row = ((int64_t)block * num_kv_heads + g_kv) * block_size + (key - block_of(key) * block_size);
+    kr = *reinterpret_cast<const u32x4*>(k_cache + row * KV4_BYTES + st_part * 16);
+    vr = *reinterpret_cast<const u32x4*>(v_cache + row * KV4_BYTES + st_part * 16);
+    ksc = *reinterpret_cast<const u32x2*>(k_scale + row * KV4_GROUPS);
+    vsc = *reinterpret_cast<const u32x2*>(v_scale + row * KV4_GROUPS);
+  };
+  auto stage = [&](int buf) {
+    const int kc = row_class(ksc), vc = row_class(vsc);
+    // a V row that is no number: its key is made none, so that the rows that see it are none and the others do not meet it
+    if (kv4_least(vsc[0]) != kv4_least(vsc[0]) || kv4_least(vsc[1]) != kv4_least(vsc[1]) || kv4_step(vsc[0]) != kv4_step(vsc[0]) ||
+        kv4_step(vsc[1]) != kv4_step(vsc[1])) {
+      ksc = u32x2{0x7fc07fc0u, 0x7fc07fc0u};
+      vsc = u32x2{0u, 0u};
+    }
+    char* const k_to = smem + buf * 2 * STAGE_BYTES + st_row * 256;
+    char* const v_to = k_to + STAGE_BYTES;
+    // nibble p of words 4 part..: values 32 (p & 3) + 16 (p >> 2) + 4 part..
+    kv4_to_f16(kr, ksc, ldexpf(1.0f, -16 * kc), [&](int p, const u32x2& v) {
+      const int unit = 4 * (p & 3) + 2 * (p >> 2) + (st_part >> 1);
+      *reinterpret_cast<u32x2*>(k_to + ((unit ^ (st_row & 15)) << 4) + (st_part & 1) * 8) = v;
+    });
+    kv4_to_f16(vr, vsc, ldexpf(1.0f, -16 * vc), [&](int p, const u32x2& v) {
+      *reinterpret_cast<u32x2*>(v_to + (((2 * (p & 3) + (p >> 2)) ^ v_turn(st_row)) << 5) + st_part * 8) = v;
+    });
+    const bool any = __any(kc != 0 || vc != 0);
+    if (any && st_part == 0) *reinterpret_cast<short*>(classes + buf * CLASSES + st_row * 2) = (short)((kc & 0xff) | vc << 8);
+    if (lane == 0) has_class[buf * NWAVES + wave] = any;
+  };
+
+  f32x16 o_acc[4] = {};
+  float m_run = -INFINITY, l_run = 0.0f;
+
+  auto tile = [&](int ks, int kt, int buf) {
+    const char* k_lds = smem + buf * 2 * STAGE_BYTES + (kt - ks) * 256;
+    const bool plain = __builtin_amdgcn_readfirstlane(*reinterpret_cast<const int*>(has_class + buf * NWAVES + (kt - ks) / 16)) == 0;
+    // of key 8 (r >> 2) + .. of a half, where the four waves' rows have any; else what another stage left
+    auto class_of = [&](int sub, int r, int of) {
+      const int key = kt - ks + sub * 32 + acc_row(r, half);
+      return has_class[buf * NWAVES + (key >> 4)] ? (int)classes[buf * CLASSES + key * 2 + of] : 0;
+    };
+    // ---- QK^T: S[key][qrow], 32 keys each ----------------------------
+    f32x16 s_acc[2] = {};
+#pragma unroll
+    for (int s = 0; s < 8; ++s) {
+#pragma unroll
+      for (int sub = 0; sub < 2; ++sub) {
+        const int krow = col + sub * 32;
+        const f16x8_mfma a = *reinterpret_cast<const f16x8_mfma*>(k_lds + krow * 256 + (((s * 2 + half) ^ (krow & 15)) << 4));
+        s_acc[sub] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, q_frag[s].m, s_acc[sub], 0, 0, 0);
+      }
+    }
+    if (!plain) {
+#pragma unroll
+      for (int sub = 0; sub < 2; ++sub)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s_acc[sub][r] = ldexpf(s_acc[sub][r], 16 * class_of(sub, r, 0));
+    }
+    if (kt + 64 > pos0 + qrow0 || kt + 64 > end_grp) {
+      // rows see keys up to their own position, which also ends the segment
+#pragma unroll
+      for (int sub = 0; sub < 2; ++sub)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int key = kt + sub * 32 + acc_row(r, half);
+          if (key > my_pos || key >= end_grp) s_acc[sub][r] = -INFINITY;
+        }
+    }
+
+    // ---- online softmax (row = lane-local) --------------------------------
+    float tmax = s_acc[0][0];
+#pragma unroll
+    for (int sub = 0; sub < 2; ++sub)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) tmax = fmaxf(tmax, s_acc[sub][r]);
+    {
+      auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(tmax), __float_as_uint(tmax), false, false);
+      tmax = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1])) * c2;
+    }
+    // the running max is renewed per row (lane) and only when it grows by more than THR2
+    float alpha = 1.0f;
+    if (!(tmax <= m_run + THR2)) {
+      const float m_new = fmaxf(m_run, tmax);
+      alpha = (m_run == -INFINITY) ? 0.0f : __builtin_amdgcn_exp2f(m_run - m_new);
+      m_run = m_new;
+    }
+    if (__builtin_amdgcn_ballot_w64(alpha != 1.0f)) {
+#pragma unroll
+      for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o_acc[dt][r] *= alpha;
+      l_run *= alpha;
+    }
+    // masked scores: fma(-inf, c2, -m) = -inf, whose exponential is 0
+    const float m_use = m_run == -INFINITY ? 0.0f : m_run;
+    uint32_t pw[2][8];
+    auto expo = [&](auto far) {
+#pragma unroll
+      for (int sub = 0; sub < 2; ++sub)
+#pragma unroll
+        for (int pr = 0; pr < 8; ++pr) {
+          f32x2 p;
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float x = s_acc[sub][2 * pr + e];
+            if constexpr (far) {
+              x *= c2;
+              asm volatile("" : "+v"(x));  // a product of its own
+              x -= m_use;
+            } else {
+              x = __builtin_fmaf(x, c2, -m_use);
+            }
+            p[e] = __builtin_amdgcn_exp2f(x);
+            l_run += p[e];
+          }
+          pw[sub][pr] = __builtin_bit_cast(uint32_t, __builtin_convertvector(p, f16x2));
+        }
+    };
+    // of a max beyond 2^18 the fma would leave what the max itself was rounded by, which is no small number any more
+    if (__builtin_amdgcn_ballot_w64(fabsf(m_use) > 262144.0f)) expo(std::true_type());
+    else expo(std::false_type());
+
+    // ---- PV: O^T += V^T x P, 16 keys at a time ------------------------------
+    const char* v_lds = k_lds + STAGE_BYTES;
+    // this lane's share of a transposed read: row (lane & 15) / 4, 4 elements of 16
+    const int tr_row = half * 8 + ((lane & 15) >> 2), tr_byte = (lane & 3) * 8, tr_slot = (lane >> 4) & 1;
+    auto fragment = [&](const uint32_t* w) {
+      Frag pf;
+      auto r0 = __builtin_amdgcn_permlane32_swap(w[0], w[2], false, false);
+      auto r1 = __builtin_amdgcn_permlane32_swap(w[1], w[3], false, false);
+      pf.u = u32x4{r0[0], r1[0], r0[1], r1[1]};
+      return pf;
+    };
+    auto values = [&](int key, int dt) {
+      union { s16x4 t[2]; f16x8_mfma m; } vf;
+#pragma unroll
+      for (int rd = 0; rd < 2; ++rd) {
+        const int row = key + tr_row + rd * 4;
+        const char* p = v_lds + row * 256 + (((dt * 2 + tr_slot) ^ v_turn(row)) << 5) + tr_byte;
+        vf.t[rd] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p);
+      }
+      return vf.m;
+    };
+    __builtin_amdgcn_s_setprio(1);
+    if (plain) {
+#pragma unroll
+      for (int sub = 0; sub < 2; ++sub)
+#pragma unroll
+        for (int kw = 0; kw < 2; ++kw) {
+          const Frag pf = fragment(&pw[sub][4 * kw]);
+#pragma unroll
+          for (int dt = 0; dt < 4; ++dt) o_acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(values(sub * 32 + kw * 16, dt), pf.m, o_acc[dt], 0, 0, 0);
+        }
+    } else {                               // the rows of each class by themselves, their power put back to their sums
+#pragma unroll
+      for (int sub = 0; sub < 2; ++sub)
+#pragma unroll
+        for (int kw = 0; kw < 2; ++kw)
+#pragma unroll 1
+          for (int c = -7; c <= 8; ++c) {
+            uint32_t w[4];
+            bool some = false;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const bool lo = class_of(sub, 8 * kw + 2 * j, 1) == c, hi = class_of(sub, 8 * kw + 2 * j + 1, 1) == c;
+              w[j] = pw[sub][4 * kw + j] & ((lo ? 0xffffu : 0u) | (hi ? 0xffff0000u : 0u));
+              some |= lo || hi;
+            }
+            if (!__any(some)) continue;
+            const Frag pf = fragment(w);
+#pragma unroll
+            for (int dt = 0; dt < 4; ++dt) {
+              const f32x16 zero = {};
+              const f32x16 own = __builtin_amdgcn_mfma_f32_32x32x16_f16(values(sub * 32 + kw * 16, dt), pf.m, zero, 0, 0, 0);
+#pragma unroll
+              for (int r = 0; r < 16; ++r) o_acc[dt][r] += ldexpf(own[r], 16 * c);
+            }
+          }
+    }
+    __builtin_amdgcn_s_setprio(0);
+  };
+
+  int buf = 0;
+  if (it.from < end_grp) {
+    ask(it.from);
+    load(it.from);
+    ask(it.from + STAGE);
+    stage(0);
+    if (it.from + STAGE < end_grp) {
+      load(it.from + STAGE);
+      ask(it.from + 2 * STAGE);
+    }
+  }
+  for (int ks = it.from; ks < end_grp; ks += STAGE, buf ^= 1) {
+    // this stage is there, and the last one's buffer, whose reads have come back, is free
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    if (ks + STAGE < end_grp) {
+      stage(buf ^ 1);
+      if (ks + 2 * STAGE < end_grp) {
+        load(ks + 2 * STAGE);
+        ask(ks + 3 * STAGE);
+      }
+    }
+    const int end = min(ks + STAGE, end_me);
+#pragma unroll 1
+    for (int kt = ks; kt < end; kt += 64) tile(ks, kt, buf);
+  }
+
+  // ---- merge half-sums, then the result or a partial ----------------------
+  {
+    auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(l_run), __float_as_uint(l_run), false, false);
+    l_run = __uint_as_float(sw[0]) + __uint_as_float(sw[1]);
+  }
+  if (it.part >= 0) {
+    float* const to = parts + (((int64_t)it.part * num_kv_heads + g_kv) * PART_ROWS + wave * QBLK + col) * PART_STRIDE;
+#pragma unroll
+    for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+      for (int g2 = 0; g2 < 4; ++g2)       // regs 4*g2..+3 = d consecutive
+        *reinterpret_cast<f32x4*>(to + dt * 32 + 8 * g2 + 4 * half) =
+            f32x4{o_acc[dt][4 * g2], o_acc[dt][4 * g2 + 1], o_acc[dt][4 * g2 + 2], o_acc[dt][4 * g2 + 3]};
+    if (half == 0) *reinterpret_cast<f32x2*>(to + 128) = f32x2{m_run, l_run};
+  } else if (active && qrow0 + col < rows_end) {
+    const float inv_l = l_run == 0.0f ? 0.0f : 1.0f / l_run;
+    bf16_t* op = out + ((int64_t)(it.row + qrow0 + col) * (num_kv_heads * GQA) + h) * 128;
+#pragma unroll
+    for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+      for (int g2 = 0; g2 < 4; ++g2) {
+        bf16x4_vec o;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[j] = f32_to_bf16(o_acc[dt][4 * g2 + j] * inv_l);
+        *reinterpret_cast<bf16x4_vec*>((short*)op + dt * 32 + 8 * g2 + 4 * half) = o;
+      }
+  }
+}
+
+// A group whose keys were cut: first packed row, rows, first part, parts
+struct Cut {
+  int row, rows, part, parts;
+};
+
+// a wave for two rows of a head at a time, four dims a lane
+__global__ void __launch_bounds__(256) attn_prefill4_merge_kernel(bf16_t* __restrict__ out, const float* __restrict__ parts,
+                                                                  const Cut* __restrict__ cuts, int gqa) {
+  const Cut c = cuts[blockIdx.y];
+  const int g_kv = blockIdx.x, num_kv_heads = gridDim.x;
+  const int d = (threadIdx.x & 31) * 4;
+  for (int i = blockIdx.z * 8 + (threadIdx.x >> 5); i < c.rows * gqa; i += gridDim.z * 8) {
+    const int row = i / gqa, head = i % gqa;
+    // row 32 t + r of head e lies in wave t * gqa + e
+    const float* at = parts + (((int64_t)c.part * num_kv_heads + g_kv) * PART_ROWS + ((row >> 5) * gqa + head) * QBLK + (row & 31)) * PART_STRIDE;
+    const int64_t step = (int64_t)num_kv_heads * PART_ROWS * PART_STRIDE;
+    float M = -INFINITY;
+    for (int p = 0; p < c.parts; ++p) M = fmaxf(M, at[p * step + 128]);
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    float l = 0.0f;
+#pragma unroll 4
+    for (int p = 0; p < c.parts; ++p) {
+      const f32x4 v = *reinterpret_cast<const f32x4*>(at + p * step + d);
+      const f32x2 ml = *reinterpret_cast<const f32x2*>(at + p * step + 128);
+      // a part whose keys none of these rows sees has no max and sums of 0; one that is no number has a sum that is none
+      const float w = ml[0] == -INFINITY ? (ml[1] == 0.0f ? 0.0f : 1.0f) : __builtin_amdgcn_exp2f(ml[0] - M);
+      l += ml[1] * w;
+      acc += v * w;
+    }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    bf16x4_vec o;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) o[r] = f32_to_bf16(acc[r] * inv);
+    *reinterpret_cast<bf16x4_vec*>((short*)out + ((int64_t)(c.row + row) * (num_kv_heads * gqa) + g_kv * gqa + head) * 128 + d) = o;
+  }
+}
+
+// floats of an item's partial for each kv head
+extern "C" int64_t attn_prefill4_part() { return (int64_t)PART_ROWS * PART_STRIDE; }
+
+#define MAX_ITEMS 65535    // of a launch: they lie on the grid's y
+
+// items [n, 8] and cuts [m, 4] int32 on the device. 0, or -1 where the LDS cannot be had
+extern "C" int launch_attn_prefill4(bf16_t* out, float* parts, const bf16_t* q, const void* k_cache, const void* v_cache,
+                                    const void* k_scale, const void* v_scale, const int* items, int n, const int* cuts, int m,
+                                    const int* block_tables, const int* seg_pos, float scale, int num_q_heads, int num_kv_heads,
+                                    int64_t q_stride, int block_size, int max_blocks, hipStream_t stream) {
+  const int gqa = num_q_heads / num_kv_heads;
+  const uint32_t inverse = block_size > 1 ? (uint32_t)(((1ull << 32) + block_size - 1) / block_size) : ~0u;
+  auto go = [&](auto kernel) {
+    if (hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, LDS_BYTES) != hipSuccess) return -1;
+    for (int i = 0; i < n; i += MAX_ITEMS)
+      hipLaunchKernelGGL(kernel, dim3(num_kv_heads, std::min(n - i, MAX_ITEMS)), dim3(64 * NWAVES), LDS_BYTES, stream, out, parts, q,
+                         (const char*)k_cache, (const char*)v_cache, (const uint32_t*)k_scale, (const uint32_t*)v_scale,
+                         reinterpret_cast<const Item*>(items) + i, block_tables, seg_pos, scale, q_stride, block_size, inverse, max_blocks);
+    return 0;
+  };
+  if ((gqa == 1 ? go(attn_prefill4_kernel<1>) : gqa == 2 ? go(attn_prefill4_kernel<2>) : gqa == 4 ? go(attn_prefill4_kernel<4>)
+                                                                                                  : go(attn_prefill4_kernel<8>)) != 0)
+    return -1;
+  for (int i = 0; i < m; i += MAX_ITEMS)
+    hipLaunchKernelGGL(attn_prefill4_merge_kernel, dim3(num_kv_heads, std::min(m - i, MAX_ITEMS), 8), dim3(256), 0, stream, out, parts,
+                       reinterpret_cast<const Cut*>(cuts) + i, gqa);
+  return 0;
+}

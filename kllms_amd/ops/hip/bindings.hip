@@ -193,6 +193,36 @@ torch::Tensor attn_decode4(torch::Tensor q, torch::Tensor k_cache, torch::Tensor
   return out;
 }
 
+extern "C" int64_t attn_prefill4_part();
+extern "C" int launch_attn_prefill4(bf16_t*, float*, const bf16_t*, const void*, const void*, const void*, const void*, const int*, int,
+                                    const int*, int, const int*, const int*, float, int, int, int64_t, int, int, hipStream_t);
+
+// Rows of segments against the 4-bit caches: items [n, 8] and cuts [m, 4] int32 of paged_plan, parts that they use; tables
+// [segments, MAXB], pos [segments] = position of each segment's first row. The segments' own keys and values are in the cache already.
+void attn_prefill4(torch::Tensor out, torch::Tensor q, torch::Tensor k_cache, torch::Tensor v_cache, torch::Tensor items,
+                   torch::Tensor cuts, int64_t parts, torch::Tensor tables, torch::Tensor pos, double scale, torch::Tensor k_scale,
+                   torch::Tensor v_scale) {
+  CHECK_BF16_ROWS(q);
+  check_kv4(k_cache, v_cache, k_scale, v_scale, q, "attn_segments_paged");
+  const int64_t H = q.size(1), KVH = k_cache.size(1), BS = k_cache.size(2);
+  TORCH_CHECK(q.size(2) == 128 && KVH > 0 && H % KVH == 0 && (H / KVH == 1 || H / KVH == 2 || H / KVH == 4 || H / KVH == 8),
+              "attn_segments_paged: head size 128, 1, 2, 4 or 8 heads to a kv head");
+  TORCH_CHECK(out.is_contiguous() && out.sizes() == q.sizes() && out.scalar_type() == at::kBFloat16 && out.device() == q.device(),
+              "attn_segments_paged: result");
+  for (const auto& t : {items, cuts, tables, pos})
+    TORCH_CHECK(t.scalar_type() == at::kInt && t.is_contiguous() && t.device() == q.device(), "attn_segments_paged: plan, tables or positions");
+  TORCH_CHECK(items.dim() == 2 && items.size(1) == 8 && cuts.dim() == 2 && cuts.size(1) == 4 && tables.dim() == 2 &&
+                  pos.numel() == tables.size(0) && parts >= 0 && items.size(0) < (1LL << 31), "attn_segments_paged: plan, tables or positions");
+  if (items.size(0) == 0 || q.size(0) == 0 || k_cache.numel() == 0 || tables.size(1) == 0) return;
+  const c10::DeviceGuard device(q.device());
+  if (!rows_aligned(q)) q = q.clone(at::MemoryFormat::Contiguous);
+  auto room = torch::empty({parts * KVH * attn_prefill4_part()}, q.options().dtype(torch::kFloat));
+  TORCH_CHECK(launch_attn_prefill4(bf(out), room.data_ptr<float>(), cbf(q), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(),
+                                   v_scale.data_ptr(), items.data_ptr<int>(), (int)items.size(0), cuts.data_ptr<int>(), (int)cuts.size(0),
+                                   tables.data_ptr<int>(), pos.data_ptr<int>(), (float)scale, (int)H, (int)KVH, q.stride(0), (int)BS,
+                                   (int)tables.size(1), cur_stream()) == 0, "attn_segments_paged: 128 KB of LDS are not available");
+}
+
 // what a step's kernels write to: 0 bf16, 1 e4m3, 2 four bits
 static int cache_kind(const torch::Tensor& k_cache) {
   return k_cache.scalar_type() == at::kByte ? CACHE_KV4 : k_cache.scalar_type() == at::kFloat8_e4m3fn ? CACHE_FP8 : CACHE_BF16;
@@ -957,6 +987,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("store_kv", &store_kv);
   m.def("rope_store", &rope_store);
   m.def("load_kv4", &load_kv4);
+  m.def("attn_prefill4", &attn_prefill4);
   m.def("attn_decode4", &attn_decode4, py::arg("q"), py::arg("k_cache"), py::arg("v_cache"), py::arg("block_tables"),
         py::arg("context_lens"), py::arg("scale"), py::arg("k_scale"), py::arg("v_scale"), py::arg("arrived") = py::none(),
         py::arg("into") = py::none());

@@ -25,6 +25,7 @@ SOURCES = [
         "elementwise.hip",
         "attn_decode.hip",
         "attn_decode4.hip",
+        "attn_prefill4.hip",
         "kv4_rows.hip",
         "attn_prefill.hip",
         "sampling.hip",

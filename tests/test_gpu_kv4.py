@@ -291,3 +291,114 @@ def test_refusals():
     for bad in (dict(slots=slots.int()), dict(k=new.float()), dict(k=new[:, :1]), dict(ks=ks.float()), dict(slots=torch.zeros(2, dtype=torch.long, device=DEV))):
         with pytest.raises(RuntimeError):
             ops.store_kv(bad.get("k", new), new, kc, vc, bad.get("slots", slots), bad.get("ks", ks), vs)
+
+
+def segments(segs, gqa, KVH, BS, seed=0, spread=0.0):
+    """q rows of segments [(start, rows)], caches and tables; every position up to a segment's last row is stored."""
+    q, kc, vc, ks, vs, tables, n = case([p + r for p, r in segs], gqa, KVH, BS, seed=seed, spread=spread)
+    rows_of = torch.tensor([r for _, r in segs])
+    start = torch.tensor([p for p, _ in segs], dtype=torch.int32)
+    seg = torch.repeat_interleave(torch.arange(len(segs)), rows_of)
+    at = torch.arange(len(seg)) - (rows_of.cumsum(0) - rows_of)[seg]
+    q = rows(len(seg), KVH * gqa, D, seed=seed + 5)
+    return q, kc, vc, ks, vs, tables, start, tables[seg].contiguous(), (start[seg] + at + 1).int()
+
+
+def attend(q, kc, vc, ks, vs, seg_tables, start, tables, lens, scale, segs, plan=None):
+    plan, short = plan or ops.paged_plan(segs, q.shape[1], kc.shape[1], DEV, kc.dtype)
+    return ops.attn_segments_paged(*(t.to(DEV) for t in (q, kc, vc, tables, lens)), scale, plan, short, seg_tables.to(DEV),
+                                   start.to(DEV), ks.to(DEV), vs.to(DEV))
+
+
+SEGMENTS = [[(0, 8)], [(5, 31), (0, 33)], [(300, 40), (0, 3), (77, 64), (1, 1), (500, 8)], [(1000, 150)], [(0, 700)],
+            [(16, 257), (128, 128), (0, 1)], [(3, 7), (2, 6)], [(40, 300), (0, 0), (41, 20)]]
+
+
+@pytest.mark.parametrize("segs", SEGMENTS)
+@pytest.mark.parametrize("gqa,KVH,BS", [(4, 2, 16), (1, 3, 16), (2, 1, 5), (8, 1, 32), (4, 1, 1)])
+def test_segments(segs, gqa, KVH, BS):
+    args = segments(segs, gqa, KVH, BS, seed=gqa + BS)
+    q, kc, vc, ks, vs, seg_tables, start, tables, lens = args
+    out = attend(*args, D ** -0.5, segs)
+    check([out], q, kc, vc, ks, vs, tables, lens, D ** -0.5)
+
+
+@pytest.mark.parametrize("gqa,KVH", [(4, 2), (1, 1), (8, 1)])
+def test_segments_whose_keys_are_cut(gqa, KVH):
+    segs = [(2500, 40), (700, 9), (3000, 8)]
+    args = segments(segs, gqa, KVH, 16, seed=3)
+    q, kc, vc, ks, vs, seg_tables, start, tables, lens = args
+    plan, _ = ops.paged_plan(segs, gqa * KVH, KVH, DEV, kc.dtype)
+    assert plan.parts > 0
+    check([attend(*args, 0.1, segs)], q, kc, vc, ks, vs, tables, lens, 0.1)
+
+
+@pytest.mark.parametrize("spread", [3.0, 20.0])
+def test_segments_with_rows_of_very_different_sizes(spread):
+    """Rows of 2^-60 to 2^60: each slab has a power of its own, sums are put back."""
+    segs = [(200, 70), (0, 40)]
+    args = segments(segs, 4, 2, 16, seed=4, spread=spread)
+    q, kc, vc, ks, vs, seg_tables, start, tables, lens = args
+    scale = 2.0 ** (-3.5 - spread)
+    check([attend(*args, scale, segs)], q, kc, vc, ks, vs, tables, lens, scale)
+
+
+def test_segments_see_what_rows_see_alone():
+    """Keys behind a row, of its own segment too, are not its own: one that is no number does not reach it."""
+    segs = [(50, 100), (20, 64)]
+    q, kc, vc, ks, vs, seg_tables, start, tables, lens = segments(segs, 4, 1, 16, seed=6)
+    blk, off = int(seg_tables[0, 90 // 16]), 90 % 16              # position 90: rows 40 and on of the first segment
+    for t in (ks, vs):
+        held = t[blk, 0, off].clone()
+        t[blk, 0, off, 1] = float("nan")
+        out = attend(q, kc, vc, ks, vs, seg_tables, start, tables, lens, 0.1, segs).cpu()
+        bad = torch.isnan(out)
+        assert not bool(bad[:40].any()) and not bool(bad[100:].any()) and bool(bad[40:100, :, 64:].all())
+        keep = list(range(40)) + list(range(100, 164))
+        check([out[keep]], q[keep], kc, vc, ks, vs, tables[keep], lens[keep], 0.1)
+        t[blk, 0, off] = held
+
+
+def test_segments_of_any_queries_and_scales():
+    segs = [(100, 40)]
+    args = list(segments(segs, 4, 2, 16, seed=7))
+    args[0][3] = 0
+    args[0][5] = (args[0][5].float() * 2.0 ** 90).bfloat16()
+    args[0][6] = (args[0][6].float() * 2.0 ** -90).bfloat16()
+    for scale in (-0.2, 0.05):
+        out = attend(*args, scale, segs).cpu()
+        keep = [r for r in range(40) if r != 5]
+        check([out[keep]], args[0][keep], *args[1:5], args[7][keep], args[8][keep], scale)
+        assert bool(torch.isfinite(out[5]).all())               # one key alone
+
+
+def test_segments_in_strided_rows_and_empty():
+    segs = [(30, 40), (0, 2)]
+    q, kc, vc, ks, vs, seg_tables, start, tables, lens = segments(segs, 4, 2, 16, seed=8)
+    rest = (kc, vc, ks, vs, seg_tables, start, tables, lens, 0.1, segs)
+    want = attend(q, *rest)
+    wide = torch.cat((q, q), 1)
+    plan = ops.paged_plan(segs, 8, 2, DEV, kc.dtype)
+    got = ops.attn_segments_paged(wide.to(DEV)[:, 8:], kc.to(DEV), vc.to(DEV), tables.to(DEV), lens.to(DEV), 0.1, *plan,
+                                  seg_tables.to(DEV), start.to(DEV), ks.to(DEV), vs.to(DEV))
+    assert torch.equal(got, want)
+    assert ops.paged_plan([], 8, 2, DEV, kc.dtype) == (None, []) and ops.paged_plan([(5, 0)], 8, 2, DEV, kc.dtype) == (None, [])
+
+
+def test_segments_replayed():
+    segs = [(900, 70), (100, 30)]
+    args = [t.to(DEV) for t in segments(segs, 4, 2, 16, seed=9)]
+    q = args[0]
+    plan = ops.paged_plan(segs, 8, 2, DEV, torch.uint8)
+    step = lambda: attend(*args, 0.1, segs, plan)
+    step()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = step()
+    for i in range(3):
+        q.copy_(rows(*q.shape, seed=60 + i))
+        want = step().clone()
+        out.zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
