@@ -26,6 +26,8 @@
 
 typedef _Float16 f16x8_mfma __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8_mfma __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
 typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
@@ -198,29 +200,40 @@ __global__ void __launch_bounds__(64 * NWAVES) attn_prefill4_kernel(
     if (lane == 0) has_class[buf * NWAVES + wave] = any;
   };
 
+  typedef __attribute__((address_space(3))) char* lds_t;
+  typedef __attribute__((address_space(3))) const f16x8_mfma* lds_frag;
+  typedef __attribute__((address_space(3))) s16x4* lds_turn;
+  const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_t)smem);
+  // where this lane reads K (row col, unit half: the others are an XOR) and V turned (row (lane & 15) / 4 of its half's eight, 4
+  // elements of 16)
+  uint32_t k_get = lds0 + col * 256 + ((half ^ (col & 15)) << 4);
+  uint32_t v_get = lds0 + STAGE_BYTES + (half * 8 + ((lane & 15) >> 2)) * 256 + ((((lane & 15) >> 2) * 2 ^ (lane >> 4 & 1)) << 5) + (lane & 3) * 8;
+  // All of the item, up to a stage that has a row of another class than 0 (false); ANY: with such rows too. (As branches of one loop
+  // they had all sums copied twice a tile: one of 2100 rows behind 7777 431 us.)
+  auto run = [&](auto any_class) {
+  constexpr bool ANY = decltype(any_class)::value;
   f32x16 o_acc[4] = {};
   float m_run = -INFINITY, l_run = 0.0f;
-
   auto tile = [&](int ks, int kt, int buf) {
-    const char* k_lds = smem + buf * 2 * STAGE_BYTES + (kt - ks) * 256;
-    const bool plain = __builtin_amdgcn_readfirstlane(*reinterpret_cast<const int*>(has_class + buf * NWAVES + (kt - ks) / 16)) == 0;
+    const uint32_t at = buf * 2 * STAGE_BYTES + (kt - ks) * 256;
+    asm volatile("" : "+v"(k_get), "+v"(v_get));       // not all their addresses for the whole loop
+    const bool plain = !ANY || __builtin_amdgcn_readfirstlane(*reinterpret_cast<const int*>(has_class + buf * NWAVES + (kt - ks) / 16)) == 0;
     // of key 8 (r >> 2) + .. of a half, where the four waves' rows have any; else what another stage left
+    int half_now = half;
+    asm volatile("" : "+v"(half_now));
     auto class_of = [&](int sub, int r, int of) {
-      const int key = kt - ks + sub * 32 + acc_row(r, half);
+      const int key = kt - ks + sub * 32 + acc_row(r, half_now);
       return has_class[buf * NWAVES + (key >> 4)] ? (int)classes[buf * CLASSES + key * 2 + of] : 0;
     };
     // ---- QK^T: S[key][qrow], 32 keys each ----------------------------
     f32x16 s_acc[2] = {};
+    const uint32_t k_at = k_get + at;
 #pragma unroll
-    for (int s = 0; s < 8; ++s) {
+    for (int s = 0; s < 8; ++s)
 #pragma unroll
-      for (int sub = 0; sub < 2; ++sub) {
-        const int krow = col + sub * 32;
-        const f16x8_mfma a = *reinterpret_cast<const f16x8_mfma*>(k_lds + krow * 256 + (((s * 2 + half) ^ (krow & 15)) << 4));
-        s_acc[sub] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, q_frag[s].m, s_acc[sub], 0, 0, 0);
-      }
-    }
-    if (!plain) {
+      for (int sub = 0; sub < 2; ++sub)    // row col + 32 sub has the same XOR
+        s_acc[sub] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*(lds_frag)(uintptr_t)((k_at ^ (s << 5)) + sub * 32 * 256), q_frag[s].m, s_acc[sub], 0, 0, 0);
+    if constexpr (ANY) if (!plain) {
 #pragma unroll
       for (int sub = 0; sub < 2; ++sub)
 #pragma unroll
@@ -291,9 +304,7 @@ __global__ void __launch_bounds__(64 * NWAVES) attn_prefill4_kernel(
     else expo(std::false_type());
 
     // ---- PV: O^T += V^T x P, 16 keys at a time ------------------------------
-    const char* v_lds = k_lds + STAGE_BYTES;
-    // this lane's share of a transposed read: row (lane & 15) / 4, 4 elements of 16
-    const int tr_row = half * 8 + ((lane & 15) >> 2), tr_byte = (lane & 3) * 8, tr_slot = (lane >> 4) & 1;
+    const uint32_t v_at = v_get + at;
     auto fragment = [&](const uint32_t* w) {
       Frag pf;
       auto r0 = __builtin_amdgcn_permlane32_swap(w[0], w[2], false, false);
@@ -304,49 +315,65 @@ __global__ void __launch_bounds__(64 * NWAVES) attn_prefill4_kernel(
     auto values = [&](int key, int dt) {
       union { s16x4 t[2]; f16x8_mfma m; } vf;
 #pragma unroll
-      for (int rd = 0; rd < 2; ++rd) {
-        const int row = key + tr_row + rd * 4;
-        const char* p = v_lds + row * 256 + (((dt * 2 + tr_slot) ^ v_turn(row)) << 5) + tr_byte;
-        vf.t[rd] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p);
-      }
+      for (int rd = 0; rd < 2; ++rd)
+        vf.t[rd] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_turn)(uintptr_t)((v_at ^ (dt << 6) ^ (rd << 5)) + (key + rd * 4) * 256));
       return vf.m;
     };
-    __builtin_amdgcn_s_setprio(1);
-    if (plain) {
+    if constexpr (ANY) if (!plain) {       // V with its powers put back, and P, as two bf16 parts each, which hold fp16's bits
 #pragma unroll
       for (int sub = 0; sub < 2; ++sub)
 #pragma unroll
         for (int kw = 0; kw < 2; ++kw) {
-          const Frag pf = fragment(&pw[sub][4 * kw]);
+          uint32_t* const w = &pw[sub][4 * kw];
+          uint32_t parts2[2][4];
 #pragma unroll
-          for (int dt = 0; dt < 4; ++dt) o_acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(values(sub * 32 + kw * 16, dt), pf.m, o_acc[dt], 0, 0, 0);
-        }
-    } else {                               // the rows of each class by themselves, their power put back to their sums
+          for (int j = 0; j < 4; ++j) {
+            const f16x2 h2 = as_f16(w[j]);
+            f32x2 x = {(float)h2[0], (float)h2[1]};
 #pragma unroll
-      for (int sub = 0; sub < 2; ++sub)
+            for (int e = 0; e < 2; ++e) {
+              parts2[e][j] = __builtin_bit_cast(uint32_t, __builtin_convertvector(x, bf16x2_t));
+              x[0] -= __uint_as_float(parts2[e][j] << 16);
+              x[1] -= __uint_as_float(parts2[e][j] & 0xffff0000u);
+            }
+            w[j] = 0u;                     // for the products below
+          }
+          union Frag16 { u32x4 u; bf16x8_mfma m; f16x8_mfma h; };
+          const Frag16 p1 = {fragment(parts2[0]).u}, p2 = {fragment(parts2[1]).u};
 #pragma unroll
-        for (int kw = 0; kw < 2; ++kw)
-#pragma unroll 1
-          for (int c = -7; c <= 8; ++c) {
-            uint32_t w[4];
-            bool some = false;
+          for (int dt = 0; dt < 4; ++dt) {
+            Frag16 v, v1, v2;
+            v.h = values(sub * 32 + kw * 16, dt);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-              const bool lo = class_of(sub, 8 * kw + 2 * j, 1) == c, hi = class_of(sub, 8 * kw + 2 * j + 1, 1) == c;
-              w[j] = pw[sub][4 * kw + j] & ((lo ? 0xffffu : 0u) | (hi ? 0xffff0000u : 0u));
-              some |= lo || hi;
-            }
-            if (!__any(some)) continue;
-            const Frag pf = fragment(w);
+              const f16x2 h2 = as_f16(v.u[j]);
+              f32x2 x;
 #pragma unroll
-            for (int dt = 0; dt < 4; ++dt) {
-              const f32x16 zero = {};
-              const f32x16 own = __builtin_amdgcn_mfma_f32_32x32x16_f16(values(sub * 32 + kw * 16, dt), pf.m, zero, 0, 0, 0);
-#pragma unroll
-              for (int r = 0; r < 16; ++r) o_acc[dt][r] += ldexpf(own[r], 16 * c);
+              for (int e = 0; e < 2; ++e) {
+                const int key = kt - ks + sub * 32 + kw * 16 + half_now * 8 + 2 * j + e;
+                x[e] = ldexpf((float)h2[e], has_class[buf * NWAVES + (key >> 4)] ? 16 * classes[buf * CLASSES + key * 2 + 1] : 0);
+              }
+              v1.u[j] = __builtin_bit_cast(uint32_t, __builtin_convertvector(x, bf16x2_t));
+              x[0] -= __uint_as_float(v1.u[j] << 16);
+              x[1] -= __uint_as_float(v1.u[j] & 0xffff0000u);
+              v2.u[j] = __builtin_bit_cast(uint32_t, __builtin_convertvector(x, bf16x2_t));
             }
+            o_acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v2.m, p2.m, o_acc[dt], 0, 0, 0);
+            o_acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v2.m, p1.m, o_acc[dt], 0, 0, 0);
+            o_acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v1.m, p2.m, o_acc[dt], 0, 0, 0);
+            o_acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v1.m, p1.m, o_acc[dt], 0, 0, 0);
           }
+        }
     }
+    __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+    for (int sub = 0; sub < 2; ++sub)
+#pragma unroll
+      for (int kw = 0; kw < 2; ++kw) {
+        const Frag pf = fragment(&pw[sub][4 * kw]);
+#pragma unroll
+        for (int dt = 0; dt < 4; ++dt) o_acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(values(sub * 32 + kw * 16, dt), pf.m, o_acc[dt], 0, 0, 0);
+      }
     __builtin_amdgcn_s_setprio(0);
   };
 
@@ -364,6 +391,13 @@ __global__ void __launch_bounds__(64 * NWAVES) attn_prefill4_kernel(
   for (int ks = it.from; ks < end_grp; ks += STAGE, buf ^= 1) {
     // this stage is there, and the last one's buffer, whose reads have come back, is free
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    if constexpr (!ANY) {
+      const u32x2 has = *reinterpret_cast<const u32x2*>(has_class + buf * NWAVES);
+      if (__builtin_amdgcn_readfirstlane(has[0] | has[1])) {
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");      // all have read it
+        return false;
+      }
+    }
     if (ks + STAGE < end_grp) {
       stage(buf ^ 1);
       if (ks + 2 * STAGE < end_grp) {
@@ -403,6 +437,9 @@ __global__ void __launch_bounds__(64 * NWAVES) attn_prefill4_kernel(
         *reinterpret_cast<bf16x4_vec*>((short*)op + dt * 32 + 8 * g2 + 4 * half) = o;
       }
   }
+  return true;
+  };
+  if (!run(std::false_type())) run(std::true_type());
 }
 
 // A group whose keys were cut: first packed row, rows, first part, parts
