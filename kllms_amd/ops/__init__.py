@@ -263,25 +263,28 @@ class Kv4Groups(NamedTuple):
 
 KV4_GROUP_ROWS = 8           # segments shorter than this attend row by row
 _KV4_UNITS = 256
-_KV4_ITEM = (8.0, 0.027)     # us of an item, and of each of its keys
+# us of an item and of each of its keys, of a second launch and of each partial's way through memory. One segment, 32 / 8 heads:
+# 2048 rows behind 256 / 4096 / 8192 (248 items) 90, 213, 348; 146 behind 1536 in items of 256 / 512 / all keys 33, 32, 61
+_KV4_ITEM, _KV4_KEY, _KV4_MERGE, _KV4_PART = 12.0, 0.036, 4.0, 0.04
 
 
 def _kv4_cuts(keys, kv_heads: int) -> int:
     """How many keys an item of groups of so many keys each has at most: what makes the rounds of all compute units
     shortest, sums' way through memory and the second launch included."""
-    total, longest = sum(keys), max(keys)
-
-    def cost(most):
-        items = kv_heads * sum(-(-k // most) for k in keys)
-        parts = items - kv_heads * sum(k <= most for k in keys)
-        at, key = _KV4_ITEM
-        return -(-items // _KV4_UNITS) * (at + min(most, longest) * key) + (5.0 + parts * 0.06 if parts else 0.0)
-
-    tries = {-(-longest // 128) * 128}
-    for waves in (1, 2, 3, 4, 6):
-        tries.add(max(256, -(-total * kv_heads // (_KV4_UNITS * waves * 128)) * 128))
-        tries.add(max(256, -(-total * kv_heads // ((_KV4_UNITS - min(255, kv_heads * len(keys) // 2)) * waves * 128)) * 128))
-    return min(sorted(tries, reverse=True), key=cost)
+    keys = torch.tensor(keys, dtype=torch.int32)
+    longest = int(keys.max())
+    best, least = longest, float("inf")
+    # halves, thirds .. of the longest, no shorter than two stages; whole groups where that is as good
+    for pieces in (1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 24, 32, 48, 64, 128):
+        most = -(-longest // (pieces * 128)) * 128
+        if pieces > 1 and most < 256:
+            break
+        n = (keys + (most - 1)) // most
+        items, parts = kv_heads * int(n.sum()), kv_heads * int(n[n > 1].sum())
+        cost = -(-items // _KV4_UNITS) * (_KV4_ITEM + min(most, longest) * _KV4_KEY) + (_KV4_MERGE + parts * _KV4_PART if parts else 0.0)
+        if cost < least:
+            best, least = most, cost
+    return best
 
 
 def kv4_plan(segs, heads: int, kv_heads: int, device) -> tuple:

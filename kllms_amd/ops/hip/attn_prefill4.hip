@@ -83,6 +83,8 @@ __device__ __forceinline__ void kv4_to_f16(const u32x4& w, const u32x2& scales, 
     least[g] = as_f16(pack_f16(l, l));
   }
   const f16x2 base = as_f16(0x64006400u);
+  uint32_t mask = 0x000f000fu, magic = 0x64006400u;
+  asm volatile("" : "+s"(mask), "+v"(magic));          // one instruction for both: it takes no two literals
 #pragma unroll
   for (int up = 0; up < 2; ++up) {         // lower halves of the words, nibbles 0 to 3, then the upper ones
     uint32_t m[2];
@@ -93,7 +95,7 @@ __device__ __forceinline__ void kv4_to_f16(const u32x4& w, const u32x2& scales, 
       u32x2 v;
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const f16x2 n = as_f16((m[i] >> 4 * p & 0x000f000fu) | 0x64006400u) - base;
+        const f16x2 n = as_f16((m[i] >> 4 * p & mask) | magic) - base;
         v[i] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(n, step[p >> 1], least[p >> 1]));
       }
       put(up * 4 + p, v);
@@ -398,16 +400,20 @@ __global__ void __launch_bounds__(64 * NWAVES) attn_prefill4_kernel(
         return false;
       }
     }
-    if (ks + STAGE < end_grp) {
-      stage(buf ^ 1);
-      if (ks + 2 * STAGE < end_grp) {
-        load(ks + 2 * STAGE);
-        ask(ks + 3 * STAGE);
+    auto next = [&] {
+      if (ks + STAGE < end_grp) {
+        stage(buf ^ 1);
+        if (ks + 2 * STAGE < end_grp) {
+          load(ks + 2 * STAGE);
+          ask(ks + 3 * STAGE);
+        }
       }
-    }
+    };
+    if (wave < NWAVES / 2) next();
     const int end = min(ks + STAGE, end_me);
 #pragma unroll 1
     for (int kt = ks; kt < end; kt += 64) tile(ks, kt, buf);
+    if (wave >= NWAVES / 2) next();        // the other wave of a SIMD: one makes keys while the other multiplies
   }
 
   // ---- merge half-sums, then the result or a partial ----------------------
@@ -447,18 +453,20 @@ struct Cut {
   int row, rows, part, parts;
 };
 
-// a wave for two rows of a head at a time, four dims a lane
+// 32 lanes for a row of a head, four dims a lane
 __global__ void __launch_bounds__(256) attn_prefill4_merge_kernel(bf16_t* __restrict__ out, const float* __restrict__ parts,
                                                                   const Cut* __restrict__ cuts, int gqa) {
   const Cut c = cuts[blockIdx.y];
   const int g_kv = blockIdx.x, num_kv_heads = gridDim.x;
   const int d = (threadIdx.x & 31) * 4;
-  for (int i = blockIdx.z * 8 + (threadIdx.x >> 5); i < c.rows * gqa; i += gridDim.z * 8) {
+  const int i = blockIdx.z * 8 + (threadIdx.x >> 5);
+  if (i < c.rows * gqa) {
     const int row = i / gqa, head = i % gqa;
     // row 32 t + r of head e lies in wave t * gqa + e
     const float* at = parts + (((int64_t)c.part * num_kv_heads + g_kv) * PART_ROWS + ((row >> 5) * gqa + head) * QBLK + (row & 31)) * PART_STRIDE;
     const int64_t step = (int64_t)num_kv_heads * PART_ROWS * PART_STRIDE;
     float M = -INFINITY;
+#pragma unroll 8
     for (int p = 0; p < c.parts; ++p) M = fmaxf(M, at[p * step + 128]);
     f32x4 acc = {0.f, 0.f, 0.f, 0.f};
     float l = 0.0f;
@@ -503,7 +511,7 @@ extern "C" int launch_attn_prefill4(bf16_t* out, float* parts, const bf16_t* q, 
                                                                                                   : go(attn_prefill4_kernel<8>)) != 0)
     return -1;
   for (int i = 0; i < m; i += MAX_ITEMS)
-    hipLaunchKernelGGL(attn_prefill4_merge_kernel, dim3(num_kv_heads, std::min(m - i, MAX_ITEMS), 8), dim3(256), 0, stream, out, parts,
+    hipLaunchKernelGGL(attn_prefill4_merge_kernel, dim3(num_kv_heads, std::min(m - i, MAX_ITEMS), PART_ROWS / 8), dim3(256), 0, stream, out, parts,
                        reinterpret_cast<const Cut*>(cuts) + i, gqa);
   return 0;
 }
