@@ -9,10 +9,11 @@
 // values, of 8 bits, so a quotient that is no half itself is 2^-17 of it away from one.
 //
 // On the ring and tiles of tile_product.h, to which a row of K integers is one of K / 2 bf16: as many bytes and
-// matrix instructions of twice the products. Up to 128 rows the stream of W is the bound, in tiles of 64 or 128 rows of W
-// (linear_rows.hip has the reasons); above, tiles of 256 and the matrix units (linear_tiles.hip). A product of few tiles is shared out
-// over K; each workgroup leaves its sums past the L2 and the last one to arrive adds them up. The counters for that are zeroed by the
-// launch that makes the codes, which comes before anyway.
+// matrix instructions of twice the products. Where W's stream or the depth of K is the bound, tiles of 64 or 128 rows of W
+// (linear_rows.hip has the reasons), two workgroups to a compute unit where the ring leaves room; else tiles of 256 and the
+// matrix units (linear_tiles.hip). int8_plan weighs them. A product of few tiles is shared out over K: each workgroup leaves its
+// sums past the L2 and the last one to arrive adds them up. The counters for that are zeroed by the launch that makes the codes,
+// which comes before anyway.
 //
 // K is a multiple of 16; the codes' rows are filled up to whole stages with zeros, which what W has behind a row meets.
 
@@ -120,7 +121,7 @@ extern "C" void launch_int8_rows(int8_t* codes, float* scales, const bf16_t* x, 
 #undef LI_ROWS
 }
 
-// ---- up to 128 rows ------------------------------------------------------------------------------
+// ---- few rows or columns -------------------------------------------------------------------------
 
 // linear_rows_kernel of whole numbers. K, padded: bytes of a row of w and of x. PART leaves fp32 sums [splits, M, N], the
 // others add their shares up (part, count) and write bf16.
@@ -200,22 +201,66 @@ __global__ void __launch_bounds__(TP_THREADS, 1) linear_int8_rows_kernel(
 
 #define LI_UNITS 256       // compute units
 
+// Which kernel a product goes to: ni 2 or 4, tiles of 64 or 128 rows of W by 32 * mj of x, shared out over K; ni 8, tiles of 256
+// by 32 * mj, the last round of them in shares or not.
 struct Int8Plan {
   int ni, mj, m_tiles, splits;
 };
 
-// Tiles of up to 128 rows, as linear_plan has them for K / 2 bf16, and shares of K: one workgroup for each compute unit, four
-// stages at least
-static Int8Plan int8_plan(int M, int N, int K, int form) {
-  Int8Plan p;
-  p.m_tiles = 1;
-  p.mj = (M + 31) / 32;
-  if (form == LI_SILU) p.ni = N <= 256 * 64 || (N > 256 * 128 && p.mj == 1) ? 2 : 4;
-  else p.ni = N <= 8448 && !(p.mj == 4 && N >= 4096 && K >= 16384) ? 2 : 4;
-  const int tiles = ((form == LI_SILU ? N / 2 : N) + (form == LI_SILU ? 16 : 32) * p.ni - 1) / ((form == LI_SILU ? 16 : 32) * p.ni);
-  const int most = int8_rows_padded(K) / LI_STAGE / 4, s = (LI_UNITS + 8) / tiles;
-  p.splits = s < 1 || most < 1 ? 1 : s < most ? s : most;
-  return p;
+// us of a stage: of a workgroup that has a compute unit to itself, and of two that share one (160 KB of LDS hold two of those
+// with 80); [ni / 4][mj]
+static const double LI_ALONE[2][5] = {{0, 0.16, 0.22, 0.27, 0.32}, {0, 0, 0.32, 0.43, 0.58}};
+static const double LI_PAIR[2][5] = {{0, 0.38, 0.38, 0.46, 0.49}, {0, 0, 0.57, 0, 0}};
+static const double LI_TILE[9] = {0, 0, 0.42, 0.60, 0.72, 0.87, 1.0, 1.2, 1.3};   // of tiles of 256
+
+static constexpr int li_ring(int ni, int mj) { return ni == 2 || mj <= 2 ? 80 : 160; }   // KB
+
+// The tiles that take the least time by what rounds of compute units, stages, the stream of W, reads through the caches and
+// sums through memory take. The constants are fitted to 4500 measured products, 10 matrices of 1024 x 4096 to 28672 x 4096 by 1
+// to 2100 rows in all tiles; what they pick is 0.5% behind the best tiles on average, 11% at most. With tiles of 64 rows of W
+// and 32 * ceil(M / 32) of x up to 128 rows and those of 256 above: 4608 x 3584, 333 rows, 29.7 us and so 21.9; 2048 x 2048,
+// 128 rows, 15.5 and 11.2; 4096 x 4096, 512 rows, 34.7 and 22.
+static Int8Plan int8_plan(int64_t M, int64_t N, int64_t K, int form) {
+  const bool gated = form == LI_SILU;
+  const int64_t columns = gated ? N / 2 : N, stages = int8_rows_padded((int)K) / LI_STAGE;
+  const double stream = (double)N * K / 5.1e6;
+  Int8Plan best = {2, 1, 1, 1};
+  double least = 1e300;
+  for (int ni = 2; ni <= 4; ni += 2)
+    for (int mj = M <= 32 ? 1 : 2; mj <= (M <= 32 ? 1 : 4); ++mj) {
+      if (ni == 4 && mj == 1) continue;
+      const int64_t m_tiles = (M + 32 * mj - 1) / (32 * mj), wide = (gated ? 16 : 32) * ni;
+      if (mj > 2 && M <= 32 * (mj - 1)) continue;
+      if (form == LI_PART && m_tiles > LI_UNITS) continue;
+      const int64_t tiles = m_tiles * ((columns + wide - 1) / wide);
+      for (int64_t splits = 1; splits <= 8 && (splits == 1 || (splits * 3 <= stages && tiles * splits <= 600)); ++splits) {
+        const double deep = (double)((stages + splits - 1) / splits);
+        const int64_t of_unit = (tiles * splits + LI_UNITS - 1) / LI_UNITS;
+        const double run = li_ring(ni, mj) == 80
+                               ? (double)(of_unit / 2) * LI_PAIR[ni / 4][mj] * deep + (double)(of_unit % 2) * LI_ALONE[ni / 4][mj] * deep +
+                                     4.0 * (double)((of_unit + 1) / 2)
+                               : (double)of_unit * (LI_ALONE[ni / 4][mj] * deep + 4.0);
+        const double cost = (run > stream ? run : stream) + (double)(tiles * splits) * deep * (ni + mj) * 4096 / 44e6 +
+                            (splits > 1 ? 0.5 + 0.21 * (double)(ni * mj * splits) : 0.0);
+        if (cost < least) least = cost, best = {ni, mj, (int)m_tiles, (int)splits};
+      }
+    }
+  if (form == LI_PART || M <= 128) return best;
+  const int64_t n_tiles = (columns + (gated ? 127 : 255)) / (gated ? 128 : 256);
+  for (int mj = 8; mj >= 2; --mj) {
+    const int64_t m_tiles = (M + 32 * mj - 1) / (32 * mj), tiles = m_tiles * n_tiles, unit = (tiles + 7) / 8, rest = unit % TP_SLOTS;
+    const double round = LI_TILE[mj] * (double)stages + 5.9, reads = (double)(tiles * stages) * (8 + mj) * 4096 / 44e6;
+    const double whole = (double)((unit + TP_SLOTS - 1) / TP_SLOTS) * round;
+    if ((whole > stream ? whole : stream) + reads < least)
+      least = (whole > stream ? whole : stream) + reads, best = {8, mj, (int)m_tiles, 1};
+    if (stages < 16 || rest == 0 || rest > TP_SLOTS / 2) continue;
+    int64_t shares = TP_SLOTS / rest < TP_SHARES ? TP_SLOTS / rest : TP_SHARES;
+    shares = shares < stages / 8 ? shares : stages / 8;
+    const double shared = (double)(unit / TP_SLOTS) * round + LI_TILE[mj] * (double)stages / (double)shares + 10 + 0.48 * (double)(mj * shares);
+    if ((shared > stream ? shared : stream) + reads < least)
+      least = (shared > stream ? shared : stream) + reads, best = {8, mj, (int)m_tiles, (int)shares};
+  }
+  return best;
 }
 
 extern "C" int linear_int8_splits(int M, int N, int K) { return int8_plan(M, N, K, LI_PART).splits; }
@@ -226,7 +271,7 @@ extern "C" int linear_int8_splits(int M, int N, int K) { return int8_plan(M, N, 
 template <int NI, int MJ, int FORM, bool ONCE>
 static int linear_int8_rows_go(const Int8Plan& p, void* out, const int8_t* x, const float* xs, const int8_t* w, const float* ws,
                                const bf16_t* bias, float* part, int* count, int M, int N, int K, hipStream_t stream) {
-  constexpr int KB = NI == 2 || MJ <= 2 ? 80 : 160, BN = (FORM == LI_SILU ? 16 : 32) * NI;
+  constexpr int KB = li_ring(NI, MJ), BN = (FORM == LI_SILU ? 16 : 32) * NI;
   if (!tp_lds_ready(reinterpret_cast<const void*>(linear_int8_rows_kernel<NI, MJ, FORM, KB, ONCE>))) return -1;
   constexpr int LDS = TileRing<MJ, NI, KB * 1024>::STRIDE * TileRing<MJ, NI, KB * 1024>::RING;
   const int64_t all = (int64_t)(((FORM == LI_SILU ? N / 2 : N) + BN - 1) / BN) * p.splits * p.m_tiles;
@@ -239,7 +284,7 @@ template <int FORM>
 static int linear_int8_rows_form(const Int8Plan& p, void* out, const int8_t* x, const float* xs, const int8_t* w, const float* ws,
                                  const bf16_t* bias, float* part, int* count, int M, int N, int K, bool once, hipStream_t stream) {
   const int64_t bytes = (int64_t)N * K;
-  once = once ? bytes >= LI_ONCE : bytes >= LI_ONCE_ALONE;
+  once = p.m_tiles == 1 && (once ? bytes >= LI_ONCE : bytes >= LI_ONCE_ALONE);   // row tiles read W one after the other
 #define LI_CASE(NI, MJ)                                                                                                           \
   if (p.ni == NI && p.mj == MJ)                                                                                                   \
     return once ? linear_int8_rows_go<NI, MJ, FORM, true>(p, out, x, xs, w, ws, bias, part, count, M, N, K, stream)               \
@@ -248,7 +293,6 @@ static int linear_int8_rows_form(const Int8Plan& p, void* out, const int8_t* x, 
   LI_CASE(2, 2);
   LI_CASE(2, 3);
   LI_CASE(2, 4);
-  LI_CASE(4, 1);
   LI_CASE(4, 2);
   LI_CASE(4, 3);
   LI_CASE(4, 4);
@@ -256,7 +300,7 @@ static int linear_int8_rows_form(const Int8Plan& p, void* out, const int8_t* x, 
   return -1;
 }
 
-// ---- more rows -----------------------------------------------------------------------------------
+// ---- large products ------------------------------------------------------------------------------
 
 #define LI_BAND 8          // row tiles of a band
 
@@ -329,30 +373,6 @@ __global__ void __launch_bounds__(TP_THREADS, 1) linear_int8_tiles_kernel(
   }
 }
 
-// us of a round of tiles of 32 * MJ rows by 256 columns and 64 stages, with all compute units at work
-static const int LI_COST[9] = {0, 0, 44, 49, 60, 68, 77, 88, 97};
-
-// MJ of the tiles of more than 128 rows, + 16 where the last round is shared out over K
-static int int8_tiles_pick(int64_t M, int64_t N, int64_t K, bool gated) {
-  const int64_t n_tiles = gated ? (N + 127) / 128 : (N + 255) / 256, stages = int8_rows_padded((int)K) / LI_STAGE;
-  int best = 8;
-  double least = 1e30;
-  for (int mj = 8; mj >= 2; --mj) {
-    const int64_t tiles = (M + 32 * mj - 1) / (32 * mj) * n_tiles;
-    const double round = LI_COST[mj] * (stages / 64.0);
-    const double whole = (tiles + LI_UNITS - 1) / LI_UNITS * round;
-    if (whole < least) least = whole, best = mj;
-    const int64_t unit = (tiles + 7) / 8, rest = unit % TP_SLOTS;
-    if (stages < 16 || rest == 0 || rest > TP_SLOTS / 2) continue;
-    int64_t shares = TP_SLOTS / rest < TP_SHARES ? TP_SLOTS / rest : TP_SHARES;
-    shares = shares < stages / 8 ? shares : stages / 8;
-    // the sums' way through memory: 16 us for four shares of 64 rows, 28 for three of 256
-    const double shared = unit / TP_SLOTS * round + round / shares + 10 + 0.75 * mj * shares;
-    if (shared < least) least = shared, best = mj + 16;
-  }
-  return best;
-}
-
 template <int ACT, int MJ>
 static int linear_int8_tiles_go(void* out, const int8_t* x, const float* xs, const int8_t* w, const float* ws, const bf16_t* bias,
                                 float* part, int* count, int M, int N, int K, hipStream_t stream) {
@@ -367,41 +387,37 @@ static int linear_int8_tiles_go(void* out, const int8_t* x, const float* xs, con
 
 // ---- the calls -----------------------------------------------------------------------------------
 
-#define LI_ROWS_MOST 128
-
 // floats of part and zeros of count that a product (form 0 or 1; N: rows of w) takes, 0 where it has no shares
 extern "C" int64_t linear_int8_room(int M, int N, int K, int form, int* zeros) {
   *zeros = 0;
-  if (M <= LI_ROWS_MOST) {
-    const Int8Plan p = int8_plan(M, N, K, form);
-    if (p.splits == 1) return 0;
-    const int64_t tiles = ((form == LI_SILU ? N / 2 : N) + (form == LI_SILU ? 16 : 32) * p.ni - 1) / ((form == LI_SILU ? 16 : 32) * p.ni);
-    *zeros = (int)(tiles * p.m_tiles);
-    return tiles * p.m_tiles * p.splits * (p.ni * p.mj * TP_THREADS * 4);
+  const Int8Plan p = int8_plan(M, N, K, form);
+  if (p.splits == 1) return 0;
+  if (p.ni == 8) {
+    *zeros = LI_UNITS;
+    return (int64_t)LI_UNITS * 256 * 32 * p.mj;
   }
-  const int mj = int8_tiles_pick(M, form == LI_SILU ? N / 2 : N, K, form == LI_SILU);
-  if (mj < 16) return 0;
-  *zeros = LI_UNITS;
-  return (int64_t)LI_UNITS * 256 * 32 * (mj & 15);
+  const int wide = (form == LI_SILU ? 16 : 32) * p.ni;
+  const int64_t tiles = (int64_t)p.m_tiles * (((form == LI_SILU ? N / 2 : N) + wide - 1) / wide);
+  *zeros = (int)tiles;
+  return tiles * p.splits * (p.ni * p.mj * TP_THREADS * 4);
 }
 
 // form 0: bf16 [M, N] (+ bias), 1: silu(gate) * up bf16 [M, N / 2]; 2: fp32 sums [splits, M, N] of up to 128 rows. part and
 // count (zeroed): of linear_int8_room. 0, or -1 where the LDS cannot be had.
 extern "C" int launch_linear_int8(void* out, const int8_t* x, const float* xs, const int8_t* w, const float* ws, const bf16_t* bias,
                                   float* part, int* count, int M, int N, int K, int form, bool once, hipStream_t stream) {
-  if (M <= LI_ROWS_MOST) {
-    const Int8Plan p = int8_plan(M, N, K, form);
+  const Int8Plan p = int8_plan(M, N, K, form);
+  if (p.ni < 8)
     return form == LI_SILU   ? linear_int8_rows_form<LI_SILU>(p, out, x, xs, w, ws, bias, part, count, M, N, K, once, stream)
            : form == LI_PART ? linear_int8_rows_form<LI_PART>(p, out, x, xs, w, ws, bias, part, count, M, N, K, once, stream)
                              : linear_int8_rows_form<LI_BF16>(p, out, x, xs, w, ws, bias, part, count, M, N, K, once, stream);
-  }
   const bool gated = form == LI_SILU;
   const int n = gated ? N / 2 : N;
 #define LI_CASE(MJ)                                                                                                 \
   case MJ:                                                                                                          \
     return gated ? linear_int8_tiles_go<1, MJ>(out, x, xs, w, ws, bias, part, count, M, n, K, stream)               \
                  : linear_int8_tiles_go<0, MJ>(out, x, xs, w, ws, bias, part, count, M, n, K, stream)
-  switch (int8_tiles_pick(M, n, K, gated) & 15) {
+  switch (p.mj) {
     LI_CASE(2);
     LI_CASE(3);
     LI_CASE(4);

@@ -225,6 +225,14 @@ __device__ __forceinline__ void tile_product(A (&acc)[NI][MJ], const W& w, const
 #pragma unroll
   for (int r = 0; r < NR; ++r) read(0, r, 0);
 
+  if constexpr (std::is_same<A, i32x4>::value) {
+    // whole numbers begin as what they stay, accumulation registers; of constants the compiler makes sums that it moves between
+    // registers in every stage (6144 x 4096, 2100 rows in tiles of 160: 102 us; 88 so)
+#pragma unroll
+    for (int i = 0; i < NI; ++i)
+#pragma unroll
+      for (int j = 0; j < MJ; ++j) asm volatile("" : "+a"(acc[i][j]));
+  }
   uint32_t buf = 0;
 #pragma unroll 1
   for (int s = 0; s < stages; ++s) {
