@@ -589,6 +589,10 @@ extern "C" int linear_int8_splits(int M, int N, int K);
 extern "C" int launch_linear_int8(void* out, const int8_t* x, const float* xs, const int8_t* w, const float* ws, const bf16_t* bias,
                                   float* part, int* count, int M, int N, int K, int form, bool once, hipStream_t stream);
 
+extern "C" bool linear_int8_few(int M, int N, int K, int form);
+extern "C" int launch_linear_int8_few(void* out, const bf16_t* x, int64_t x_stride, const int8_t* w, const float* ws, const bf16_t* bias, int M,
+                                      int N, int K, int form, bool once, hipStream_t stream);
+
 static bool on_16_bytes_at(const torch::Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0; }
 
 static void check_int8_rows(const torch::Tensor& x, const char* who) {
@@ -647,6 +651,11 @@ torch::Tensor linear_int8(torch::Tensor x, torch::Tensor w, torch::Tensor w_scal
   auto out = form == 2 ? torch::empty({S, M, N}, x.options().dtype(torch::kFloat)) : torch::empty({M, form == 1 ? N / 2 : N}, x.options());
   if (M == 0) return out;
   x = int8_readable(x);
+  if (linear_int8_few((int)std::min<int64_t>(M, 1 << 20), (int)N, (int)K, (int)form)) {
+    launch_linear_int8_few(out.data_ptr(), cbf(x), x.stride(0), w.data_ptr<int8_t>(), w_scale.data_ptr<float>(), bias ? cbf(*bias) : nullptr,
+                           (int)M, (int)N, (int)K, (int)form, once, cur_stream());
+    return out;
+  }
   int zeros = 0;
   const int64_t room = form == 2 ? 0 : linear_int8_room((int)M, (int)N, (int)K, (int)form, &zeros);
   const int64_t padded = int8_rows_padded((int)K);

@@ -11,7 +11,7 @@
 // On the ring and tiles of tile_product.h, to which a row of K integers is one of K / 2 bf16: as many bytes and
 // matrix instructions of twice the products. Where W's stream or the depth of K is the bound, tiles of 64 or 128 rows of W
 // (linear_rows.hip has the reasons), two workgroups to a compute unit where the ring leaves room; else tiles of 256 and the
-// matrix units (linear_tiles.hip). int8_plan weighs them. A product of few tiles is shared out over K: each workgroup leaves its
+// matrix units (linear_tiles.hip). int8_plan weighs them. Up to 8 rows go in one launch that makes the codes too. A product of few tiles is shared out over K: each workgroup leaves its
 // sums past the L2 and the last one to arrive adds them up. The counters for that are zeroed by the launch that makes the codes,
 // which comes before anyway.
 //
@@ -42,10 +42,21 @@ struct Int8Row {
     inverse = sound && m > 0.0f ? 1.0f / most : 0.0f;
     scale = sound ? m / 127.0f : __uint_as_float(0x7fc00000u);       // such a row is NaN as a whole
   }
-  __device__ __forceinline__ uint32_t code(float x) const {          // one byte
+  // its code is the lowest byte: added to 1.5 * 2^23, a number this small is rounded as rint does and stands in the last bits. No
+  // number passes 127 by as much as that sees; of a row that is not sound the codes do not matter.
+  __device__ __forceinline__ uint32_t code(float x) const {
     const float t = x * up, q = t * inverse;
-    const float n = __builtin_rintf(__builtin_fmaf(__builtin_fmaf(-q, most, t), inverse, q));
-    return (uint32_t)(int)fminf(fmaxf(n, -127.0f), 127.0f) & 0xffu;
+    return __float_as_uint(__builtin_fmaf(__builtin_fmaf(-q, most, t), inverse, q) + 12582912.0f);
+  }
+  __device__ __forceinline__ u32x2 codes(const u16x8& x) const {
+    uint32_t c[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) c[j] = code(bf16_to_f32((short)x[j]));
+    auto four = [&](int j) {
+      return __builtin_amdgcn_perm(__builtin_amdgcn_perm(c[j + 3], c[j + 2], 0x0c0c0400u), __builtin_amdgcn_perm(c[j + 1], c[j], 0x0c0c0400u),
+                                   0x05040100u);
+    };
+    return u32x2{four(0), four(4)};
   }
 };
 
@@ -88,12 +99,7 @@ __global__ void __launch_bounds__(256) int8_rows_kernel(int8_t* __restrict__ cod
   }
   const Int8Row by(most);
   if (lane == 0) scales[m] = by.scale;
-  auto put = [&](int i, const u16x8& a) {
-    uint32_t w[2] = {0u, 0u};
-#pragma unroll
-    for (int j = 0; j < 8; ++j) w[j >> 2] |= by.code(bf16_to_f32((short)a[j])) << ((j & 3) * 8);
-    to[i] = u32x2{w[0], w[1]};
-  };
+  auto put = [&](int i, const u16x8& a) { to[i] = by.codes(a); };
   if constexpr (R > 0) {
 #pragma unroll
     for (int r = 0; r < R; ++r)
@@ -119,6 +125,219 @@ extern "C" void launch_int8_rows(int8_t* codes, float* scales, const bf16_t* x, 
   else if (padded <= 16384) LI_ROWS(256, 8);
   else LI_ROWS(256, 0);
 #undef LI_ROWS
+}
+
+// ---- up to 8 rows of x, in one launch --------------------------------------------------------------
+
+#define LI_UNITS 256       // compute units
+
+#define LF_WAVES 8
+#define LF_ROWS 8
+
+// A workgroup takes 16 rows of W (16 of gate and 16 of up), a wave an eighth of K: everything it reads is on its way from its
+// first instructions on, x first, since loads come back in order. While W comes, the rows' maxima are found (one barrier) and
+// each wave makes the codes of its own part of K, which it alone reads. W goes from memory to the registers that the matrix
+// cores take it from, NS stages a wave. The waves' sums meet in LDS. R: rows of x, M of which exist; the others are not looked at.
+template <int NS, int R, int T, int FORM, bool ONCE>
+__global__ void __launch_bounds__(64 * LF_WAVES) linear_int8_few_kernel(void* __restrict__ out, const bf16_t* __restrict__ x,
+                                                                       int64_t x_stride, const int8_t* __restrict__ w,
+                                                                       const float* __restrict__ ws, const bf16_t* __restrict__ bias,
+                                                                       int M, int N, int K) {
+  constexpr bool GATED = FORM == LI_SILU;
+  constexpr int V = (NS + 3) / 4, ROW = NS * LI_STAGE + 16;   // 16: rows at different banks
+  constexpr int CODES = LF_WAVES * R * ROW, SUMS = LF_WAVES * T * 1024;
+  __shared__ __attribute__((aligned(16))) char smem[CODES > SUMS ? CODES : SUMS];
+  __shared__ __attribute__((aligned(16))) uint32_t tops[(R + 1) / 2][LF_WAVES];
+  const int lane = threadIdx.x & 63, col = lane & 15, grp = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int columns = GATED ? N / 2 : N, n0 = blockIdx.x * (GATED ? 16 : 16 * T);
+  const int stages_all = (K + LI_STAGE - 1) / LI_STAGE;
+  const int first = stages_all * wave / LF_WAVES, stages = stages_all * (wave + 1) / LF_WAVES - first, k0 = first * LI_STAGE;
+  constexpr uint32_t NOWHERE = 0x7fffffffu;        // behind every range: zeros
+  u16x8 v[R][V];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const auto row = __builtin_amdgcn_make_buffer_rsrc(const_cast<bf16_t*>(x + (int64_t)min(r, M - 1) * x_stride), 0, K * 2, 0x00020000);
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const int i = lane + j * 64;
+      v[r][j] = __builtin_bit_cast(u16x8, __builtin_amdgcn_raw_buffer_load_b128(row, i < stages * 16 ? (k0 + i * 8) * 2 : NOWHERE, 0, 0));
+    }
+  }
+  u32x4 b[T][NS][2];
+#pragma unroll
+  for (int t = 0; t < T; ++t) {
+    const auto rows = __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t*>(w + (int64_t)min(n0 + t * (GATED ? columns : 16), N - 16) * K), 0, 16 * K,
+                                                           0x00020000);
+#pragma unroll
+    for (int s = 0; s < NS; ++s)
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks)
+        b[t][s][ks] = __builtin_amdgcn_raw_buffer_load_b128(rows, s < stages ? col * K + k0 + s * LI_STAGE + ks * 64 + grp * 16 : NOWHERE, 0,
+                                                            ONCE ? 2 : 0);
+  }
+  __builtin_amdgcn_sched_barrier(0);
+  // two rows' maxima side by side
+  uint32_t top[(R + 1) / 2];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    u16x8 m = v[r][0] & (u16x8)(unsigned short)0x7fff;
+#pragma unroll
+    for (int j = 1; j < V; ++j) m = __builtin_elementwise_max(m, v[r][j] & (u16x8)(unsigned short)0x7fff);
+    uint32_t of = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) of = max(of, (uint32_t)m[j]);
+    top[r >> 1] = r & 1 ? top[r >> 1] | of << 16 : of;
+  }
+  typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+#pragma unroll
+  for (int p = 0; p < (R + 1) / 2; ++p) {
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1)
+      top[p] = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, top[p]),
+                                                                     __builtin_bit_cast(u16x2, __shfl_xor(top[p], off))));
+    if (lane == 0) tops[p][wave] = top[p];
+  }
+  // not __syncthreads: what is on its way from memory does not have to have come
+  asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+  // lane r has row r's scale
+  u16x2 most = {};
+#pragma unroll
+  for (int e = 0; e < LF_WAVES; ++e) most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2, tops[min((lane & 7) >> 1, (R + 1) / 2 - 1)][e]));
+  const Int8Row mine(lane & 1 ? most[1] : most[0]);
+  char* codes = smem + wave * (R * ROW);
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    if (r >= M) continue;
+    Int8Row by = mine;
+    by.up = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(mine.up), r));
+    by.most = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(mine.most), r));
+    by.inverse = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(mine.inverse), r));
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const int i = lane + j * 64;
+      if (NS % 4 == 0 || i < NS * 16) *reinterpret_cast<u32x2*>(codes + r * ROW + i * 8) = by.codes(v[r][j]);
+    }
+  }
+  i32x4 acc[T];
+#pragma unroll
+  for (int t = 0; t < T; ++t) acc[t] = i32x4{0, 0, 0, 0};
+  const char* of = codes + min(col, M - 1) * ROW + grp * 16;
+#pragma unroll
+  for (int s = 0; s < NS; ++s)
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks) {
+      const i32x4 c = *reinterpret_cast<const i32x4*>(of + s * LI_STAGE + ks * 64);
+#pragma unroll
+      for (int t = 0; t < T; ++t) acc[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, b[t][s][ks]), c, acc[t], 0, 0, 0);
+    }
+  __syncthreads();                                 // the codes are done with
+#pragma unroll
+  for (int t = 0; t < T; ++t) reinterpret_cast<i32x4*>(smem)[(t * LF_WAVES + wave) * 64 + lane] = acc[t];
+  const float s = __shfl(mine.scale, col & 7);
+  __syncthreads();
+  if (wave > 0 || col >= M) return;
+#pragma unroll
+  for (int t = 0; t < T; ++t)
+#pragma unroll
+    for (int e = 1; e < LF_WAVES; ++e) acc[t] += reinterpret_cast<const i32x4*>(smem)[(t * LF_WAVES + e) * 64 + lane];
+  f32x4 y[T];
+#pragma unroll
+  for (int t = 0; t < T; ++t) {
+    const int n = min(n0 + t * (GATED ? columns : 16), N - 16) + grp * 4;
+    const f32x4 by = *reinterpret_cast<const f32x4*>(ws + n);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) y[t][r] = (float)acc[t][r] * s * by[r];
+    if (FORM == LI_BF16 && bias) {
+      const bf16x4_vec add = *reinterpret_cast<const bf16x4_vec*>((const short*)bias + n);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) y[t][r] += bf16_to_f32(add[r]);
+    }
+  }
+  if constexpr (GATED) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) y[0][r] = y[0][r] / (1.0f + __expf(-y[0][r])) * y[1][r];
+  }
+#pragma unroll
+  for (int t = 0; t < (GATED ? 1 : T); ++t) {
+    const int n = n0 + t * 16 + grp * 4;
+    if (n >= columns) continue;
+    if constexpr (FORM == LI_PART)
+      *reinterpret_cast<f32x4*>((float*)out + (int64_t)col * N + n) = y[t];
+    else
+      *reinterpret_cast<bf16x4_vec*>((short*)out + (int64_t)col * columns + n) = tp_pack(y[t][0], y[t][1], y[t][2], y[t][3]);
+  }
+}
+
+struct Int8Few {
+  int ns, tiles;             // stages of a wave, 0 where a product goes the way of two launches; tiles of 16 rows of W
+};
+
+// Two tiles where one each makes more workgroups than compute units, but no more than twice as many: half as often are the
+// codes made (6144 x 4096, 5 rows: 9.4 us, 10.3 with one; 8 rows 10.6 and 11.9). Deep products of few rows would lose the second
+// workgroup of a compute unit to registers by that (8192 x 8192, 4 rows: 19.3 us, 16.8 with one).
+//
+// Each workgroup makes the codes anew, which costs most where many workgroups meet few weights: rounds * rows * steps of 64
+// vectors are held against the stream of W. Two launches and so, us, on either side of that line: 9728 x 896 gated, 4 rows 7.9 and
+// 7.5, 5 rows 7.8 and 9.1; 16384 x 4096, 5 rows 19.0 and 17.3, 8 rows 18.9 and 20.0. Far from it: 4096 x 4096, 1 row 11.5
+// and 5.8, 8 rows 11.8 and 8.3; 1024 x 4096, 5 rows 9.8 and 6.2; 4096 x 14336, 1 row 19.5 and 14.0.
+static Int8Few int8_few(int M, int N, int K, int form) {
+  if (M > LF_ROWS) return {0, 0};
+  const int stages = (K + LI_STAGE * LF_WAVES - 1) / (LI_STAGE * LF_WAVES), most = form == LI_SILU ? 4 : M <= 4 ? 16 : 8;   // by registers
+  if (stages > most) return {0, 0};
+  const int ns = stages <= 2 ? 2 : stages <= 4 ? 4 : stages <= 8 ? 8 : 16;
+  const int tiles = form == LI_SILU || (N > 16 * LI_UNITS && N <= 32 * LI_UNITS && (ns <= 4 || (ns == 8 && M > 4))) ? 2 : 1;
+  const int64_t rounds = (N / 16 + (int64_t)tiles * LI_UNITS - 1) / ((int64_t)tiles * LI_UNITS);
+  if ((double)(rounds * M * ((ns + 3) / 4)) > 8 + (double)N * K / 4.5e6) return {0, 0};
+  return {ns, tiles};
+}
+
+extern "C" bool linear_int8_few(int M, int N, int K, int form) { return int8_few(M, N, K, form).ns > 0; }
+
+#define LI_ONCE (8 << 20)
+#define LI_ONCE_ALONE ((int64_t)320 << 20)
+
+template <int NS, int R, int T, int FORM>
+static int linear_int8_few_go(void* out, const bf16_t* x, int64_t x_stride, const int8_t* w, const float* ws, const bf16_t* bias, int M, int N,
+                              int K, bool once, hipStream_t stream) {
+  const dim3 grid(FORM == LI_SILU ? N / 32 : (N / 16 + T - 1) / T), block(64 * LF_WAVES);
+  if (once)
+    hipLaunchKernelGGL((linear_int8_few_kernel<NS, R, T, FORM, true>), grid, block, 0, stream, out, x, x_stride, w, ws, bias, M, N, K);
+  else
+    hipLaunchKernelGGL((linear_int8_few_kernel<NS, R, T, FORM, false>), grid, block, 0, stream, out, x, x_stride, w, ws, bias, M, N, K);
+  return 0;
+}
+
+// as launch_linear_int8, of x itself; linear_int8_few says whether it may
+extern "C" int launch_linear_int8_few(void* out, const bf16_t* x, int64_t x_stride, const int8_t* w, const float* ws, const bf16_t* bias, int M,
+                                      int N, int K, int form, bool once, hipStream_t stream) {
+  const int64_t bytes = (int64_t)N * K;
+  once = once ? bytes >= LI_ONCE : bytes >= LI_ONCE_ALONE;
+  const auto [ns, tiles] = int8_few(M, N, K, form);
+#define LF_CASE(NS, R)                                                                                                             \
+  if (ns == NS && M <= R) {                                                                                                        \
+    if constexpr (NS <= 8) {                                                                                                       \
+      if (form == LI_BF16 && tiles == 2) return linear_int8_few_go<NS, R, 2, LI_BF16>(out, x, x_stride, w, ws, bias, M, N, K, once, stream); \
+      if (form == LI_PART && tiles == 2) return linear_int8_few_go<NS, R, 2, LI_PART>(out, x, x_stride, w, ws, bias, M, N, K, once, stream); \
+    }                                                                                                                              \
+    if (form == LI_BF16) return linear_int8_few_go<NS, R, 1, LI_BF16>(out, x, x_stride, w, ws, bias, M, N, K, once, stream);       \
+    if (form == LI_PART) return linear_int8_few_go<NS, R, 1, LI_PART>(out, x, x_stride, w, ws, bias, M, N, K, once, stream);       \
+    if constexpr (NS <= 4) return linear_int8_few_go<NS, R, 2, LI_SILU>(out, x, x_stride, w, ws, bias, M, N, K, once, stream);     \
+  }
+  LF_CASE(2, 1)
+  LF_CASE(2, 4)
+  LF_CASE(2, 8)
+  LF_CASE(4, 1)
+  LF_CASE(4, 4)
+  LF_CASE(4, 6)
+  LF_CASE(4, 8)
+  LF_CASE(8, 1)
+  LF_CASE(8, 4)
+  LF_CASE(8, 8)
+  LF_CASE(16, 1)
+  LF_CASE(16, 4)
+#undef LF_CASE
+  return -1;
 }
 
 // ---- few rows or columns -------------------------------------------------------------------------
@@ -199,7 +418,6 @@ __global__ void __launch_bounds__(TP_THREADS, 1) linear_int8_rows_kernel(
   }
 }
 
-#define LI_UNITS 256       // compute units
 
 // Which kernel a product goes to: ni 2 or 4, tiles of 64 or 128 rows of W by 32 * mj of x, shared out over K; ni 8, tiles of 256
 // by 32 * mj, the last round of them in shares or not.
@@ -263,10 +481,9 @@ static Int8Plan int8_plan(int64_t M, int64_t N, int64_t K, int form) {
   return best;
 }
 
-extern "C" int linear_int8_splits(int M, int N, int K) { return int8_plan(M, N, K, LI_PART).splits; }
-
-#define LI_ONCE (8 << 20)
-#define LI_ONCE_ALONE ((int64_t)320 << 20)
+extern "C" int linear_int8_splits(int M, int N, int K) {
+  return linear_int8_few(M, N, K, LI_PART) ? 1 : int8_plan(M, N, K, LI_PART).splits;
+}
 
 template <int NI, int MJ, int FORM, bool ONCE>
 static int linear_int8_rows_go(const Int8Plan& p, void* out, const int8_t* x, const float* xs, const int8_t* w, const float* ws,

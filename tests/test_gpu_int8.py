@@ -105,6 +105,51 @@ def test_sums_in_shares(M, N, K):
     assert bool(((part.double().sum(0).cpu() - y).abs() <= 2 ** -22 * size + 1e-30).all())
 
 
+@pytest.mark.parametrize("M", [1, 2, 3, 4, 5, 6, 7, 8, 9])
+@pytest.mark.parametrize("N,K", [(32, 16), (64, 144), (4096, 1040), (4128, 2064), (8224, 4112), (544, 8208), (256, 16384), (128, 16400)])
+def test_few_rows(M, N, K):
+    """Codes made on the way: stages that end inside K, waves without a stage, an odd number of tiles, all forms."""
+    x, (w, ws) = rows(M, K, seed=M + K), weights(N, K, seed=N)
+    bias = torch.randn(N, generator=torch.Generator().manual_seed(2)).bfloat16()
+    if M > 2:
+        x[1] = 0
+    args = [t.to(DEV) for t in (x, w, ws)]
+    check(ops.linear_int8(*args), x, w, ws)
+    check(ops.linear_int8(*args, bias.to(DEV), once=True), x, w, ws, bias)
+    small = ws * (0.05 * 64 / K ** 0.5)
+    check(ops.linear_silu_int8(args[0], args[1], small.to(DEV)), x, w, small, gated=True)
+    part = ops.linear_part_int8(*args)
+    # each share's exact sum is rounded by 2^-24 as it becomes fp32 and at both scales, 3 * 2^-24 < 2^-22 of its own size; the
+    # shares' sizes add up to no more than the products' do, and may cancel
+    xc, xs = torch_ref.quantize_rows(x)
+    y = (xc.double() @ w.double().t()) * xs.double()[:, None] * ws.double()
+    size = (xc.double().abs() @ w.double().abs().t()) * xs.double()[:, None] * ws.double()
+    assert bool(((part.double().sum(0).cpu() - y).abs() <= 2 ** -22 * size + 1e-30).all())
+
+
+@pytest.mark.parametrize("M", [1, 8])
+def test_few_rows_the_last_of_memory(M):
+    """Rows of x and W that end where their storage does, and rows of x far apart."""
+    N, K = 48, 1040
+    x, (w, ws) = rows(M, K, seed=9), weights(N, K, seed=4)
+    apart = torch.full((M, 1 << 21), float("nan"), dtype=torch.bfloat16, device=DEV)
+    apart[:, -K:] = x.to(DEV)
+    want = ops.linear_int8(x.to(DEV), w.to(DEV), ws.to(DEV))
+    check(want, x, w, ws)
+    assert torch.equal(ops.linear_int8(apart[:, -K:], w.to(DEV), ws.to(DEV)), want)
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
+@pytest.mark.parametrize("at", [0, 1023, 4095])
+def test_few_rows_that_are_no_numbers(bad, at):
+    x, (w, ws) = rows(5, 4096, seed=6), weights(6144, 4096)
+    x[2, at] = bad
+    got = ops.linear_int8(x.to(DEV), w.to(DEV), ws.to(DEV)).cpu()
+    assert bool(torch.isnan(got[2]).all())
+    keep = [0, 1, 3, 4]
+    check(got[keep], x[keep], w, ws)
+
+
 def test_rows_that_are_no_numbers_are_their_own_alone():
     x, (w, ws) = rows(6, 256), weights(64, 256)
     x[1, 3], x[4, 200] = float("nan"), float("inf")
