@@ -121,7 +121,7 @@ static void store_kv4(torch::Tensor k, torch::Tensor v, torch::Tensor k_cache, t
   TORCH_CHECK(k.size(2) == 128 && v.sizes() == k.sizes() && v.device() == k.device() && k_cache.size(1) == G, "store_kv: rows [T, kv heads, 128]");
   TORCH_CHECK(slots.scalar_type() == at::kLong && slots.dim() == 1 && slots.numel() == T && slots.is_contiguous() &&
                   slots.device() == k.device(), "store_kv: a slot for each row, int64");
-  TORCH_CHECK(T < (1LL << 31), "store_kv: rows exceed 32-bit indexing");
+  TORCH_CHECK(T * 2 * G < (1LL << 32), "store_kv: rows exceed 32-bit indexing");
   if (T == 0 || k_cache.numel() == 0) return;
   const c10::DeviceGuard device(k.device());
   if (!rows_aligned(k)) k = k.clone(at::MemoryFormat::Contiguous);
@@ -139,7 +139,7 @@ std::tuple<torch::Tensor, torch::Tensor> load_kv4(torch::Tensor k_cache, torch::
   TORCH_CHECK(slots.scalar_type() == at::kLong && slots.dim() == 1 && slots.is_contiguous() && slots.device() == k_cache.device(),
               "load_kv: slots int64 [T]");
   const int64_t T = slots.numel(), G = k_cache.size(1);
-  TORCH_CHECK(T < (1LL << 31), "load_kv: rows exceed 32-bit indexing");
+  TORCH_CHECK(T * 2 * G < (1LL << 32), "load_kv: rows exceed 32-bit indexing");
   const c10::DeviceGuard device(k_cache.device());
   auto k = torch::empty({T, G, 128}, k_scale.options()), v = torch::empty_like(k);
   if (k.numel() == 0) return {k, v};

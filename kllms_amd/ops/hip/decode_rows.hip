@@ -191,7 +191,7 @@ __global__ void __launch_bounds__(256) rope_store_rows_kernel(
     const float x = bf16_to_f32(lo), y = bf16_to_f32(hi);
     const Kv4Group ga(-wave_reduce_max(-x), wave_reduce_max(x), __ballot(x != x) == 0);
     const Kv4Group gb(-wave_reduce_max(-y), wave_reduce_max(y), __ballot(y != y) == 0);
-    uint32_t w = (ga.code(x) | gb.code(y) << 8) << (4 * ((lane >> 5) + 4 * (lane >> 4 & 1)));
+    uint32_t w = kv4_pair(ga, gb, x, y) << (4 * ((lane >> 5) + 4 * (lane >> 4 & 1)));
     w |= __shfl_xor(w, 16);
     w |= __shfl_xor(w, 32);
     if (lane < 16) ((uint32_t*)(is_k ? k_cache : v_cache))[row * (KV4_BYTES / 4) + lane] = w;
