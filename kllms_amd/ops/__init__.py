@@ -261,7 +261,11 @@ class Kv4Groups(NamedTuple):
     parts: int
 
 
-KV4_GROUP_ROWS = 8           # segments shorter than this attend row by row
+# Segments of fewer rows attend row by row, and all of them where rows * keys * kv heads are fewer than that. us together and
+# row by row, 32 / 8 heads: 8 rows each of 4 segments behind 4000 keys 31 and 31, 12 rows 31 and 47; of 12 behind 2000 8 rows 42 and
+# 37, 12 rows 42 and 56. 24 rows each of 4 behind 500 (400 000) 19 and 19, 16 rows (270 000) 18 and 15; 32 rows behind 500
+# (140 000) 19 and 13
+KV4_GROUP_ROWS, KV4_FEW = 10, 300_000
 _KV4_UNITS = 256
 # us of an item and of each of its keys, of a second launch and of each partial's way through memory. One segment, 32 / 8 heads:
 # 2048 rows behind 256 / 4096 / 8192 (248 items) 90, 213, 348; 146 behind 1536 in items of 256 / 512 / all keys 33, 32, 61
@@ -287,12 +291,12 @@ def _kv4_cuts(keys, kv_heads: int) -> int:
     return best
 
 
-def kv4_plan(segs, heads: int, kv_heads: int, device) -> tuple:
-    """paged_plan of the 4-bit cache."""
+def kv4_plan(segs, heads: int, kv_heads: int, device, least: int = 1) -> tuple:
+    """paged_plan of the 4-bit cache: segments of ``least`` rows and more attend together."""
     rows = 256 // (heads // kv_heads)
     groups, short, row = [], [], 0
     for i, (start, n) in enumerate(segs):
-        if n >= KV4_GROUP_ROWS:
+        if n >= max(least, 1):
             groups.extend((row, n, r, i, start + min(n, r + rows)) for r in range(0, n, rows))
         elif n and short and short[-1][0] + short[-1][1] == row:
             short[-1] = (short[-1][0], short[-1][1] + n)
@@ -322,7 +326,8 @@ def paged_plan(segs, heads: int, kv_heads: int, device, cache_dtype=torch.bfloat
     """What attn_segments_paged takes of segments [(start position, rows)]: (groups of rows that attend together, or None,
     [(first row, rows)] of those that attend row by row). Made once for all layers of a pass."""
     if cache_dtype == torch.uint8 and heads // kv_heads in (1, 2, 4, 8) and heads % kv_heads == 0:
-        return kv4_plan(segs, heads, kv_heads, device)
+        few = kv_heads * sum(n * (start + n) for start, n in segs) < KV4_FEW
+        return kv4_plan(segs, heads, kv_heads, device, 1 << 31 if few else KV4_GROUP_ROWS)
     if cache_dtype == torch.bfloat16 and paged_prefill_pays(segs, kv_heads):
         return paged_prefill_plan(segs, device, 64 if paged_prefill_few(segs, heads) else 256)
     rows = sum(n for _, n in segs)

@@ -12,9 +12,8 @@
 typedef __bf16 bf16x8_kv4 __attribute__((ext_vector_type(8)));
 typedef float f32x8_kv4 __attribute__((ext_vector_type(8)));
 
-// Row of a position in [NB, G, block]. A division of 64 bits takes a hundred instructions, one of 32 a fifth.
+// Row of a position in [NB, G, block]; a cache has fewer than 2^31, and a division of 32 bits is a fifth of one of 64
 __device__ __forceinline__ int64_t kv4_row_of(int64_t slot, int G, int g, int block_size) {
-  if ((uint64_t)slot >> 32) return (slot / block_size * G + g) * block_size + slot % block_size;
   const uint32_t block = (uint32_t)slot / (uint32_t)block_size;
   return ((int64_t)block * G + g) * block_size + (uint32_t)slot % (uint32_t)block_size;
 }

@@ -305,7 +305,7 @@ def segments(segs, gqa, KVH, BS, seed=0, spread=0.0):
 
 
 def attend(q, kc, vc, ks, vs, seg_tables, start, tables, lens, scale, segs, plan=None):
-    plan, short = plan or ops.paged_plan(segs, q.shape[1], kc.shape[1], DEV, kc.dtype)
+    plan, short = plan or ops.kv4_plan(segs, q.shape[1], kc.shape[1], DEV)
     return ops.attn_segments_paged(*(t.to(DEV) for t in (q, kc, vc, tables, lens)), scale, plan, short, seg_tables.to(DEV),
                                    start.to(DEV), ks.to(DEV), vs.to(DEV))
 
@@ -328,9 +328,26 @@ def test_segments_whose_keys_are_cut(gqa, KVH):
     segs = [(2500, 40), (700, 9), (3000, 8)]
     args = segments(segs, gqa, KVH, 16, seed=3)
     q, kc, vc, ks, vs, seg_tables, start, tables, lens = args
-    plan, _ = ops.paged_plan(segs, gqa * KVH, KVH, DEV, kc.dtype)
+    plan, _ = ops.kv4_plan(segs, gqa * KVH, KVH, DEV)
     assert plan.parts > 0
     check([attend(*args, 0.1, segs)], q, kc, vc, ks, vs, tables, lens, 0.1)
+
+
+@pytest.mark.parametrize("segs,least", [([(0, 1), (64, 1), (300, 2), (7, 5)], 1), ([(40, 30), (9, 9), (0, 12), (3, 2)], 10),
+                                        ([(40, 30), (9, 9)], 100)])
+def test_segments_together_and_row_by_row(segs, least):
+    args = segments(segs, 4, 2, 16, seed=12)
+    q, kc, vc, ks, vs, seg_tables, start, tables, lens = args
+    plan, short = ops.kv4_plan(segs, 8, 2, DEV, least)
+    alone = sum(n for _, n in segs if n < least)
+    assert sum(n for _, n in short) == alone and (plan is None) == (alone == len(q))
+    check([attend(*args, 0.1, segs, (plan, short))], q, kc, vc, ks, vs, tables, lens, 0.1)
+
+
+def test_plan_goes_row_by_row_where_there_is_little():
+    assert ops.paged_plan([(500, 32)], 32, 8, DEV, torch.uint8) == (None, [(0, 32)])
+    plan, short = ops.paged_plan([(4000, 16), (4000, 9), (4000, 40)], 32, 8, DEV, torch.uint8)
+    assert plan is not None and short == [(16, 9)]
 
 
 @pytest.mark.parametrize("spread", [3.0, 20.0])
@@ -378,7 +395,7 @@ def test_segments_in_strided_rows_and_empty():
     rest = (kc, vc, ks, vs, seg_tables, start, tables, lens, 0.1, segs)
     want = attend(q, *rest)
     wide = torch.cat((q, q), 1)
-    plan = ops.paged_plan(segs, 8, 2, DEV, kc.dtype)
+    plan = ops.kv4_plan(segs, 8, 2, DEV)
     got = ops.attn_segments_paged(wide.to(DEV)[:, 8:], kc.to(DEV), vc.to(DEV), tables.to(DEV), lens.to(DEV), 0.1, *plan,
                                   seg_tables.to(DEV), start.to(DEV), ks.to(DEV), vs.to(DEV))
     assert torch.equal(got, want)
@@ -389,7 +406,7 @@ def test_segments_replayed():
     segs = [(900, 70), (100, 30)]
     args = [t.to(DEV) for t in segments(segs, 4, 2, 16, seed=9)]
     q = args[0]
-    plan = ops.paged_plan(segs, 8, 2, DEV, torch.uint8)
+    plan = ops.kv4_plan(segs, 8, 2, DEV)
     step = lambda: attend(*args, 0.1, segs, plan)
     step()
     g = torch.cuda.CUDAGraph()
