@@ -255,10 +255,14 @@ def paged_prefill_plan(segs, device, rows: int = 256) -> tuple:
 class Kv4Groups(NamedTuple):
     """Groups of a segment's rows that attend over the 4-bit cache together: ``items`` int32 [n, 8] (first packed row and rows of
     the segment, first row of the group, segment, first and last key, where its sums go, 0) and ``cuts`` [m, 4] (first packed
-    row, rows, first part, parts) of groups whose keys are cut into ``parts`` altogether."""
+    row, rows, first part, parts) of groups whose keys are cut into ``parts`` altogether; of ``rows`` packed rows in ``segments``
+    segments, with ``heads`` heads to a kv head."""
     items: torch.Tensor
     cuts: torch.Tensor
     parts: int
+    rows: int
+    segments: int
+    heads: int
 
 
 # Segments of fewer rows attend row by row, and all of them where rows * keys * kv heads are fewer than that. us together and
@@ -319,7 +323,8 @@ def kv4_plan(segs, heads: int, kv_heads: int, device, least: int = 1) -> tuple:
         parts += pieces
     items.sort(key=lambda g: g[4] - g[5])                # longest first
     flat = upload(torch.tensor([x for g in items for x in g] + [x for c in cuts for x in c], dtype=torch.int32), device)
-    return Kv4Groups(flat[:8 * len(items)].view(-1, 8), flat[8 * len(items):].view(-1, 4), parts), short
+    return Kv4Groups(flat[:8 * len(items)].view(-1, 8), flat[8 * len(items):].view(-1, 4), parts, sum(n for _, n in segs), len(segs),
+                     heads // kv_heads), short
 
 
 def paged_plan(segs, heads: int, kv_heads: int, device, cache_dtype=torch.bfloat16) -> tuple:
@@ -340,6 +345,10 @@ def attn_segments_paged(q, k_cache, v_cache, block_tables, context_lens, scale, 
     ``plan`` and ``short``: of paged_plan for this cache's type. A 4-bit value row that is no number makes the rows that
     attend together and see it none as a whole."""
     _check_kv4(k_cache, k_scale, v_scale)
+    if k_cache.dtype == torch.uint8 and plan is not None and (
+            q.shape[0] < plan.rows or seg_tables.shape[0] < plan.segments or q.shape[1] != plan.heads * k_cache.shape[1]):
+        raise ValueError(f"a plan of {plan.rows} rows in {plan.segments} segments with {plan.heads} heads to a kv head: got q {list(q.shape)}, "
+                         f"tables {list(seg_tables.shape)}, {k_cache.shape[1]} kv heads")
     out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     if k_cache.dtype == torch.uint8:
         if plan is not None:

@@ -652,8 +652,9 @@ torch::Tensor linear_int8(torch::Tensor x, torch::Tensor w, torch::Tensor w_scal
   if (M == 0) return out;
   x = int8_readable(x);
   if (linear_int8_few((int)std::min<int64_t>(M, 1 << 20), (int)N, (int)K, (int)form)) {
-    launch_linear_int8_few(out.data_ptr(), cbf(x), x.stride(0), w.data_ptr<int8_t>(), w_scale.data_ptr<float>(), bias ? cbf(*bias) : nullptr,
-                           (int)M, (int)N, (int)K, (int)form, once, cur_stream());
+    TORCH_CHECK(launch_linear_int8_few(out.data_ptr(), cbf(x), x.stride(0), w.data_ptr<int8_t>(), w_scale.data_ptr<float>(),
+                                       bias ? cbf(*bias) : nullptr, (int)M, (int)N, (int)K, (int)form, once, cur_stream()) == 0,
+                "linear_int8: a form of few rows that is not there");
     return out;
   }
   int zeros = 0;

@@ -175,3 +175,17 @@ def test_a_copied_block_takes_its_scales_along():
 def test_models_with_states_are_refused():
     with pytest.raises(ValueError, match="int4"):
         engine(model="tiny-zutalix")
+
+
+def test_a_plan_of_other_rows_is_refused():
+    segs = [(40, 20), (0, 12)]
+    plan, short = ops.kv4_plan(segs, 8, 2, "cpu")
+    assert (plan.rows, plan.segments, plan.heads) == (32, 2, 4)
+    q, cache = torch.zeros(32, 8, 128, dtype=torch.bfloat16), torch.zeros(4, 2, 16, 64, dtype=torch.uint8)
+    scales, tables, start = torch.zeros(4, 2, 16, 2, 2, dtype=torch.bfloat16), torch.zeros(2, 4, dtype=torch.int32), torch.zeros(2, dtype=torch.int32)
+    lens = torch.zeros(32, dtype=torch.int32)
+    for bad in (dict(q=q[:31]), dict(seg_tables=tables[:1]), dict(q=torch.zeros(32, 4, 128, dtype=torch.bfloat16))):
+        args = {**dict(q=q, k_cache=cache, v_cache=cache, block_tables=tables, context_lens=lens, scale=0.1, plan=plan, short=short, seg_tables=tables,
+                       seg_start=start, k_scale=scales, v_scale=scales), **bad}
+        with pytest.raises(ValueError, match="a plan of 32 rows in 2 segments"):
+            ops.attn_segments_paged(**args)
