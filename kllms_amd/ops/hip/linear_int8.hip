@@ -274,21 +274,24 @@ struct Int8Few {
 };
 
 // Two tiles where one each makes more workgroups than compute units, but no more than twice as many: half as often are the
-// codes made (6144 x 4096, 5 rows: 9.4 us, 10.3 with one; 8 rows 10.6 and 11.9). Deep products of few rows would lose the second
-// workgroup of a compute unit to registers by that (8192 x 8192, 4 rows: 19.3 us, 16.8 with one).
+// codes made (6144 x 4096, 5 rows: 9.4 us, 10.3 with one; 8 rows 10.6 and 11.9). Deeper products have no registers for that.
 //
-// Each workgroup makes the codes anew, which costs most where many workgroups meet few weights: rounds * rows * steps of 64
-// vectors are held against the stream of W. Two launches and so, us, on either side of that line: 9728 x 896 gated, 4 rows 7.9 and
-// 7.5, 5 rows 7.8 and 9.1; 16384 x 4096, 5 rows 19.0 and 17.3, 8 rows 18.9 and 20.0. Far from it: 4096 x 4096, 1 row 11.5
-// and 5.8, 8 rows 11.8 and 8.3; 1024 x 4096, 5 rows 9.8 and 6.2; 4096 x 14336, 1 row 19.5 and 14.0.
+// Each workgroup makes the codes anew. In one round of workgroups that is hidden for long; in more the way of two launches, which
+// streams W a little faster, catches up. us of two launches and so:
+//   one round   4096 x 4096   1 row 11.4, 5.9   8 rows 11.6, 8.3     1024 x 4096   1 row 9.7, 4.7   8 rows 9.8, 7.4     1152 x 896   5 rows 7.2, 5.6
+//               4096 x 14336  1 row 19.0, 14.0   4 rows 19.7, 18.1     896 x 4864   6 rows 10.1, 9.7   8 rows 10.2, 10.4
+//   two         9728 x 896 gated   4 rows 8.0, 7.5   5 rows 7.9, 9.1     8192 x 8192   4 rows 19.2, 16.7   5 rows 19.5, 20.8
+//   four        16384 x 4096   4 rows 17.3, 16.3   6 rows 17.5, 18.0     28672 x 4096 gated   1 row 26.4, 25.1   5 rows 26.3, 27.9
+//               13824 x 5120   1 row 18.8, 17.1   2 rows 18.8, 20.2
+//   eight       32768 x 4096   3 rows 27.6, 26.8   5 rows 27.6, 30.6
 static Int8Few int8_few(int M, int N, int K, int form) {
   if (M > LF_ROWS) return {0, 0};
   const int stages = (K + LI_STAGE * LF_WAVES - 1) / (LI_STAGE * LF_WAVES), most = form == LI_SILU ? 4 : M <= 4 ? 16 : 8;   // by registers
   if (stages > most) return {0, 0};
-  const int ns = stages <= 2 ? 2 : stages <= 4 ? 4 : stages <= 8 ? 8 : 16;
-  const int tiles = form == LI_SILU || (N > 16 * LI_UNITS && N <= 32 * LI_UNITS && (ns <= 4 || (ns == 8 && M > 4))) ? 2 : 1;
+  const int ns = stages <= 2 ? 2 : stages <= 4 ? 4 : stages <= 8 ? 8 : 16, steps = (ns + 3) / 4;
+  const int tiles = form == LI_SILU || (N > 16 * LI_UNITS && N <= 32 * LI_UNITS && ns <= 4) ? 2 : 1;
   const int64_t rounds = (N / 16 + (int64_t)tiles * LI_UNITS - 1) / ((int64_t)tiles * LI_UNITS);
-  if ((double)(rounds * M * ((ns + 3) / 4)) > 8 + (double)N * K / 4.5e6) return {0, 0};
+  if (rounds == 1 ? M * steps > 16 : M > 4 || rounds * steps * steps > 8) return {0, 0};
   return {ns, tiles};
 }
 
@@ -316,7 +319,7 @@ extern "C" int launch_linear_int8_few(void* out, const bf16_t* x, int64_t x_stri
   const auto [ns, tiles] = int8_few(M, N, K, form);
 #define LF_CASE(NS, R)                                                                                                             \
   if (ns == NS && M <= R) {                                                                                                        \
-    if constexpr (NS <= 8) {                                                                                                       \
+    if constexpr (NS <= 4) {                                                                                                       \
       if (form == LI_BF16 && tiles == 2) return linear_int8_few_go<NS, R, 2, LI_BF16>(out, x, x_stride, w, ws, bias, M, N, K, once, stream); \
       if (form == LI_PART && tiles == 2) return linear_int8_few_go<NS, R, 2, LI_PART>(out, x, x_stride, w, ws, bias, M, N, K, once, stream); \
     }                                                                                                                              \
