@@ -201,6 +201,7 @@ def test_weights_of_more_than_2_gb():
         check(got[:, -16:], x[:M], part, ws[-16:].cpu())
 
 
+@torch.inference_mode()                  # as the engine captures: torch's own state is of one kind for all captures
 def test_replayed():
     x, (w, ws) = rows(5, 4096), weights(6144, 4096)
     long, (w2, ws2) = rows(333, 3584), weights(4608, 3584)

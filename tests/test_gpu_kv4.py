@@ -245,6 +245,7 @@ def test_caches_of_more_than_2_gb():
     assert torch.equal(a, b) and torch.equal(a.cpu(), torch_ref.kv4_values(*torch_ref.kv4_quantize(new.cpu())).bfloat16())
 
 
+@torch.inference_mode()                  # as the engine captures: torch's own state is of one kind for all captures
 def test_replayed_and_on_another_stream():
     """Captured with the store, replayed with other work between; two graphs of one cache."""
     q, kc, vc, ks, vs, tables, n = (t.to(DEV) for t in case([700, 20], 4, 2, 16, seed=16))
@@ -402,6 +403,7 @@ def test_segments_in_strided_rows_and_empty():
     assert ops.paged_plan([], 8, 2, DEV, kc.dtype) == (None, []) and ops.paged_plan([(5, 0)], 8, 2, DEV, kc.dtype) == (None, [])
 
 
+@torch.inference_mode()                  # as the engine captures: torch's own state is of one kind for all captures
 def test_segments_replayed():
     segs = [(900, 70), (100, 30)]
     args = [t.to(DEV) for t in segments(segs, 4, 2, 16, seed=9)]
