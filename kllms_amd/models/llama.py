@@ -128,11 +128,17 @@ class LlamaMLP(nn.Module):
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         return self.down_proj(self.activate(x))
 
-    def activate(self, x: torch.Tensor) -> torch.Tensor:
-        """silu(gate) * up."""
+    def takes_codes(self):
+        """The projection that activate multiplies Int8Rows with, None where it takes rows."""
+        p = self.gate_up_proj
+        return p if (p.weight.dtype == torch.int8 and p.bias is None and ops.only_weights(p, ColumnParallelLinear)
+                     and ops.no_global_hooks()) else None
+
+    def activate(self, x) -> torch.Tensor:
+        """silu(gate) * up of rows, or of Int8Rows where takes_codes."""
         p = self.gate_up_proj
         plain = ops.only_weights(p, ColumnParallelLinear) and ops.no_global_hooks()
-        if plain and p.bias is None and p.weight.dtype == torch.int8:
+        if plain and p.bias is None and p.weight.dtype == torch.int8:      # takes Int8Rows too
             return ops.linear_silu_int8(x, p.weight, p.weight_scale, p.once)
         act = ops.linear_silu(x, p.weight) if plain and p.bias is None else None
         if act is not None:
@@ -373,8 +379,16 @@ class LlamaForCausalLM(nn.Module):
             m.quantize_(self._once)
 
     @staticmethod
-    def _sums(x: torch.Tensor, p, once: bool) -> torch.Tensor:
-        """fp32 sums [S, M, N] of a few rows with a projection's weights."""
+    def _normed(part: torch.Tensor, residual: torch.Tensor, norm, p, form: int):
+        """residual += part and its norm, as the projection p reads it: as Int8Rows where it would quantize them in a launch
+        of its own. p None: rows."""
+        if p is not None and p.weight.dtype == torch.int8 and not ops.int8_makes_codes(residual.shape[0], p.weight, form):
+            return ops.add_norm_rows_int8(part, residual, norm.weight, norm.eps)
+        return ops.add_norm_rows(part, residual, norm.weight, norm.eps)
+
+    @staticmethod
+    def _sums(x, p, once: bool) -> torch.Tensor:
+        """fp32 sums [S, M, N] of a few rows (or Int8Rows) with a projection's weights."""
         if p.weight.dtype == torch.int8:
             return ops.linear_part_int8(x, p.weight, p.weight_scale, once)
         return ops.linear_part(x, p.weight, once)
@@ -420,14 +434,15 @@ class LlamaForCausalLM(nn.Module):
                 q = ops.rope_store_rows(self._sums(x, at.qkv_proj, once), at.qkv_proj.bias, at.num_heads,
                                         batch.positions, self.cos_sin, k_cache, v_cache, batch.slot_mapping, k_scale, v_scale)
                 att = at.attend_cache(q, batch, arrived)
-            x = ops.add_norm_rows(self._sums(att.view(T, -1), at.o_proj, once), residual, norm.weight, norm.eps)
-            norm = layers[i + 1].input_layernorm if i + 1 < len(layers) else self.norm
             mlp = layer.mlp
+            x = self._normed(self._sums(att.view(T, -1), at.o_proj, once), residual, norm, mlp.takes_codes() if isinstance(mlp, LlamaMLP) else None, 1)
+            norm = layers[i + 1].input_layernorm if i + 1 < len(layers) else self.norm
             if isinstance(mlp, LlamaMLP):
                 w = mlp.gate_up_proj.weight
                 act = (ops.linear_silu_rows(x, w, once) if w.dtype == torch.bfloat16 and (self._silu_rows(T, w) or self._silu_streams(T, w))
                        else mlp.activate(x))
-                x = ops.add_norm_rows(self._sums(act, mlp.down_proj, once), residual, norm.weight, norm.eps)
+                follows = layers[i + 1].self_attn.qkv_proj if i + 1 < len(layers) and batch.mode == "decode" else None
+                x = self._normed(self._sums(act, mlp.down_proj, once), residual, norm, follows, 2)
             else:
                 x, residual = ops.fused_add_rmsnorm(mlp(x), residual, norm.weight, norm.eps)
         return x

@@ -546,21 +546,45 @@ def linear_clamped_glu(x: torch.Tensor, w: torch.Tensor, limit: float, alpha: fl
 
 # --- products in 8-bit integers -----------------------------------------------------
 
-def _check_int8(x: torch.Tensor, w: torch.Tensor) -> None:
+class Int8Rows(NamedTuple):
+    """Rows in 8-bit integers: ``codes`` int8 [M, K], ``scales`` fp32 [M]. The products take them in place of the rows and give
+    what the rows would have given, in bf16."""
+    codes: torch.Tensor
+    scales: torch.Tensor
+
+
+def _check_int8(x, w: torch.Tensor) -> None:
+    if isinstance(x, Int8Rows):
+        x, scales = x
+        if x.dtype != torch.int8 or scales.dtype != torch.float32 or scales.shape != x.shape[:1]:
+            raise ValueError(f"rows as int8 codes with an fp32 scale each: got {x.dtype} {list(x.shape)}, {scales.dtype} {list(scales.shape)}")
     if w.dtype != torch.int8 or w.dim() != 2 or x.dim() != 2 or x.shape[1] != w.shape[1]:
         raise ValueError(f"x [M, K] with int8 weights [N, K]: got {list(x.shape)} with {w.dtype} {list(w.shape)}")
     if x.requires_grad and torch.is_grad_enabled():
         raise RuntimeError("products in 8-bit integers have no gradient: call them under torch.no_grad()")
 
 
-def quantize_rows(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+def _product_int8(x, w, w_scale, bias, form: int, once: bool) -> torch.Tensor:
+    if isinstance(x, Int8Rows):
+        return _hip_or_raise().linear_int8_codes(x.codes, x.scales, w, w_scale, bias, form, once)
+    return _hip_or_raise().linear_int8(x, w, w_scale, bias, form, once)
+
+
+def int8_makes_codes(rows: int, w: torch.Tensor, form: int) -> bool:
+    """Whether a product of so many rows with w [N, K] on the GPU (form 0: linear_int8, 1: linear_silu_int8, 2: linear_part_int8)
+    makes the codes of its rows on the way: then it takes the rows themselves faster than Int8Rows."""
+    return _hip_or_raise().linear_int8_few(rows, w.shape[0], w.shape[1], form)
+
+
+def quantize_rows(x: torch.Tensor) -> Int8Rows:
     """(codes int8 [M, K], scales fp32 [M]) of rows: x / scale to the nearest whole number, scale = max |x| / 127 of the
-    row. A row with a value that is no finite number has the scale NaN. On the GPU x is bf16, K a multiple of 16."""
+    row. A row with a value that is no finite number has the scale NaN. On the GPU x is bf16, K a multiple of 16. For rows that
+    several products read; one product quantizes its rows itself."""
     if x.dim() != 2:
         raise ValueError(f"rows [M, K]: got {list(x.shape)}")
     if x.is_cuda and not _force_torch():
-        return _hip_or_raise().quantize_rows(x)
-    return torch_ref.quantize_rows(x)
+        return Int8Rows(*_hip_or_raise().quantize_rows(x))
+    return Int8Rows(*torch_ref.quantize_rows(x))
 
 
 def quantize_weights(w: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -573,12 +597,12 @@ def quantize_weights(w: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
 
 def linear_int8(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, bias: Optional[torch.Tensor] = None,
                 once: bool = False) -> torch.Tensor:
-    """x @ w^T (+ bias) in 8-bit integers, in x's dtype: x [M, K] quantized row by row (quantize_rows), w int8 [N, K] with a
-    scale for each row (quantize_weights), exact 32-bit sums. On the GPU x is bf16, K a multiple of 16 up to 131072, N one of 16.
-    ``once``: weights_once of the caller's model."""
+    """x @ w^T (+ bias) in 8-bit integers, in x's dtype: x [M, K] quantized row by row (quantize_rows), or Int8Rows; w int8
+    [N, K] with a scale for each row (quantize_weights), exact 32-bit sums. On the GPU x is bf16, K a multiple of 16 up to
+    131072, N one of 16. ``once``: weights_once of the caller's model."""
     _check_int8(x, w)
-    if x.is_cuda and not _force_torch():
-        return _hip_or_raise().linear_int8(x, w, w_scale, bias, 0, once)
+    if (x.codes if isinstance(x, Int8Rows) else x).is_cuda and not _force_torch():
+        return _product_int8(x, w, w_scale, bias, 0, once)
     return torch_ref.linear_int8(x, w, w_scale, bias)
 
 
@@ -587,14 +611,14 @@ def linear_silu_int8(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, on
     _check_int8(x, w)
     if w.shape[0] % 2:
         raise ValueError("gate and up have the same rows")
-    if x.is_cuda and not _force_torch():
-        return _hip_or_raise().linear_int8(x, w, w_scale, None, 1, once)
+    if (x.codes if isinstance(x, Int8Rows) else x).is_cuda and not _force_torch():
+        return _product_int8(x, w, w_scale, None, 1, once)
     return torch_ref.linear_silu_int8(x, w, w_scale)
 
 
 def linear_part_int8(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, once: bool = False) -> torch.Tensor:
     """linear_int8 of up to LINEAR_ROWS_MAX rows as fp32 sums [S, M, N] over S shares of K, like linear_part (GPU only)."""
-    return _hip_or_raise().linear_int8(x, w, w_scale, None, 2, once)
+    return _product_int8(x, w, w_scale, None, 2, once)
 
 
 def embed_norm_rows(ids, table, weight, eps, unknown=None, clear=None):
@@ -607,6 +631,11 @@ def embed_norm_rows(ids, table, weight, eps, unknown=None, clear=None):
 def add_norm_rows(part, residual, weight, eps):
     """residual += the sums of ``part`` (in place); returns rms(residual) * weight."""
     return _hip_or_raise().add_norm_rows(part, residual, weight, eps)
+
+
+def add_norm_rows_int8(part, residual, weight, eps) -> Int8Rows:
+    """quantize_rows(add_norm_rows(...)) in one launch, for rows of a multiple of 128 (GPU only)."""
+    return Int8Rows(*_hip_or_raise().add_norm_rows_int8(part, residual, weight, eps))
 
 
 def rope_store_rows(part, bias, num_heads, positions, cos_sin, k_cache, v_cache, slot_mapping, k_scale=None, v_scale=None):

@@ -595,10 +595,14 @@ extern "C" int launch_linear_int8_few(void* out, const bf16_t* x, int64_t x_stri
 
 static bool on_16_bytes_at(const torch::Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0; }
 
+static void check_int8_sizes(int64_t M, int64_t K, const char* who) {
+  TORCH_CHECK(K % 16 == 0 && K >= 16 && K <= 131072 && M < (1LL << 30),
+              who, ": K is a multiple of 16, up to 131072 (a sum of more products does not fit 32 bits)");
+}
+
 static void check_int8_rows(const torch::Tensor& x, const char* who) {
   TORCH_CHECK(x.is_cuda() && x.scalar_type() == at::kBFloat16 && x.dim() == 2, who, ": rows are bf16 [M, K] on the GPU");
-  TORCH_CHECK(x.size(1) % 16 == 0 && x.size(1) >= 16 && x.size(1) <= 131072 && x.size(0) < (1LL << 30),
-              who, ": K is a multiple of 16, up to 131072 (a sum of more products does not fit 32 bits)");
+  check_int8_sizes(x.size(0), x.size(1), who);
 }
 
 // rows that 16-byte loads can read
@@ -630,13 +634,10 @@ static void check_int8_weights(const torch::Tensor& w, const torch::Tensor& w_sc
                   w_scale.device() == like.device() && on_16_bytes_at(w_scale), "linear_int8: a contiguous fp32 scale for each row of the weights");
 }
 
-// form 0: x [M, K] w^T (+ bias) in bf16, 1: silu(gate) * up of a fused [gate; up], 2: fp32 sums [S, M, N] of up to 128 rows.
-// once: the weights of the caller's step do not stay in the caches until its next
-torch::Tensor linear_int8(torch::Tensor x, torch::Tensor w, torch::Tensor w_scale, std::optional<torch::Tensor> bias, int64_t form,
-                          bool once) {
-  check_int8_rows(x, "linear_int8");
+// The result of a product of M rows (fp32 shares of form 2), its operands checked; a bias off 8 bytes is copied
+static torch::Tensor int8_result(const torch::Tensor& x, const torch::Tensor& w, const torch::Tensor& w_scale, std::optional<torch::Tensor>& bias,
+                                 int64_t form, int64_t M, int64_t K, const torch::TensorOptions& bf16, bool few = false) {
   TORCH_CHECK(form >= 0 && form <= 2, "linear_int8: form 0 to 2");
-  const int64_t M = x.size(0), K = x.size(1);
   check_int8_weights(w, w_scale, K, x, form);
   const int64_t N = w.size(0);
   TORCH_CHECK(form != 2 || (M >= 1 && M <= 128), "linear_int8: sums of 1 to 128 rows");
@@ -646,12 +647,31 @@ torch::Tensor linear_int8(torch::Tensor x, torch::Tensor w, torch::Tensor w_scal
                     bias->device() == x.device(), "linear_int8: bias bf16 [N] of a plain product");
     if (reinterpret_cast<uintptr_t>(bias->data_ptr()) % 8) bias = bias->clone();
   }
+  if (form != 2) return torch::empty({M, form == 1 ? N / 2 : N}, bf16);
+  return torch::empty({few ? 1 : linear_int8_splits((int)M, (int)N, (int)K), M, N}, bf16.dtype(torch::kFloat));
+}
+
+static void int8_product(torch::Tensor& out, const int8_t* x, const float* xs, const torch::Tensor& w, const torch::Tensor& w_scale,
+                         const std::optional<torch::Tensor>& bias, int64_t room, int* count, int64_t M, int64_t N, int64_t K, int64_t form,
+                         bool once) {
+  auto part = room ? torch::empty({room}, out.options().dtype(torch::kFloat)) : torch::Tensor();
+  TORCH_CHECK(launch_linear_int8(out.data_ptr(), x, xs, w.data_ptr<int8_t>(), w_scale.data_ptr<float>(), bias ? cbf(*bias) : nullptr,
+                                 room ? part.data_ptr<float>() : nullptr, count, (int)M, (int)N, (int)K, (int)form, once, cur_stream()) == 0,
+              "linear_int8: 160 KB of LDS are not available");
+}
+
+// form 0: x [M, K] w^T (+ bias) in bf16, 1: silu(gate) * up of a fused [gate; up], 2: fp32 sums [S, M, N] of up to 128 rows.
+// once: the weights of the caller's step do not stay in the caches until its next
+torch::Tensor linear_int8(torch::Tensor x, torch::Tensor w, torch::Tensor w_scale, std::optional<torch::Tensor> bias, int64_t form,
+                          bool once) {
+  check_int8_rows(x, "linear_int8");
+  const int64_t M = x.size(0), K = x.size(1), N = w.size(0);
   const c10::DeviceGuard device(x.device());
-  const int S = form == 2 ? linear_int8_splits((int)M, (int)N, (int)K) : 1;
-  auto out = form == 2 ? torch::empty({S, M, N}, x.options().dtype(torch::kFloat)) : torch::empty({M, form == 1 ? N / 2 : N}, x.options());
+  const bool few = linear_int8_few((int)M, (int)N, (int)K, (int)form);
+  auto out = int8_result(x, w, w_scale, bias, form, M, K, x.options(), few);
   if (M == 0) return out;
   x = int8_readable(x);
-  if (linear_int8_few((int)std::min<int64_t>(M, 1 << 20), (int)N, (int)K, (int)form)) {
+  if (few) {
     TORCH_CHECK(launch_linear_int8_few(out.data_ptr(), cbf(x), x.stride(0), w.data_ptr<int8_t>(), w_scale.data_ptr<float>(),
                                        bias ? cbf(*bias) : nullptr, (int)M, (int)N, (int)K, (int)form, once, cur_stream()) == 0,
                 "linear_int8: a form of few rows that is not there");
@@ -663,14 +683,34 @@ torch::Tensor linear_int8(torch::Tensor x, torch::Tensor w, torch::Tensor w_scal
   // codes, scales and counters in one allocation
   const int64_t scales_at = M * padded, count_at = scales_at + (M + 3) / 4 * 16;
   auto work = torch::empty({count_at + 4 * zeros}, x.options().dtype(torch::kByte));
-  auto part = room ? torch::empty({room}, x.options().dtype(torch::kFloat)) : torch::Tensor();
   char* at = reinterpret_cast<char*>(work.data_ptr());
   launch_int8_rows(reinterpret_cast<int8_t*>(at), reinterpret_cast<float*>(at + scales_at), cbf(x), x.stride(0), (int)M, (int)K,
                    reinterpret_cast<int*>(at + count_at), zeros, cur_stream());
-  TORCH_CHECK(launch_linear_int8(out.data_ptr(), reinterpret_cast<int8_t*>(at), reinterpret_cast<float*>(at + scales_at), w.data_ptr<int8_t>(),
-                                 w_scale.data_ptr<float>(), bias ? cbf(*bias) : nullptr, room ? part.data_ptr<float>() : nullptr,
-                                 reinterpret_cast<int*>(at + count_at), (int)M, (int)N, (int)K, (int)form, once, cur_stream()) == 0,
-              "linear_int8: 160 KB of LDS are not available");
+  int8_product(out, reinterpret_cast<int8_t*>(at), reinterpret_cast<float*>(at + scales_at), w, w_scale, bias, room,
+               reinterpret_cast<int*>(at + count_at), M, N, K, form, once);
+  return out;
+}
+
+// linear_int8 of rows that are codes already: int8 [M, K] and their scales fp32 [M]
+torch::Tensor linear_int8_codes(torch::Tensor codes, torch::Tensor scales, torch::Tensor w, torch::Tensor w_scale,
+                                std::optional<torch::Tensor> bias, int64_t form, bool once) {
+  TORCH_CHECK(codes.is_cuda() && codes.scalar_type() == at::kChar && codes.dim() == 2 && scales.scalar_type() == at::kFloat &&
+                  scales.dim() == 1 && scales.is_contiguous() && scales.size(0) == codes.size(0) && scales.device() == codes.device(),
+              "linear_int8: codes int8 [M, K] with a scale fp32 for each row on one device");
+  const int64_t M = codes.size(0), K = codes.size(1), N = w.size(0);
+  check_int8_sizes(M, K, "linear_int8");
+  const c10::DeviceGuard device(codes.device());
+  auto out = int8_result(codes, w, w_scale, bias, form, M, K, codes.options().dtype(torch::kBFloat16));
+  if (M == 0) return out;
+  // whole stages, zeros behind K
+  const int64_t padded = int8_rows_padded((int)K);
+  if (padded != K) codes = at::constant_pad_nd(codes, {0, padded - K});
+  if (!codes.is_contiguous() || !on_16_bytes_at(codes)) codes = codes.clone(at::MemoryFormat::Contiguous);
+  int zeros = 0;
+  const int64_t room = form == 2 ? 0 : linear_int8_room((int)M, (int)N, (int)K, (int)form, &zeros);
+  auto count = zeros ? torch::zeros({zeros}, codes.options().dtype(torch::kInt)) : torch::Tensor();
+  int8_product(out, codes.data_ptr<int8_t>(), scales.data_ptr<float>(), w, w_scale, bias, room, zeros ? count.data_ptr<int>() : nullptr, M, N, K,
+               form, once);
   return out;
 }
 
@@ -814,7 +854,7 @@ bool rows_weights_ok(const std::vector<torch::Tensor>& ws, const torch::Tensor& 
 // --- row-wise steps of a decode step (decode_rows.hip) -------------------------
 extern "C" void launch_add_norm_rows(bf16_t* out, bf16_t* residual, const float* part, const int64_t* ids,
                                      const bf16_t* table, const bf16_t* w, int S, int M, int n, int64_t vocab,
-                                     float eps, int* unknown, int* clear, int clears, hipStream_t stream);
+                                     float eps, int* unknown, int* clear, int clears, float* scales, hipStream_t stream);
 extern "C" void launch_rope_store_rows(bf16_t* q_out, const float* part, const bf16_t* bias, const int64_t* positions,
                                        const float* cos_sin, void* k_cache, void* v_cache, void* k_scale,
                                        void* v_scale, const int64_t* slots, int S, int M, int H, int G,
@@ -825,16 +865,29 @@ extern "C" void launch_decode_inputs(int64_t* ids, int64_t* positions, int64_t* 
                                      int scratch_block, int block_size, hipStream_t stream);
 
 // residual += split sums [S, M, n]; returns rms(residual) * weight
-torch::Tensor add_norm_rows(torch::Tensor part, torch::Tensor residual, torch::Tensor weight, double eps) {
+static void add_norm_rows_into(void* out, float* scales, torch::Tensor part, torch::Tensor residual, torch::Tensor weight, double eps) {
   CHECK_BF16_CONTIG(residual); CHECK_BF16_CONTIG(weight);
   TORCH_CHECK(part.is_cuda() && part.is_contiguous() && part.scalar_type() == at::kFloat && part.dim() == 3);
   const int S = part.size(0), M = part.size(1), n = part.size(2);
   TORCH_CHECK(residual.dim() == 2 && residual.size(0) == M && residual.size(1) == n && weight.numel() == n &&
                   n % 4 == 0 && n <= 16384 && S >= 1 && M >= 1, "add_norm_rows: sizes");
+  launch_add_norm_rows((bf16_t*)out, bf(residual), part.data_ptr<float>(), nullptr, nullptr, cbf(weight), S, M, n, 0,
+                       (float)eps, nullptr, nullptr, 0, scales, cur_stream());
+}
+
+torch::Tensor add_norm_rows(torch::Tensor part, torch::Tensor residual, torch::Tensor weight, double eps) {
   auto out = torch::empty_like(residual);
-  launch_add_norm_rows(bf(out), bf(residual), part.data_ptr<float>(), nullptr, nullptr, cbf(weight), S, M, n, 0,
-                       (float)eps, nullptr, nullptr, 0, cur_stream());
+  add_norm_rows_into(out.data_ptr(), nullptr, part, residual, weight, eps);
   return out;
+}
+
+// quantize_rows of add_norm_rows, of rows that whole stages of the products divide
+std::tuple<torch::Tensor, torch::Tensor> add_norm_rows_int8(torch::Tensor part, torch::Tensor residual, torch::Tensor weight, double eps) {
+  TORCH_CHECK(residual.dim() == 2 && residual.size(1) % 128 == 0, "add_norm_rows_int8: rows of a multiple of 128");
+  auto codes = torch::empty(residual.sizes(), residual.options().dtype(torch::kChar));
+  auto scales = torch::empty({residual.size(0)}, residual.options().dtype(torch::kFloat));
+  add_norm_rows_into(codes.data_ptr(), scales.data_ptr<float>(), part, residual, weight, eps);
+  return {codes, scales};
 }
 
 // (rms(table[ids]) * weight, table[ids]); an id outside the table gives a row of NaN and sets unknown (empty, or one
@@ -853,7 +906,7 @@ std::vector<torch::Tensor> embed_norm_rows(torch::Tensor ids, torch::Tensor tabl
   auto out = torch::empty_like(residual);
   launch_add_norm_rows(bf(out), bf(residual), nullptr, ids.data_ptr<int64_t>(), cbf(table), cbf(weight), 0, M, n,
                        table.size(0), (float)eps, unknown.numel() ? unknown.data_ptr<int>() : nullptr,
-                       clear ? clear->data_ptr<int>() : nullptr, clear ? (int)clear->numel() : 0, cur_stream());
+                       clear ? clear->data_ptr<int>() : nullptr, clear ? (int)clear->numel() : 0, nullptr, cur_stream());
   return {out, residual};
 }
 
@@ -968,6 +1021,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("once") = false);
   m.def("rows_weights_ok", &rows_weights_ok);
   m.def("add_norm_rows", &add_norm_rows);
+  m.def("add_norm_rows_int8", &add_norm_rows_int8);
   m.def("embed_norm_rows", &embed_norm_rows, py::arg("ids"), py::arg("table"), py::arg("weight"), py::arg("eps"),
         py::arg("unknown"), py::arg("clear") = py::none());
   m.def("rope_store_rows", &rope_store_rows);
@@ -975,7 +1029,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("quantize_rows", &quantize_rows);
   m.def("linear_int8", &linear_int8, py::arg("x"), py::arg("w"), py::arg("w_scale"), py::arg("bias"), py::arg("form"),
         py::arg("once") = false);
-  m.def("linear_int8_splits", &linear_int8_splits);
+  m.def("linear_int8_codes", &linear_int8_codes);
+  m.def("linear_int8_few", &linear_int8_few);
   m.def("linear_tiles", &linear_tiles);
   m.def("linear_tiles_rows", &linear_tiles_rows);
   m.def("linear_tiles_pick", &linear_tiles_pick);

@@ -16,6 +16,7 @@
 
 #include <type_traits>
 
+#include "int8.h"
 #include "kv4.h"
 
 #define DR_THREADS 1024
@@ -66,15 +67,36 @@ __device__ __forceinline__ float row_sum(float v, float* scratch) {
   return over_wave(scratch[threadIdx.x & 15], false);      // 16 waves
 }
 
+// Largest of the workgroup, by the same moves
+__device__ __forceinline__ uint32_t row_most(uint32_t v, uint32_t* scratch) {
+  auto moved = [](uint32_t x, auto how) { return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, decltype(how)::value, 0xf, 0xf, false); };
+  auto over_wave = [&](uint32_t x, bool halves) -> uint32_t {
+    x = max(x, moved(x, std::integral_constant<int, 0xb1>()));
+    x = max(x, moved(x, std::integral_constant<int, 0x4e>()));
+    x = max(x, moved(x, std::integral_constant<int, 0x141>()));
+    x = max(x, moved(x, std::integral_constant<int, 0x140>()));
+    if (!halves) return x;
+    const auto s = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+    x = max((uint32_t)s[0], (uint32_t)s[1]);
+    const auto t = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+    return max((uint32_t)t[0], (uint32_t)t[1]);
+  };
+  v = over_wave(v, true);
+  if ((threadIdx.x & 63) == 0) scratch[threadIdx.x >> 6] = v;
+  __syncthreads();
+  return over_wave(scratch[threadIdx.x & 15], false);      // 16 waves
+}
+
 // residual[m] += sum of splits (written back, bf16), or residual[m] = table[ids[m]]
-// (EMBED, which also zeroes ``clear``); out[m] = rms(residual[m]) * w. One workgroup per row, the row in registers:
-// rows of up to 4 * DR_THREADS * VECS elements.
-template <bool EMBED, int VECS>
+// (EMBED, which also zeroes ``clear``); out[m] = rms(residual[m]) * w, or what int8_rows_kernel makes of that (scales). One
+// workgroup per row, the row in registers: rows of up to 4 * DR_THREADS * VECS elements.
+template <bool EMBED, int VECS, bool CODES = false>
 __global__ void __launch_bounds__(DR_THREADS) add_norm_rows_kernel(
     bf16_t* __restrict__ out, bf16_t* __restrict__ residual, const float* __restrict__ part,
     const int64_t* __restrict__ ids, const bf16_t* __restrict__ table, const bf16_t* __restrict__ w, int S, int M,
-    int n, int64_t vocab, float eps, int* __restrict__ unknown, int* __restrict__ clear, int clears) {
+    int n, int64_t vocab, float eps, int* __restrict__ unknown, int* __restrict__ clear, int clears, float* __restrict__ scales) {
   __shared__ float red[16];
+  __shared__ uint32_t red_most[16];
   if constexpr (EMBED)
     for (int i = blockIdx.x * DR_THREADS + threadIdx.x; i < clears; i += gridDim.x * DR_THREADS) clear[i] = 0;
   const int m = blockIdx.x, tid = threadIdx.x;
@@ -112,26 +134,42 @@ __global__ void __launch_bounds__(DR_THREADS) add_norm_rows_kernel(
   }
   ss = row_sum(ss, red);
   const float inv = rsqrtf(ss / n + eps);
+  bf16x4_vec o[VECS];
+  uint32_t most = 0;
 #pragma unroll
   for (int k = 0; k < VECS; ++k) {
     const int i = tid + k * DR_THREADS;
     if (i >= nvec) break;
-    bf16x4_vec o;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) o[j] = f32_to_bf16(x[k][j] * inv * bf16_to_f32(g[k][j]));
-    ov[i] = o;
+    for (int j = 0; j < 4; ++j) {
+      o[k][j] = f32_to_bf16(x[k][j] * inv * bf16_to_f32(g[k][j]));
+      most = max(most, (uint32_t)(o[k][j] & 0x7fff));
+    }
+    if constexpr (!CODES) ov[i] = o[k];
+  }
+  if constexpr (CODES) {
+    const Int8Row by(row_most(most, red_most));
+    if (tid == 0) scales[m] = by.scale;
+    uint32_t* codes = reinterpret_cast<uint32_t*>(out) + (int64_t)m * nvec;
+#pragma unroll
+    for (int k = 0; k < VECS; ++k) {
+      const int i = tid + k * DR_THREADS;
+      if (i >= nvec) break;
+      codes[i] = by.four(o[k][0], o[k][1], o[k][2], o[k][3]);
+    }
   }
 }
 
 extern "C" void launch_add_norm_rows(bf16_t* out, bf16_t* residual, const float* part, const int64_t* ids,
                                      const bf16_t* table, const bf16_t* w, int S, int M, int n, int64_t vocab,
-                                     float eps, int* unknown, int* clear, int clears, hipStream_t stream) {
+                                     float eps, int* unknown, int* clear, int clears, float* scales, hipStream_t stream) {
   auto go = [&](auto kernel) {
     hipLaunchKernelGGL(kernel, dim3(M), dim3(DR_THREADS), 0, stream, out, residual, part, ids, table, w, S, M, n, vocab, eps,
-                       unknown, clear, clears);
+                       unknown, clear, clears, scales);
   };
   const bool narrow = n <= 4 * DR_THREADS;
-  if (ids) narrow ? go(add_norm_rows_kernel<true, 1>) : go(add_norm_rows_kernel<true, 4>);
+  if (scales) narrow ? go(add_norm_rows_kernel<false, 1, true>) : go(add_norm_rows_kernel<false, 4, true>);
+  else if (ids) narrow ? go(add_norm_rows_kernel<true, 1>) : go(add_norm_rows_kernel<true, 4>);
   else narrow ? go(add_norm_rows_kernel<false, 1>) : go(add_norm_rows_kernel<false, 4>);
 }
 

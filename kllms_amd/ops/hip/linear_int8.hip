@@ -19,46 +19,14 @@
 
 #include <atomic>
 
+#include "int8.h"
 #include "tile_product.h"
 
-typedef unsigned short u16x8 __attribute__((ext_vector_type(8)));
-typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
 
 #define LI_STAGE 128       // bytes of a row in a stage
 enum Int8Form { LI_BF16 = 0, LI_SILU = 1, LI_PART = 2 };
 
 // ---- codes ---------------------------------------------------------------------------------------
-
-// What rows are multiplied with before they are rounded: 127 / most by an inverse and what it leaves, both taken near one
-struct Int8Row {
-  float up, most, inverse, scale;
-  __device__ __forceinline__ explicit Int8Row(uint32_t bits) {       // of the largest magnitude, as bf16
-    const float m = __uint_as_float(bits << 16);
-    const bool sound = bits < 0x7f80u;                               // neither infinite nor NaN
-    const int e = max((int)(bits >> 7) - 127, -120);
-    const float f = ldexpf(1.0f, -e);
-    up = 127.0f * f;
-    most = m * f;
-    inverse = sound && m > 0.0f ? 1.0f / most : 0.0f;
-    scale = sound ? m / 127.0f : __uint_as_float(0x7fc00000u);       // such a row is NaN as a whole
-  }
-  // its code is the lowest byte: added to 1.5 * 2^23, a number this small is rounded as rint does and stands in the last bits. No
-  // number passes 127 by as much as that sees; of a row that is not sound the codes do not matter.
-  __device__ __forceinline__ uint32_t code(float x) const {
-    const float t = x * up, q = t * inverse;
-    return __float_as_uint(__builtin_fmaf(__builtin_fmaf(-q, most, t), inverse, q) + 12582912.0f);
-  }
-  __device__ __forceinline__ u32x2 codes(const u16x8& x) const {
-    uint32_t c[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) c[j] = code(bf16_to_f32((short)x[j]));
-    auto four = [&](int j) {
-      return __builtin_amdgcn_perm(__builtin_amdgcn_perm(c[j + 3], c[j + 2], 0x0c0c0400u), __builtin_amdgcn_perm(c[j + 1], c[j], 0x0c0c0400u),
-                                   0x05040100u);
-    };
-    return u32x2{four(0), four(4)};
-  }
-};
 
 // LANES threads a row, R vectors of 8 of each (R 0: any number, read twice). codes [M, padded], zeros behind K; clears
 // ``clear`` beside.
@@ -484,9 +452,8 @@ static Int8Plan int8_plan(int64_t M, int64_t N, int64_t K, int form) {
   return best;
 }
 
-extern "C" int linear_int8_splits(int M, int N, int K) {
-  return linear_int8_few(M, N, K, LI_PART) ? 1 : int8_plan(M, N, K, LI_PART).splits;
-}
+// shares of form 2 of a product whose codes are made before it
+extern "C" int linear_int8_splits(int M, int N, int K) { return int8_plan(M, N, K, LI_PART).splits; }
 
 template <int NI, int MJ, int FORM, bool ONCE>
 static int linear_int8_rows_go(const Int8Plan& p, void* out, const int8_t* x, const float* xs, const int8_t* w, const float* ws,

@@ -112,12 +112,13 @@ def quantize_weights(w: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
 
 
 def linear_int8(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, bias=None) -> torch.Tensor:
-    """(quantized x) w^T with both scales (+ bias), fp32 before the rounding to x's dtype; w int8 [N, K], w_scale fp32 [N]."""
-    return _linear_int8(x, w, w_scale, bias).to(x.dtype)
+    """(quantized x) w^T with both scales (+ bias), fp32 before the rounding to x's dtype; w int8 [N, K], w_scale fp32 [N].
+    x may be what quantize_rows gives: then the result is bf16."""
+    return _linear_int8(x, w, w_scale, bias).to(torch.bfloat16 if isinstance(x, tuple) else x.dtype)
 
 
 def _linear_int8(x, w, w_scale, bias=None) -> torch.Tensor:
-    codes, scales = quantize_rows(x)
+    codes, scales = x if isinstance(x, tuple) else quantize_rows(x)
     sums = codes.double() @ w.double().t()                # whole numbers, exact
     y = sums.float() * scales[:, None] * w_scale
     return y if bias is None else y + bias.float()
@@ -126,7 +127,7 @@ def _linear_int8(x, w, w_scale, bias=None) -> torch.Tensor:
 def linear_silu_int8(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor) -> torch.Tensor:
     """silu(gate) * up of a fused [gate; up] int8 matrix."""
     gate, up = _linear_int8(x, w, w_scale).chunk(2, -1)
-    return (torch.nn.functional.silu(gate) * up).to(x.dtype)
+    return (torch.nn.functional.silu(gate) * up).to(torch.bfloat16 if isinstance(x, tuple) else x.dtype)
 
 
 # --- paged KV cache -----------------------------------------------------------

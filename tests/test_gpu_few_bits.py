@@ -36,11 +36,12 @@ def test_graphs_give_what_eager_steps_give(model, weight, cache):
     assert all(len(t) > 0 for o in runs[0] for t in o)
 
 
-def test_a_step_on_the_few_row_kernels_is_one_of_the_modules():
+@pytest.mark.parametrize("B", [5, 24])
+def test_a_step_on_the_few_row_kernels_is_one_of_the_modules(B):
     """The step's sums in shares against the layers' own calls: the same whole numbers, rounded at other places."""
     eng = engine(weight_dtype="int8", kv_cache_dtype="int4")
     model, kv = eng.model, eng.kv
-    B, ctx = 5, 70
+    ctx = 70
     g = torch.Generator().manual_seed(1)
     per = -(-ctx // 16)
     tables = torch.arange(B * per, dtype=torch.int32).view(B, per).cuda()

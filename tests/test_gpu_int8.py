@@ -105,6 +105,61 @@ def test_sums_in_shares(M, N, K):
     assert bool(((part.double().sum(0).cpu() - y).abs() <= 2 ** -22 * size + 1e-30).all())
 
 
+@pytest.mark.parametrize("M", [1, 7, 40, 129, 400])
+@pytest.mark.parametrize("N,K", [(64, 16), (544, 144), (2048, 1024), (6144, 4096)])
+def test_products_of_codes_are_those_of_rows(M, N, K):
+    x, (w, ws) = rows(M, K, seed=M + N), weights(N, K, seed=N)
+    bias = torch.randn(N, generator=torch.Generator().manual_seed(2)).bfloat16().to(DEV)
+    x, w, ws = (t.to(DEV) for t in (x, w, ws))
+    small = ws * 0.05
+    codes = ops.quantize_rows(x)
+    assert isinstance(codes, ops.Int8Rows)
+    packed = ops.Int8Rows(codes.codes.contiguous(), codes.scales)
+    behind = torch.randint(-127, 128, (M, K + 160), dtype=torch.int8, device=DEV)        # rows of a wider matrix, others' codes behind
+    behind[:, 16:16 + K] = codes.codes
+    for c in (codes, packed, ops.Int8Rows(behind[:, 16:16 + K], codes.scales)):
+        assert torch.equal(ops.linear_int8(c, w, ws, bias), ops.linear_int8(x, w, ws, bias))
+        assert torch.equal(ops.linear_silu_int8(c, w, small), ops.linear_silu_int8(x, w, small))
+        if M <= 128:
+            # 3 roundings of 2^-24 of each share's size either way, whose sizes add up to the products' at most
+            size = (codes.codes.double().abs() @ w.double().abs().t()) * codes.scales.double()[:, None] * ws.double()
+            far = (ops.linear_part_int8(c, w, ws).double().sum(0) - ops.linear_part_int8(x, w, ws).double().sum(0)).abs()
+            assert bool((far <= 2 ** -21 * size + 1e-30).all())
+
+
+@pytest.mark.parametrize("M", [1, 9, 128])
+@pytest.mark.parametrize("n", [128, 1024, 4096, 8192, 16384])
+def test_norm_that_leaves_codes(M, n):
+    g = torch.Generator().manual_seed(n + M)
+    part = (torch.randn(2, M, n, generator=g) * 3).to(DEV)
+    residual, weight = torch.randn(M, n, generator=g).bfloat16().to(DEV), torch.randn(n, generator=g).bfloat16().to(DEV)
+    if M > 2:
+        part[0, 1, 5] = float("nan")
+        residual[2] = 0
+        part[:, 2] = 0
+    two = residual.clone()
+    want = ops.quantize_rows(ops.add_norm_rows(part, residual, weight, 1e-5))
+    got = ops.add_norm_rows_int8(part, two, weight, 1e-5)
+    sound = ~torch.isnan(want.scales)
+    assert torch.equal(sound, ~torch.isnan(got.scales)) and int((~sound).sum()) == (M > 2)
+    assert torch.equal(got.codes[sound], want.codes[sound]) and torch.equal(got.scales[sound], want.scales[sound])
+    assert torch.equal(two[sound], residual[sound])
+
+
+def test_refusals_of_codes():
+    x, (w, ws) = rows(20, 256).to(DEV), weights(64, 256)
+    w, ws = w.to(DEV), ws.to(DEV)
+    c = ops.quantize_rows(x)
+    for bad in (ops.Int8Rows(x, c.scales), ops.Int8Rows(c.codes, c.scales.half()), ops.Int8Rows(c.codes, c.scales[:3]), ops.Int8Rows(c.codes[:, :128], c.scales)):
+        with pytest.raises(ValueError):
+            ops.linear_int8(bad, w, ws)
+    for bad in (ops.Int8Rows(c.codes, c.scales.cpu()), ops.Int8Rows(c.codes, torch.cat((c.scales, c.scales))[::2])):
+        with pytest.raises(RuntimeError):
+            ops.linear_int8(bad, w, ws)
+    with pytest.raises(RuntimeError, match="multiple of 128"):
+        ops.add_norm_rows_int8(torch.zeros(1, 2, 96, device=DEV), torch.zeros(2, 96, device=DEV).bfloat16(), torch.ones(96, device=DEV).bfloat16(), 1e-5)
+
+
 @pytest.mark.parametrize("M", [1, 2, 3, 4, 5, 6, 7, 8, 9])
 @pytest.mark.parametrize("N,K", [(32, 16), (64, 144), (4096, 1040), (4128, 2064), (8224, 4112), (544, 8208), (256, 16384), (128, 16400)])
 def test_few_rows(M, N, K):

@@ -109,3 +109,14 @@ def test_layers_are_the_operator():
 def test_other_families_are_refused():
     with pytest.raises(ValueError, match="int8"):
         engine(model="tiny-zutalix")
+
+
+def test_rows_that_are_codes_already():
+    g = torch.Generator().manual_seed(8)
+    x, (w, ws) = torch.randn(5, 48, generator=g).bfloat16(), ops.quantize_weights(torch.randn(32, 48, generator=g))
+    c = ops.quantize_rows(x)
+    assert torch.equal(ops.linear_int8(c, w, ws), ops.linear_int8(x, w, ws))
+    assert torch.equal(ops.linear_silu_int8(c, w, ws), ops.linear_silu_int8(x, w, ws))
+    for bad in (ops.Int8Rows(x, c.scales), ops.Int8Rows(c.codes, c.scales.double()), ops.Int8Rows(c.codes, c.scales[:2])):
+        with pytest.raises(ValueError):
+            ops.linear_int8(bad, w, ws)
