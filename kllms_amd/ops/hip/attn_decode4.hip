@@ -74,8 +74,12 @@ struct Deal {
   int row, length, share, shares, start;   // workgroups of the row, from slot ``start`` on; row -1: nobody's slot
 };
 __device__ __forceinline__ int tiles_of(int length) { return (int)(((int64_t)length + TKEYS - 1) / TKEYS); }
-// any number does, as long as all agree: the tiles go round
-__device__ __forceinline__ int shares_of(int tiles, float inverse) { return max((int)ceilf(tiles * inverse - 1e-3f), 1); }
+// any number does, as long as all agree: the tiles go round. A share takes 3 us to be joined, a round of four tiles 1.9: those that
+// save less than two rounds are not made (one context of 300 9.7 us in two, 8.4 in one; of 530 9.9 in three, 10.3)
+__device__ __forceinline__ int shares_of(int tiles, float inverse) {
+  const int n = max((int)ceilf(tiles * inverse - 1e-3f), 1);
+  return tiles > 8 && ceilf(tiles * 0.25f) - ceilf(tiles * 0.25f * __builtin_amdgcn_rcpf((float)n) - 1e-3f) >= 2.0f ? n : 1;
+}
 template <int CTRL, int ROWS = 0xf>
 __device__ __forceinline__ int lane_moved(int x) { return __builtin_amdgcn_update_dpp(0, x, CTRL, ROWS, 0xf, false); }
 __device__ __forceinline__ int scan(int x) {             // of this lane's and those before it
@@ -90,7 +94,7 @@ __device__ __forceinline__ int scan(int x) {             // of this lane's and t
 __device__ __forceinline__ int last_lane(int x) { return __builtin_amdgcn_readlane(x, 63); }
 // BY_ROW: of row ``at``; else of slot ``at``. EACH: rows of a lane
 template <bool BY_ROW, int EACH>
-__device__ __forceinline__ Deal deal_rows(const int* __restrict__ lengths, int B, int64_t limit, int slots, int at) {
+__device__ __forceinline__ Deal deal_rows(const int* __restrict__ lengths, int B, int kv_heads, int64_t limit, int slots, int at) {
   const int lane = threadIdx.x & 63;
   int length[EACH], z[EACH], n = 0;
 #pragma unroll
@@ -99,9 +103,12 @@ __device__ __forceinline__ Deal deal_rows(const int* __restrict__ lengths, int B
     length[e] = row < B ? (int)min((int64_t)max(lengths[row], 0), limit) : 0;
     n += tiles_of(length[e]);
   }
-  // not more workgroups than there are four tiles for
+  // Not more workgroups than there are four tiles for; of many contexts, which fill the chip as they are, more tiles: a sixteenth of how
+  // many there are, but of contexts that are longer than most as many as most have. 32 / 8 heads, us: 32 of 1000 15.9 in two shares each,
+  // 13.8 in one; 16 of 1000 13.0 in four, 12.7 in two; 24 of 530 14.4 in two and three, 11.4 in one
   const float all = (float)max(last_lane(scan(n)), 1);
-  auto inverse = [&](float of) { return fminf(__builtin_amdgcn_rcpf(all) * of, 0.25f); };
+  const float most = __builtin_amdgcn_rcpf(fmaxf(4.0f, fminf((float)B * kv_heads * (1.0f / 16), all * 1.5f * __builtin_amdgcn_rcpf((float)B))));
+  auto inverse = [&](float of) { return fminf(__builtin_amdgcn_rcpf(all) * of, most); };
   const float per0 = inverse(slots), per1 = inverse(slots - 0.5f * B);
   n = 0;                                   // slots by the first and by the second, 16 bits each
 #pragma unroll
@@ -130,13 +137,14 @@ __device__ __forceinline__ Deal deal_rows(const int* __restrict__ lengths, int B
   return d;
 }
 template <bool BY_ROW>
-__device__ __forceinline__ Deal deal(const int* __restrict__ lengths, int B, int64_t limit, int slots, int at) {
+__device__ __forceinline__ Deal deal(const int* __restrict__ lengths, int B, int kv_heads, int64_t limit, int slots, int at) {
   if (slots <= B) return Deal{at, (int)min((int64_t)max(lengths[at], 0), limit), 0, 1, at};
   if (B == 1) {
     const int length = (int)min((int64_t)max(lengths[0], 0), limit), n = min(shares_of(tiles_of(length), 0.25f), slots);
     return Deal{BY_ROW || at < n ? 0 : -1, length, at, n, 0};
   }
-  return B <= 64 ? deal_rows<BY_ROW, 1>(lengths, B, limit, slots, at) : deal_rows<BY_ROW, DEAL_ROWS / 64>(lengths, B, limit, slots, at);
+  return B <= 64 ? deal_rows<BY_ROW, 1>(lengths, B, kv_heads, limit, slots, at)
+                 : deal_rows<BY_ROW, DEAL_ROWS / 64>(lengths, B, kv_heads, limit, slots, at);
 }
 
 // The partials [GQA, PART_STRIDE] of Z workgroups, ``apart`` floats from each other, in their order, to rows of the result,
@@ -220,7 +228,7 @@ __global__ __launch_bounds__(NTHREADS, GQA == 8 || !WHOLE ? 3 : 4) void attn_dec
   __shared__ float m_lds[4][16], l_lds[4][16];
   __shared__ int last_lds;
   const int g_kv = blockIdx.x, num_kv_heads = gridDim.x;
-  const Deal mine = deal<false>(context_lens, B, (int64_t)max_blocks * block_size, slots, blockIdx.y);
+  const Deal mine = deal<false>(context_lens, B, num_kv_heads, (int64_t)max_blocks * block_size, slots, blockIdx.y);
   const int b = __builtin_amdgcn_readfirstlane(mine.row), z = __builtin_amdgcn_readfirstlane(mine.share);
   const int Z = __builtin_amdgcn_readfirstlane(mine.shares), L = __builtin_amdgcn_readfirstlane(mine.length);
   if (b < 0) return;
@@ -637,10 +645,10 @@ __global__ __launch_bounds__(NTHREADS, GQA == 8 || !WHOLE ? 3 : 4) void attn_dec
 // the same in a launch of its own, a workgroup for each head
 __global__ __launch_bounds__(NTHREADS) void attn_decode4_merge_kernel(bf16_t* __restrict__ out, const float* __restrict__ partials,
                                                                      const int* __restrict__ context_lens, int64_t limit, int B,
-                                                                     int slots) {
+                                                                     int kv_heads, int slots) {
   __shared__ float sums[NTHREADS][4], ml[NTHREADS][2];
   const int h = blockIdx.x, num_q_heads = gridDim.x, b = blockIdx.y;
-  const Deal mine = deal<true>(context_lens, B, limit, slots, b);
+  const Deal mine = deal<true>(context_lens, B, kv_heads, limit, slots, b);
   const int Z = __builtin_amdgcn_readfirstlane(mine.shares);
   if (Z == 1) return;                      // its one workgroup has written the result
   merge4<1>(out + ((int64_t)b * num_q_heads + h) * 128,
@@ -704,6 +712,6 @@ extern "C" void launch_attn_decode4(bf16_t* out, float* partials, int* arrived, 
 #undef LAUNCH
     if (slots > B && !arrived)
       hipLaunchKernelGGL(attn_decode4_merge_kernel, dim3(num_q_heads, rows), dim3(NTHREADS), 0, stream, o, partials, context_lens + b0, limit,
-                         rows, slots);
+                         rows, num_kv_heads, slots);
   }
 }
