@@ -187,6 +187,10 @@ __global__ void __launch_bounds__(64 * LF_WAVES) linear_int8_few_kernel(void* __
       if (NS % 4 == 0 || i < NS * 16) *reinterpret_cast<u32x2*>(codes + r * ROW + i * 8) = by.codes(v[r][j]);
     }
   }
+  // this wave's own part of LDS: in order, only the compiler is held
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
   i32x4 acc[T];
 #pragma unroll
   for (int t = 0; t < T; ++t) acc[t] = i32x4{0, 0, 0, 0};
