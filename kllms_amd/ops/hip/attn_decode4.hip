@@ -77,8 +77,10 @@ __device__ __forceinline__ int tiles_of(int length) { return (int)(((int64_t)len
 // any number does, as long as all agree: the tiles go round. A share takes 3 us to be joined, a round of four tiles 1.9: those that
 // save less than two rounds are not made (one context of 300 9.7 us in two, 8.4 in one; of 530 9.9 in three, 10.3)
 __device__ __forceinline__ int shares_of(int tiles, float inverse) {
-  const int n = max((int)ceilf(tiles * inverse - 1e-3f), 1);
-  return tiles > 8 && ceilf(tiles * 0.25f) - ceilf(tiles * 0.25f * __builtin_amdgcn_rcpf((float)n) - 1e-3f) >= 2.0f ? n : 1;
+  // written as the operations that they are: both kernels have to come to the same number
+  const int n = max((int)ceilf(__builtin_fmaf((float)tiles, inverse, -1e-3f)), 1);
+  const float rounds = ceilf(__builtin_fmaf(tiles * 0.25f, __builtin_amdgcn_rcpf((float)n), -1e-3f));
+  return tiles > 8 && ceilf(tiles * 0.25f) - rounds >= 2.0f ? n : 1;
 }
 template <int CTRL, int ROWS = 0xf>
 __device__ __forceinline__ int lane_moved(int x) { return __builtin_amdgcn_update_dpp(0, x, CTRL, ROWS, 0xf, false); }

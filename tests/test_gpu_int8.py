@@ -161,7 +161,8 @@ def test_refusals_of_codes():
 
 
 @pytest.mark.parametrize("M", [1, 2, 3, 4, 5, 6, 7, 8, 9])
-@pytest.mark.parametrize("N,K", [(32, 16), (64, 144), (4096, 1040), (4128, 2064), (8224, 4112), (544, 8208), (256, 16384), (128, 16400)])
+@pytest.mark.parametrize("N,K", [(32, 16), (64, 144), (4096, 1040), (4128, 2064), (8224, 4112), (544, 8208), (256, 16384), (128, 16400), (512, 8192),
+                                 (1040, 4096), (4608, 4096)])
 def test_few_rows(M, N, K):
     """Codes made on the way: stages that end inside K, waves without a stage, an odd number of tiles, all forms."""
     x, (w, ws) = rows(M, K, seed=M + K), weights(N, K, seed=N)
@@ -172,7 +173,8 @@ def test_few_rows(M, N, K):
     check(ops.linear_int8(*args), x, w, ws)
     check(ops.linear_int8(*args, bias.to(DEV), once=True), x, w, ws, bias)
     small = ws * (0.05 * 64 / K ** 0.5)
-    check(ops.linear_silu_int8(args[0], args[1], small.to(DEV)), x, w, small, gated=True)
+    if N % 32 == 0:
+        check(ops.linear_silu_int8(args[0], args[1], small.to(DEV)), x, w, small, gated=True)
     part = ops.linear_part_int8(*args)
     # each share's exact sum is rounded by 2^-24 as it becomes fp32 and at both scales, 3 * 2^-24 < 2^-22 of its own size; the
     # shares' sizes add up to no more than the products' do, and may cancel

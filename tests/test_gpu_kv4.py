@@ -172,6 +172,13 @@ def test_one_context_much_longer_than_the_others(ctx, KVH, BS):
     check(both(*args, D ** -0.5), *args, D ** -0.5)
 
 
+@pytest.mark.parametrize("ctx", [[520] * 24, [1000] * 16, [2000] * 16, [640, 641] * 3, [900 + 60 * i for i in range(12)]])
+def test_contexts_that_nearly_fill_the_chip(ctx):
+    """Where shares of a context are one, two or four by how many contexts there are."""
+    args = case(ctx, 4, 8, 16, seed=len(ctx), shared=3)
+    check(both(*args, D ** -0.5), *args, D ** -0.5)
+
+
 @pytest.mark.parametrize("gqa", [1, 2, 4, 8])
 @pytest.mark.parametrize("spread", [3.0, 20.0])
 def test_steps_and_scores_of_very_different_sizes(gqa, spread):
