@@ -640,8 +640,8 @@ __global__ __launch_bounds__(NTHREADS, GQA == 8 || !WHOLE ? 3 : 4) void attn_dec
   }
   __syncthreads();
   if (!last_lds) return;
-  merge4<GQA>(to, part - (int64_t)z * num_kv_heads * (GQA * PART_STRIDE), Z, num_kv_heads * (GQA * PART_STRIDE), reinterpret_cast<float(&)[NTHREADS][4]>(o_lds[0]),
-              reinterpret_cast<float(&)[NTHREADS][2]>(o_lds[1]));
+  merge4<GQA>(to, part - (int64_t)z * num_kv_heads * (GQA * PART_STRIDE), Z, num_kv_heads * (GQA * PART_STRIDE),
+              reinterpret_cast<float(&)[NTHREADS][4]>(o_lds[0]), reinterpret_cast<float(&)[NTHREADS][2]>(o_lds[1]));
 }
 
 // the same in a launch of its own, a workgroup for each head

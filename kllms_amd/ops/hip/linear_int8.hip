@@ -11,9 +11,12 @@
 // On the ring and tiles of tile_product.h, to which a row of K integers is one of K / 2 bf16: as many bytes and
 // matrix instructions of twice the products. Where W's stream or the depth of K is the bound, tiles of 64 or 128 rows of W
 // (linear_rows.hip has the reasons), two workgroups to a compute unit where the ring leaves room; else tiles of 256 and the
-// matrix units (linear_tiles.hip). int8_plan weighs them. Up to 8 rows go in one launch that makes the codes too. A product of few tiles is shared out over K: each workgroup leaves its
-// sums past the L2 and the last one to arrive adds them up. The counters for that are zeroed by the launch that makes the codes,
-// which comes before anyway.
+// matrix units (linear_tiles.hip). int8_plan weighs them. Up to 8 rows go in one launch that makes the codes too (int8_few). A
+// product of few tiles is shared out over K: each workgroup leaves its sums past the L2 and the last one to arrive adds them up.
+// The counters for that are zeroed by the launch that makes the codes, which comes before anyway.
+//
+// Measured, us: 6144 x 4096, 5 rows 7.9 (25 MB, 3.2 TB/s); 28672 x 4096 with the activation, 120 rows 34 (W at 3.9 TB/s), 7777 rows 805
+// (2270 TOP/s, the card's power limit; the library's 8192^3 has 2083); 4608 x 3584 with bias, 333 rows 17.9.
 //
 // K is a multiple of 16; the codes' rows are filled up to whole stages with zeros, which what W has behind a row meets.
 

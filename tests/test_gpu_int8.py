@@ -150,7 +150,8 @@ def test_refusals_of_codes():
     x, (w, ws) = rows(20, 256).to(DEV), weights(64, 256)
     w, ws = w.to(DEV), ws.to(DEV)
     c = ops.quantize_rows(x)
-    for bad in (ops.Int8Rows(x, c.scales), ops.Int8Rows(c.codes, c.scales.half()), ops.Int8Rows(c.codes, c.scales[:3]), ops.Int8Rows(c.codes[:, :128], c.scales)):
+    for bad in (ops.Int8Rows(x, c.scales), ops.Int8Rows(c.codes, c.scales.half()), ops.Int8Rows(c.codes, c.scales[:3]),
+                ops.Int8Rows(c.codes[:, :128], c.scales)):
         with pytest.raises(ValueError):
             ops.linear_int8(bad, w, ws)
     for bad in (ops.Int8Rows(c.codes, c.scales.cpu()), ops.Int8Rows(c.codes, torch.cat((c.scales, c.scales))[::2])):

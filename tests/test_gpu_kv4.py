@@ -296,7 +296,8 @@ def test_refusals():
         with pytest.raises(RuntimeError):
             call(**bad)
     new, slots = rows(1, 2, D).to(DEV), torch.zeros(1, dtype=torch.long, device=DEV)
-    for bad in (dict(slots=slots.int()), dict(k=new.float()), dict(k=new[:, :1]), dict(ks=ks.float()), dict(slots=torch.zeros(2, dtype=torch.long, device=DEV))):
+    for bad in (dict(slots=slots.int()), dict(k=new.float()), dict(k=new[:, :1]), dict(ks=ks.float()),
+                dict(slots=torch.zeros(2, dtype=torch.long, device=DEV))):
         with pytest.raises(RuntimeError):
             ops.store_kv(bad.get("k", new), new, kc, vc, bad.get("slots", slots), bad.get("ks", ks), vs)
 
