@@ -74,8 +74,8 @@ struct Deal {
   int row, length, share, shares, start;   // workgroups of the row, from slot ``start`` on; row -1: nobody's slot
 };
 __device__ __forceinline__ int tiles_of(int length) { return (int)(((int64_t)length + TKEYS - 1) / TKEYS); }
-// any number does, as long as all agree: the tiles go round. A share takes 3 us to be joined, a round of four tiles 1.9: those that
-// save less than two rounds are not made (one context of 300 9.7 us in two, 8.4 in one; of 530 9.9 in three, 10.3)
+// any number does, as long as all agree: the tiles go round. Joining shares takes 2 us, a round of four tiles 1.9: those that
+// save less than two rounds are not made (one context of 530 8.9 us in three, 10.3 in one)
 __device__ __forceinline__ int shares_of(int tiles, float inverse) {
   // written as the operations that they are: both kernels have to come to the same number
   const int n = max((int)ceilf(__builtin_fmaf((float)tiles, inverse, -1e-3f)), 1);
@@ -150,11 +150,12 @@ __device__ __forceinline__ Deal deal(const int* __restrict__ lengths, int B, int
 }
 
 // The partials [GQA, PART_STRIDE] of Z workgroups, ``apart`` floats from each other, in their order, to rows of the result,
-// by all threads
-template <int GQA>
+// by all threads. DEEP of them are asked for before the first is waited for, in fours that are there (all 16, there or not, and
+// stores of 4 bytes before it: 1 us more)
+template <int GQA, int DEEP>
 __device__ __forceinline__ void merge4(bf16_t* __restrict__ out, const float* all, int Z, int apart, float (&sums)[NTHREADS][4],
                                        float (&ml)[NTHREADS][2]) {
-  constexpr int SETS = NTHREADS / (32 * GQA), DEEP = 16;
+  constexpr int SETS = NTHREADS / (32 * GQA);
   const int tid = threadIdx.x, h = (tid >> 5) % GQA, d = (tid & 31) * 4, set = tid / (32 * GQA);
   const auto far = __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(all), 0, ((Z - 1) * apart + GQA * PART_STRIDE) * 4, 0x00020000);
   float M = -INFINITY, sum = 0.0f;
@@ -164,11 +165,15 @@ __device__ __forceinline__ void merge4(bf16_t* __restrict__ out, const float* al
     f32x4 part[DEEP];
     f32x2 of[DEEP];
 #pragma unroll
-    for (int e = 0; e < DEEP; ++e) {       // behind the last one zeros
-      const int at = ((z0 + e * SETS) * apart + h * PART_STRIDE) * 4;
-      of[e] = __builtin_bit_cast(f32x2, __builtin_amdgcn_raw_buffer_load_b64(far, at + 512, 0, FAR));
-      part[e] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(far, at + d * 4, 0, FAR));
-    }
+    for (int e0 = 0; e0 < DEEP; e0 += 4)
+      if (z0 - set + e0 * SETS < Z) {      // the same for all threads
+#pragma unroll
+        for (int e = e0; e < e0 + 4; ++e) {  // behind the last one zeros
+          const int at = ((z0 + e * SETS) * apart + h * PART_STRIDE) * 4;
+          of[e] = __builtin_bit_cast(f32x2, __builtin_amdgcn_raw_buffer_load_b64(far, at + 512, 0, FAR));
+          part[e] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(far, at + d * 4, 0, FAR));
+        }
+      }
     const float before = M;
 #pragma unroll
     for (int e = 0; e < DEEP; ++e)
@@ -624,8 +629,14 @@ __global__ __launch_bounds__(NTHREADS, GQA == 8 || !WHOLE ? 3 : 4) void attn_dec
       for (int r = 0; r < VEC; ++r) ((short*)to)[h * 128 + d + r] = f32_to_bf16(l == 0.0f ? 0.0f : acc[r] / l);
     } else {
       const auto far = __builtin_amdgcn_make_buffer_rsrc(part, 0, GQA * PART_STRIDE * 4, 0x00020000);
-#pragma unroll
-      for (int r = 0; r < VEC; ++r) __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(acc[r]), far, (h * PART_STRIDE + d + r) * 4, 0, FAR);
+      const int at = (h * PART_STRIDE + d) * 4;
+      if constexpr (VEC == 4)
+        __builtin_amdgcn_raw_buffer_store_b128(u32x4{__float_as_uint(acc[0]), __float_as_uint(acc[1]), __float_as_uint(acc[2]), __float_as_uint(acc[3])},
+                                              far, at, 0, FAR);
+      else if constexpr (VEC == 2)
+        __builtin_amdgcn_raw_buffer_store_b64(u32x2{__float_as_uint(acc[0]), __float_as_uint(acc[1])}, far, at, 0, FAR);
+      else
+        __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(acc[0]), far, at, 0, FAR);
       if (d == 0) __builtin_amdgcn_raw_buffer_store_b64(u32x2{__float_as_uint(M), __float_as_uint(l)}, far, (h * PART_STRIDE + 128) * 4, 0, FAR);
     }
   }
@@ -640,7 +651,7 @@ __global__ __launch_bounds__(NTHREADS, GQA == 8 || !WHOLE ? 3 : 4) void attn_dec
   }
   __syncthreads();
   if (!last_lds) return;
-  merge4<GQA>(to, part - (int64_t)z * num_kv_heads * (GQA * PART_STRIDE), Z, num_kv_heads * (GQA * PART_STRIDE),
+  merge4<GQA, 8>(to, part - (int64_t)z * num_kv_heads * (GQA * PART_STRIDE), Z, num_kv_heads * (GQA * PART_STRIDE),
               reinterpret_cast<float(&)[NTHREADS][4]>(o_lds[0]), reinterpret_cast<float(&)[NTHREADS][2]>(o_lds[1]));
 }
 
@@ -653,7 +664,7 @@ __global__ __launch_bounds__(NTHREADS) void attn_decode4_merge_kernel(bf16_t* __
   const Deal mine = deal<true>(context_lens, B, kv_heads, limit, slots, b);
   const int Z = __builtin_amdgcn_readfirstlane(mine.shares);
   if (Z == 1) return;                      // its one workgroup has written the result
-  merge4<1>(out + ((int64_t)b * num_q_heads + h) * 128,
+  merge4<1, 16>(out + ((int64_t)b * num_q_heads + h) * 128,
             partials + ((int64_t)__builtin_amdgcn_readfirstlane(mine.start) * num_q_heads + h) * PART_STRIDE, Z, num_q_heads * PART_STRIDE,
             sums, ml);
 }

@@ -4,6 +4,9 @@
 // between its eight lanes. A workgroup has one head of KV4_TOKENS tokens: what it writes of the cache lies together, also the
 // scales, of which 16 positions share a line (with all heads of two tokens to a workgroup the parts of a line came from eight
 // L2s).
+//
+// What bounds them: memory, and beside it on the way in the vector units (290 instructions for 16 values). Measured, 8 heads, us in and
+// back out: 120 tokens 2.9, 2.7 (a launch); 7777 10.8, 10.7 (41 MB each); 30000 41.9, 28.4.
 
 #include "kv4.h"
 
