@@ -696,13 +696,14 @@ extern "C" void launch_attn_decode4(bf16_t* out, float* partials, int* arrived, 
                                     int max_blocks, int64_t q_stride, int B, hipStream_t stream) {
   const int gqa = num_q_heads / num_kv_heads;
   const int64_t limit = (int64_t)max_blocks * block_size;
-  const int slots = attn_decode4_slots(B, num_kv_heads, limit);
+  // more than B of at most DEAL_ROWS rows, which are one launch; else every row of a launch has one workgroup, whatever the others'
+  const int dealt = attn_decode4_slots(B, num_kv_heads, limit);
   // merged by the last workgroup, unless its work alone is more than a launch: heads times shares of a context
-  if ((int64_t)(slots / B) * gqa > 192) arrived = nullptr;
+  if ((int64_t)(dealt / B) * gqa > 192) arrived = nullptr;
   const uint32_t inverse = block_size > 1 ? (uint32_t)(((1ull << 32) + block_size - 1) / block_size) : ~0u;
   for (int b0 = 0; b0 < B; b0 += MAX_ROWS) {
-    const int rows = B - b0 < MAX_ROWS ? B - b0 : MAX_ROWS;
-    const dim3 grid(num_kv_heads, std::max(rows, slots));
+    const int rows = B - b0 < MAX_ROWS ? B - b0 : MAX_ROWS, slots = dealt > B ? dealt : rows;
+    const dim3 grid(num_kv_heads, slots);
     bf16_t* o = out + (int64_t)b0 * num_q_heads * 128;
     const bf16_t* q0 = q + (int64_t)b0 * q_stride;
     const int* bt = block_tables + (int64_t)b0 * max_blocks;
@@ -723,7 +724,7 @@ extern "C" void launch_attn_decode4(bf16_t* out, float* partials, int* arrived, 
     }
 #undef DISPATCH
 #undef LAUNCH
-    if (slots > B && !arrived)
+    if (slots > rows && !arrived)
       hipLaunchKernelGGL(attn_decode4_merge_kernel, dim3(num_q_heads, rows), dim3(NTHREADS), 0, stream, o, partials, context_lens + b0, limit,
                          rows, num_kv_heads, slots);
   }

@@ -429,3 +429,21 @@ def test_segments_replayed():
         g.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("B", [65535, 65536, 65839])              # one launch, a second of one row, a second of more rows than are dealt out
+def test_more_decode_rows_than_a_grid_has_in_y(B):
+    """A row for each token of long prompt portions, against the same rows in two calls: contexts of up to ten tiles, the
+    first rows' and the second launch's among them, of which fewer rows would be given several workgroups."""
+    q, kc, vc, ks, vs, tables, _ = case([640] * 8, 4, 1, 16, seed=31)
+    g = torch.Generator().manual_seed(B)
+    own = torch.randint(0, 8, (B,), generator=g)
+    n = torch.randint(0, 641, (B,), generator=g).int()
+    n[:4], n[-4:] = 640, 640
+    q = torch.randn(B, 4, D, generator=g).bfloat16()
+    q, kc, vc, ks, vs, tables, n = (t.to(DEV) for t in (q, kc, vc, ks, vs, tables[own], n))
+    call = lambda a, b: ops.attn_decode_paged(q[a:b], kc, vc, tables[a:b], n[a:b], 0.1, ks, vs)
+    out = call(0, B)
+    assert torch.equal(out, torch.cat([call(0, 40000), call(40000, B)]))
+    some = torch.tensor([0, 3, 255, 256, 65534, B - 1])
+    check([out[some]], *(t.cpu() for t in (q[some], kc, vc, ks, vs, tables[some], n[some])), 0.1)
