@@ -104,7 +104,8 @@ def store_kv(
     """k_scale/v_scale: [NB, KVH, BS] fp32 per-row dequant scales, REQUIRED
     when the caches are fp8 (written here: s = amax(|row|)/448), None for bf16.
     4-bit caches are uint8 [NB, KVH, BS, D / 2] with scales bf16 [NB, KVH, BS, D / 64, 2],
-    the steps and least values of groups of 64 values (torch_ref.kv4_quantize), written here too.
+    the steps and least values of groups of 64 values (torch_ref.kv4_quantize), written here too;
+    their rows of slots outside the cache go nowhere.
     Slots that are read later have to differ: two rows of one slot leave a mixture of both."""
     _check_kv4(k_cache, k_scale, v_scale)
     if k.is_cuda and not _force_torch():
@@ -134,7 +135,8 @@ def load_kv(k_cache, v_cache, slots, k_scale, v_scale) -> Tuple[torch.Tensor, to
 
 
 def rope_store(q, k, v, positions, cos_sin, k_cache, v_cache, slot_mapping, k_scale=None, v_scale=None) -> None:
-    """rope_inplace(q, k) and store_kv(k, v): one launch for aligned rows of head size 128, else the two."""
+    """rope_inplace(q, k) and store_kv(k, v): one launch for aligned rows of head size 128, else the two. A 4-bit cache's
+    slots may lie outside it: those rows are turned and go nowhere."""
     _check_kv4(k_cache, k_scale, v_scale)
     if (q.is_cuda and not _force_torch() and q.dtype == k.dtype == v.dtype == torch.bfloat16
             and q.shape[2] == 128 and k.stride(0) == v.stride(0)
@@ -639,7 +641,8 @@ def add_norm_rows_int8(part, residual, weight, eps) -> Int8Rows:
 
 
 def rope_store_rows(part, bias, num_heads, positions, cos_sin, k_cache, v_cache, slot_mapping, k_scale=None, v_scale=None):
-    """Rotates q and k of the fused qkv sums, stores k and v into the paged cache; returns q [M, H, 128]."""
+    """Rotates q and k of the fused qkv sums, stores k and v into the paged cache (rows of slots outside a 4-bit one go
+    nowhere); returns q [M, H, 128]."""
     f = _none(part, torch.float32)
     return _hip_or_raise().rope_store_rows(
         part, bias if bias is not None else _none(part, torch.bfloat16), num_heads,

@@ -260,7 +260,7 @@ void store_kv(torch::Tensor k, torch::Tensor v, torch::Tensor k_cache, torch::Te
 extern "C" void launch_rope_store(bf16_t* q, bf16_t* k, const bf16_t* v, const int64_t* positions,
                                   const float* cos_sin, void* k_cache, void* v_cache, void* k_scale, void* v_scale,
                                   const int64_t* slots, int T, int H, int G, int q_stride, int kv_stride,
-                                  int block_size, int kind, hipStream_t stream);
+                                  int block_size, int64_t held, int kind, hipStream_t stream);
 
 // rope_inplace and store_kv of rows of head size 128 in one launch; views of 16-byte aligned rows
 void rope_store(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor positions, torch::Tensor cos_sin,
@@ -289,7 +289,7 @@ void rope_store(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor
   launch_rope_store(bf(q), bf(k), cbf(v), positions.data_ptr<int64_t>(), cos_sin.data_ptr<float>(), k_cache.data_ptr(),
                     v_cache.data_ptr(), kind ? k_scale.data_ptr() : nullptr,
                     kind ? v_scale.data_ptr() : nullptr, slots.data_ptr<int64_t>(), T, H, G, (int)q.stride(0),
-                    (int)k.stride(0), BS, kind, cur_stream());
+                    (int)k.stride(0), BS, k_cache.size(0) * BS, kind, cur_stream());
 }
 
 // mask_size: -1 for plain decode rows, from 0 (plain causal) on for those of a block-local layer
@@ -858,7 +858,7 @@ extern "C" void launch_add_norm_rows(bf16_t* out, bf16_t* residual, const float*
 extern "C" void launch_rope_store_rows(bf16_t* q_out, const float* part, const bf16_t* bias, const int64_t* positions,
                                        const float* cos_sin, void* k_cache, void* v_cache, void* k_scale,
                                        void* v_scale, const int64_t* slots, int S, int M, int H, int G,
-                                       int block_size, int kind, hipStream_t stream);
+                                       int block_size, int64_t held, int kind, hipStream_t stream);
 extern "C" void launch_decode_inputs(int64_t* ids, int64_t* positions, int64_t* slots, int* ctx, int* tables,
                                      const int64_t* ids_in, const int64_t* positions_in, const int64_t* slots_in,
                                      const int* ctx_in, const int* tables_in, int B, int bs, int nb, int mb,
@@ -938,7 +938,7 @@ torch::Tensor rope_store_rows(torch::Tensor part, torch::Tensor bias, int64_t H,
                          positions.data_ptr<int64_t>(), cos_sin.data_ptr<float>(), k_cache.data_ptr(),
                          v_cache.data_ptr(), kind ? k_scale.data_ptr() : nullptr,
                          kind ? v_scale.data_ptr() : nullptr, slots.data_ptr<int64_t>(), S, M, (int)H, G, BS,
-                         kind, cur_stream());
+                         k_cache.size(0) * BS, kind, cur_stream());
   return q;
 }
 

@@ -175,13 +175,14 @@ extern "C" void launch_add_norm_rows(bf16_t* out, bf16_t* residual, const float*
 
 // qkv sums [S, M, (H + 2G) * 128] (+ bias): q and k rotated (entry i with i + 64), q
 // out as bf16 rows, k and v into the paged cache - as bf16, as e4m3 with a scale
-// per row (amax / 448 of the bf16 row), or in 4 bits (kv4.h). A wave per (row, head), two dims a lane.
+// per row (amax / 448 of the bf16 row), or in 4 bits (kv4.h; rows of slots outside the ``held`` positions go nowhere). A wave
+// per (row, head), two dims a lane.
 template <int KIND>
 __global__ void __launch_bounds__(256) rope_store_rows_kernel(
     bf16_t* __restrict__ q_out, const float* __restrict__ part, const bf16_t* __restrict__ bias,
     const int64_t* __restrict__ positions, const float* __restrict__ cos_sin, void* __restrict__ k_cache,
     void* __restrict__ v_cache, void* __restrict__ k_scale, void* __restrict__ v_scale,
-    const int64_t* __restrict__ slots, int S, int M, int H, int G, int block_size) {
+    const int64_t* __restrict__ slots, int S, int M, int H, int G, int block_size, int64_t held) {
   const int m = blockIdx.y;
   const int lane = threadIdx.x & 63;
   const int head = blockIdx.x * 4 + (threadIdx.x >> 6);
@@ -223,6 +224,7 @@ __global__ void __launch_bounds__(256) rope_store_rows_kernel(
   }
   const bool is_k = head < H + G;
   const int g = head - H - (is_k ? 0 : G);
+  if (KIND == CACHE_KV4 && (slot < 0 || slot >= held)) return;
   const int64_t row = ((slot / block_size) * G + g) * block_size + slot % block_size;
   if constexpr (KIND == CACHE_KV4) {
     // the halves of a row are its groups; word n is of the lanes n, n + 16, n + 32, n + 48
@@ -252,12 +254,12 @@ __global__ void __launch_bounds__(256) rope_store_rows_kernel(
 extern "C" void launch_rope_store_rows(bf16_t* q_out, const float* part, const bf16_t* bias, const int64_t* positions,
                                        const float* cos_sin, void* k_cache, void* v_cache, void* k_scale,
                                        void* v_scale, const int64_t* slots, int S, int M, int H, int G,
-                                       int block_size, int kind, hipStream_t stream) {
+                                       int block_size, int64_t held, int kind, hipStream_t stream) {
   hipLaunchKernelGGL(kind == CACHE_KV4   ? rope_store_rows_kernel<CACHE_KV4>
                      : kind == CACHE_FP8 ? rope_store_rows_kernel<CACHE_FP8>
                                          : rope_store_rows_kernel<CACHE_BF16>,
                      dim3((H + 2 * G + 3) / 4, M), dim3(256), 0, stream, q_out, part, bias, positions, cos_sin, k_cache, v_cache,
-                     k_scale, v_scale, slots, S, M, H, G, block_size);
+                     k_scale, v_scale, slots, S, M, H, G, block_size, held);
 }
 
 // Inputs of a captured decode step, in one launch (twelve copies and fills otherwise):

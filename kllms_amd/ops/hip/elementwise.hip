@@ -221,14 +221,14 @@ extern "C" __global__ void __launch_bounds__(256) store_kv_fp8_kernel(
 // e4m3 with a scale per row (as store_kv_fp8_kernel) or in 4 bits (kv4.h). A thread holds entries c..c+7 and
 // c+64..c+71 of a head: 16-byte accesses throughout, where a rotation of 2-byte accesses
 // with a workgroup per head and the store behind it took 132 us for 12000 rows of 48
-// heads and this takes 50 (320 MB, 6.4 TB/s).
+// heads and this takes 50 (320 MB, 6.4 TB/s). held: positions of the cache
 // --------------------------------------------------------------------------
 template <int KIND>
 __global__ void __launch_bounds__(256) rope_store_kernel(
     bf16_t* __restrict__ q, bf16_t* __restrict__ k, const bf16_t* __restrict__ v,
     const int64_t* __restrict__ positions, const float* __restrict__ cos_sin, void* __restrict__ k_cache,
     void* __restrict__ v_cache, void* __restrict__ k_scale, void* __restrict__ v_scale,
-    const int64_t* __restrict__ slots, int64_t n, int H, int G, int q_stride, int kv_stride, int block_size) {
+    const int64_t* __restrict__ slots, int64_t n, int H, int G, int q_stride, int kv_stride, int block_size, int64_t held) {
   const int heads = H + 2 * G;
   for (int64_t idx = (int64_t)blockIdx.x * 256 + threadIdx.x; idx < n; idx += (int64_t)gridDim.x * 256) {
     const int piece = (int)(idx & 7);
@@ -257,6 +257,7 @@ __global__ void __launch_bounds__(256) rope_store_kernel(
     if (is_q) continue;
     const int g = head - H - (is_v ? G : 0);
     const int64_t slot = slots[t];
+    if (KIND == CACHE_KV4 && (slot < 0 || slot >= held)) continue;       // nobody's, as in kv4_store_kernel; a row's eight lanes as one
     const int64_t at = ((slot / block_size) * G + g) * block_size + slot % block_size;
     if constexpr (KIND == CACHE_KV4) {
       kv4_store_row((uint32_t*)(is_v ? v_cache : k_cache) + at * (KV4_BYTES / 4), (uint32_t*)(is_v ? v_scale : k_scale) + at * KV4_GROUPS,
@@ -290,7 +291,7 @@ __global__ void __launch_bounds__(256) rope_store_kernel(
 extern "C" void launch_rope_store(bf16_t* q, bf16_t* k, const bf16_t* v, const int64_t* positions,
                                   const float* cos_sin, void* k_cache, void* v_cache, void* k_scale, void* v_scale,
                                   const int64_t* slots, int T, int H, int G, int q_stride, int kv_stride,
-                                  int block_size, int kind, hipStream_t stream) {
+                                  int block_size, int64_t held, int kind, hipStream_t stream) {
   const int64_t n = (int64_t)T * (H + 2 * G) * 8;
   const int64_t blocks = (n + 255) / 256;
   const dim3 grid((unsigned)(blocks < 16384 ? blocks : 16384));
@@ -298,5 +299,5 @@ extern "C" void launch_rope_store(bf16_t* q, bf16_t* k, const bf16_t* v, const i
                      : kind == CACHE_FP8 ? rope_store_kernel<CACHE_FP8>
                                          : rope_store_kernel<CACHE_BF16>,
                      grid, dim3(256), 0, stream, q, k, v, positions, cos_sin, k_cache, v_cache, k_scale, v_scale, slots, n, H, G,
-                     q_stride, kv_stride, block_size);
+                     q_stride, kv_stride, block_size, held);
 }

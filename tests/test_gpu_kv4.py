@@ -447,3 +447,35 @@ def test_more_decode_rows_than_a_grid_has_in_y(B):
     assert torch.equal(out, torch.cat([call(0, 40000), call(40000, B)]))
     some = torch.tensor([0, 3, 255, 256, 65534, B - 1])
     check([out[some]], *(t.cpu() for t in (q[some], kc, vc, ks, vs, tables[some], n[some])), 0.1)
+
+
+def test_turned_rows_for_no_slot_go_nowhere():
+    """rope_store of aligned rows, of rows off 16 bytes and of a decode step's sums: a slot in front of the cache, the first one
+    behind it and far ones. Rows of other memory lie on both sides, so that what went there would be seen."""
+    T, H, G, BS, NB, off = 7, 4, 2, 4, 3, 2
+    inside, slots = torch.tensor([0, 3, 6]), torch.tensor([2, -1, NB * BS, 7, -BS, 1 << 40, NB * BS - 1], device=DEV)
+    qkv = rows(T, H + 2 * G, D, seed=33).to(DEV)
+    pos = torch.zeros(T, dtype=torch.long, device=DEV)           # where turning rounds nothing: all forms have the same rows
+    cos_sin = torch_ref.build_cos_sin_cache(D, 64, 1e4, "cpu").to(DEV)
+    shapes = [(G, BS, D // 2), (G, BS, D // 2), (G, BS, 2, 2), (G, BS, 2, 2)]
+
+    def caches():                                 # blocks off.. off + NB of larger ones
+        big = [torch.zeros(NB + 2 * off, *s, dtype=torch.uint8 if len(s) == 3 else torch.bfloat16, device=DEV) for s in shapes]
+        return big, [t[off:off + NB] for t in big]
+
+    odd = torch.empty(qkv.numel() + 1, dtype=torch.bfloat16, device=DEV)[1:].view(qkv.shape)
+    stored = []
+    for rows_at in (torch.empty_like(qkv), odd):
+        rows_at.copy_(qkv)
+        big, c = caches()
+        ops.rope_store(*rows_at.split([H, G, G], 1), pos, cos_sin, c[0], c[1], slots, c[2], c[3])
+        stored.append((big, c, rows_at.clone()))
+    big, c = caches()
+    got = ops.rope_store_rows(qkv.view(1, T, -1).float().contiguous(), None, H, pos, cos_sin, c[0], c[1], slots, c[2], c[3])
+    stored.append((big, c, torch.cat((got, stored[0][2][:, H:]), 1)))
+    for big, c, turned in stored:
+        assert torch.equal(turned, stored[0][2])                  # of all rows
+        want = [torch.zeros(NB + 2 * off, *s, dtype=t.dtype) for s, t in zip(shapes, big)]
+        inner = [t[off:off + NB] for t in want]
+        torch_ref.store_kv(turned[:, H:H + G].cpu()[inside], turned[:, H + G:].cpu()[inside], inner[0], inner[1], slots.cpu()[inside], inner[2], inner[3])
+        assert all(torch.equal(t.cpu().float(), w.float()) for t, w in zip(big, want))
