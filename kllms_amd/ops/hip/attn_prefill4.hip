@@ -5,9 +5,10 @@
 //     each tile and head. So the keys are made once for all heads, and a short tail still has eight waves at work
 //   - 128 keys at a time: each thread has a quarter of a K row and of a V row on their way in registers, makes fp16 of them
 //     and puts them to LDS, double-buffered, while the stage before is multiplied
-//   - fp16 holds what the cache stands for to 2^-12 (with K in bf16 the result is three times further off than its own
-//     rounding makes it, behind 9000 keys). 16 keys that a wave makes have a power of 2^16 taken out, such that their largest is between
-//     2^-4 and 2^13: none, in a model, and then nothing is multiplied back. q's rows are scaled into fp16's range exactly
+//   - fp16 holds what the cache stands for to 2^-11 (with K in bf16 the result is three times further off than its own
+//     rounding makes it, behind 9000 keys). Of a group whose largest is not between 2^-10 and 2^14 a power of 2^16 is taken out that
+//     brings it there: none, in a model, and then nothing is multiplied back. Each group has its own: with one for both of a row, values 2^-20
+//     of the other group's were up to 16 % off. q's rows are scaled into fp16's range exactly
 //   - scores and softmax as in attn_prefill.hip: S = K Q^T, a lane has one row's scores, base-2 exponentials of one fma, the
 //     running max renewed when it grows by more than 8; P is fp16 in one part, 2^-12 of it, where bf16 would need two
 //   - few or long groups are cut along the keys (the plan says where); their sums meet in a second launch
@@ -41,7 +42,7 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 #define STAGE 128                  // keys staged per barrier round
 #define NWAVES 8
 #define STAGE_BYTES (STAGE * 256)  // K or V of a stage
-#define CLASSES (2 * STAGE)        // bytes of a stage's: K's and V's of each key
+#define CLASSES (4 * STAGE)        // bytes of a stage's: of K's and V's groups of each key
 #define LDS_BYTES (4 * STAGE_BYTES + 2 * CLASSES + 2 * NWAVES)
 #define PART_STRIDE 132            // of a row and head's partial: 128 sums, max, sum of exponentials
 #define PART_ROWS (NWAVES * QBLK)  // rows and heads of an item and kv head
@@ -61,29 +62,28 @@ struct Item {
   int row, len, r0, seg, from, to, part, unused;
 };
 
-// A row's class: the power of 2^16 that is taken out of it, after the largest exponent of a group's least value and step. A
-// group that is no number does not count.
-__device__ __forceinline__ int row_class(const u32x2& scales) {
-  int e = 0;
-#pragma unroll
-  for (int g = 0; g < 2; ++g) {
-    const int l = (int)(scales[g] >> 23 & 0xff), s = (int)(scales[g] >> 7 & 0xff);
-    e = max(e, l == 255 || s == 255 ? 0 : max(l, s ? s + 4 : 0));        // all values are below 2^(e - 127 + 2)
-  }
-  if (e == 0) return 0;
+// A group's class: the power of 2^16 that is taken out of it, after the largest exponent of its least value and step. A
+// group of zeros or that is no number has none.
+__device__ __forceinline__ int group_exponent(uint32_t w) {
+  const int l = (int)(w >> 23 & 0xff), s = (int)(w >> 7 & 0xff);
+  return l == 255 || s == 255 ? 0 : max(l, s ? s + 4 : 0);        // all values are below 2^(e - 127 + 2)
+}
+__device__ __forceinline__ bool has_no_class(int e) { return e == 0 || (e >= 117 && e <= 139); }
+__device__ __forceinline__ int class_of_exponent(int e) {
+  if (has_no_class(e)) return 0;
   e -= 127;
-  return e > 12 ? (e - 13 >> 4) + 1 : e < -10 ? max(-(-11 - e >> 4) - 1, -7) : 0;
+  return e > 12 ? (e - 13 >> 4) + 1 : max(-(-11 - e >> 4) - 1, -7);
 }
 
-// Four words of a row (32 values) to fp16: put(p, two words) takes those of nibble p, four neighbouring values
+// Four words of a row (32 values) to fp16, step and least value of each group: put(p, two words) takes those of nibble p, four
+// neighbouring values
 template <class P>
-__device__ __forceinline__ void kv4_to_f16(const u32x4& w, const u32x2& scales, float down, P put) {
+__device__ __forceinline__ void kv4_to_f16(const u32x4& w, const f32x2 (&scales)[2], P put) {
   f16x2 step[2], least[2];
 #pragma unroll
   for (int g = 0; g < 2; ++g) {
-    const float s = kv4_step(scales[g]) * down, l = kv4_least(scales[g]) * down;
-    step[g] = as_f16(pack_f16(s, s));
-    least[g] = as_f16(pack_f16(l, l));
+    step[g] = as_f16(pack_f16(scales[g][0], scales[g][0]));
+    least[g] = as_f16(pack_f16(scales[g][1], scales[g][1]));
   }
   const f16x2 base = as_f16(0x64006400u);
   uint32_t mask = 0x000f000fu, magic = 0x64006400u;
@@ -129,7 +129,7 @@ __global__ void __launch_bounds__(64 * NWAVES) attn_prefill4_kernel(
   const int end_grp = (int)min((int64_t)min(it.to, pos0 + rows_end), held);
   const int end_me = active ? min(end_grp, pos0 + min(rows_end, qrow0 + QBLK)) : 0;
 
-  extern __shared__ __attribute__((aligned(1024))) char smem[];          // [buffer][K | V], classes [buffer][key][K, V], [buffer][wave] has any
+  extern __shared__ __attribute__((aligned(1024))) char smem[];          // [buffer][K | V], classes [buffer][key][K's groups, V's], [buffer][wave] has any
   signed char* const classes = (signed char*)smem + 4 * STAGE_BYTES;
   signed char* const has_class = classes + 2 * CLASSES;
 
@@ -183,25 +183,42 @@ __global__ void __launch_bounds__(64 * NWAVES) attn_prefill4_kernel(
     vsc = *reinterpret_cast<const u32x2*>(v_scale + row * KV4_GROUPS);
   };
   auto stage = [&](int buf) {
-    const int kc = row_class(ksc), vc = row_class(vsc);
+    // each of a row's four threads looks at one of its groups
+    const uint32_t mine = st_part & 2 ? (st_part & 1 ? vsc[1] : vsc[0]) : (st_part & 1 ? ksc[1] : ksc[0]);
+    const int e = group_exponent(mine);
+    const bool any = __any(!has_no_class(e));
     // a V row that is no number: its key is made none, so that the rows that see it are none and the others do not meet it
     if (kv4_least(vsc[0]) != kv4_least(vsc[0]) || kv4_least(vsc[1]) != kv4_least(vsc[1]) || kv4_step(vsc[0]) != kv4_step(vsc[0]) ||
         kv4_step(vsc[1]) != kv4_step(vsc[1])) {
       ksc = u32x2{0x7fc07fc0u, 0x7fc07fc0u};
       vsc = u32x2{0u, 0u};
     }
+    f32x2 k_by[2], v_by[2];
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+      k_by[g] = f32x2{kv4_step(ksc[g]), kv4_least(ksc[g])};
+      v_by[g] = f32x2{kv4_step(vsc[g]), kv4_least(vsc[g])};
+    }
+    if (any) {
+      const int c = class_of_exponent(e);
+      classes[buf * CLASSES + st_row * 4 + st_part] = (signed char)c;
+      const float down = ldexpf(1.0f, -16 * c);
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+        k_by[g] *= __shfl(down, (lane & ~3) + g);
+        v_by[g] *= __shfl(down, (lane & ~3) + 2 + g);
+      }
+    }
     char* const k_to = smem + buf * 2 * STAGE_BYTES + st_row * 256;
     char* const v_to = k_to + STAGE_BYTES;
     // nibble p of words 4 part..: values 32 (p & 3) + 16 (p >> 2) + 4 part..
-    kv4_to_f16(kr, ksc, ldexpf(1.0f, -16 * kc), [&](int p, const u32x2& v) {
+    kv4_to_f16(kr, k_by, [&](int p, const u32x2& v) {
       const int unit = 4 * (p & 3) + 2 * (p >> 2) + (st_part >> 1);
       *reinterpret_cast<u32x2*>(k_to + ((unit ^ (st_row & 15)) << 4) + (st_part & 1) * 8) = v;
     });
-    kv4_to_f16(vr, vsc, ldexpf(1.0f, -16 * vc), [&](int p, const u32x2& v) {
+    kv4_to_f16(vr, v_by, [&](int p, const u32x2& v) {
       *reinterpret_cast<u32x2*>(v_to + (((2 * (p & 3) + (p >> 2)) ^ v_turn(st_row)) << 5) + st_part * 8) = v;
     });
-    const bool any = __any(kc != 0 || vc != 0);
-    if (any && st_part == 0) *reinterpret_cast<short*>(classes + buf * CLASSES + st_row * 2) = (short)((kc & 0xff) | vc << 8);
     if (lane == 0) has_class[buf * NWAVES + wave] = any;
   };
 
@@ -213,7 +230,7 @@ __global__ void __launch_bounds__(64 * NWAVES) attn_prefill4_kernel(
   // elements of 16)
   uint32_t k_get = lds0 + col * 256 + ((half ^ (col & 15)) << 4);
   uint32_t v_get = lds0 + STAGE_BYTES + (half * 8 + ((lane & 15) >> 2)) * 256 + ((((lane & 15) >> 2) * 2 ^ (lane >> 4 & 1)) << 5) + (lane & 3) * 8;
-  // All of the item, up to a stage that has a row of another class than 0 (false); ANY: with such rows too. (As branches of one loop
+  // All of the item, up to a stage that has a group of another class than 0 (false); ANY: with such groups too. (As branches of one loop
   // they had all sums copied twice a tile: one of 2100 rows behind 7777 431 us.)
   auto run = [&](auto any_class) {
   constexpr bool ANY = decltype(any_class)::value;
@@ -228,21 +245,30 @@ __global__ void __launch_bounds__(64 * NWAVES) attn_prefill4_kernel(
     asm volatile("" : "+v"(half_now));
     auto class_of = [&](int sub, int r, int of) {
       const int key = kt - ks + sub * 32 + acc_row(r, half_now);
-      return has_class[buf * NWAVES + (key >> 4)] ? (int)classes[buf * CLASSES + key * 2 + of] : 0;
+      return has_class[buf * NWAVES + (key >> 4)] ? (int)classes[buf * CLASSES + key * 4 + of] : 0;
     };
     // ---- QK^T: S[key][qrow], 32 keys each ----------------------------
     f32x16 s_acc[2] = {};
     const uint32_t k_at = k_get + at;
-#pragma unroll
-    for (int s = 0; s < 8; ++s)
-#pragma unroll
-      for (int sub = 0; sub < 2; ++sub)    // row col + 32 sub has the same XOR
-        s_acc[sub] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*(lds_frag)(uintptr_t)((k_at ^ (s << 5)) + sub * 32 * 256), q_frag[s].m, s_acc[sub], 0, 0, 0);
-    if constexpr (ANY) if (!plain) {
+    auto multiply_k = [&](int s, int sub, f32x16& acc) {         // row col + 32 sub has the same XOR
+      acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(*(lds_frag)(uintptr_t)((k_at ^ (s << 5)) + sub * 32 * 256), q_frag[s].m, acc, 0, 0, 0);
+    };
+    if (!plain) {                          // a group at a time, its powers put back
 #pragma unroll
       for (int sub = 0; sub < 2; ++sub)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s_acc[sub][r] = ldexpf(s_acc[sub][r], 16 * class_of(sub, r, 0));
+        for (int g = 0; g < 2; ++g) {
+          f32x16 acc = {};
+#pragma unroll
+          for (int s = 4 * g; s < 4 * g + 4; ++s) multiply_k(s, sub, acc);
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s_acc[sub][r] += ldexpf(acc[r], 16 * class_of(sub, r, g));
+        }
+    } else {
+#pragma unroll
+      for (int s = 0; s < 8; ++s)
+#pragma unroll
+        for (int sub = 0; sub < 2; ++sub) multiply_k(s, sub, s_acc[sub]);
     }
     if (kt + 64 > pos0 + qrow0 || kt + 64 > end_grp) {
       // rows see keys up to their own position, which also ends the segment
@@ -356,7 +382,7 @@ __global__ void __launch_bounds__(64 * NWAVES) attn_prefill4_kernel(
 #pragma unroll
               for (int e = 0; e < 2; ++e) {
                 const int key = kt - ks + sub * 32 + kw * 16 + half_now * 8 + 2 * j + e;
-                x[e] = ldexpf((float)h2[e], has_class[buf * NWAVES + (key >> 4)] ? 16 * classes[buf * CLASSES + key * 2 + 1] : 0);
+                x[e] = ldexpf((float)h2[e], has_class[buf * NWAVES + (key >> 4)] ? 16 * classes[buf * CLASSES + key * 4 + 2 + (dt >> 1)] : 0);
               }
               v1.u[j] = __builtin_bit_cast(uint32_t, __builtin_convertvector(x, bf16x2_t));
               x[0] -= __uint_as_float(v1.u[j] << 16);

@@ -6,7 +6,7 @@ import torch
 from kllms_amd import ops
 from kllms_amd.ops import torch_ref
 
-from kv4_oracle import attention64, values64
+from kv4_oracle import attention64, prompts64, values64
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -479,3 +479,69 @@ def test_turned_rows_for_no_slot_go_nowhere():
         inner = [t[off:off + NB] for t in want]
         torch_ref.store_kv(turned[:, H:H + G].cpu()[inside], turned[:, H + G:].cpu()[inside], inner[0], inner[1], slots.cpu()[inside], inner[2], inner[3])
         assert all(torch.equal(t.cpu().float(), w.float()) for t, w in zip(big, want))
+
+
+def grouped(x, sizes):
+    """Rows [..., 128] with values 0..63 and 64..127 in sizes of their own [..., 2]."""
+    return (x.float().unflatten(-1, (2, 64)) * sizes[..., None]).flatten(-2).bfloat16()
+
+
+def check_prompts(out, q, kc, vc, ks, vs, tables, n, scale):
+    want, off = prompts64(q, kc, vc, ks, vs, tables, n, scale)
+    far = (out.double().cpu() - want).abs()
+    assert bool((far <= off).all()), f"{float((far / off).max())} of what is allowed, at {torch.nonzero(far > off)[:3].tolist()}"
+
+
+def restore(cache, scales, table, at, x):
+    BS = cache.shape[2]
+    blk, off = table.long()[at // BS], at % BS
+    cache[blk, :, off], scales[blk, :, off] = torch_ref.kv4_quantize(x)
+
+
+@pytest.mark.parametrize("gqa,KVH", [(4, 2), (1, 1), (8, 1)])
+@pytest.mark.parametrize("segs", [[(200, 70), (0, 40)], [(2500, 40)]])
+@pytest.mark.parametrize("low", [-9, -16, -20, -24, -60])
+def test_segments_whose_groups_differ_in_size(segs, gqa, KVH, low):
+    """Values 64..127 of keys and values 2^low of the others; what q has there is as much larger (up to 2^20), so that both groups
+    say which keys count."""
+    q, kc, vc, ks, vs, seg_tables, start, tables, lens = segments(segs, gqa, KVH, 16, seed=low + 100)
+    sizes = torch.tensor([1.0, 2.0 ** low])
+    for i, (p, r) in enumerate(segs):
+        at = torch.arange(p + r)
+        restore(kc, ks, seg_tables[i], at, grouped(rows(p + r, KVH, D, seed=i + 40), sizes))
+        restore(vc, vs, seg_tables[i], at, grouped(rows(p + r, KVH, D, seed=i + 50), sizes))
+    q = grouped(q, torch.tensor([1.0, 2.0 ** min(-low, 20)]))
+    out = attend(q, kc, vc, ks, vs, seg_tables, start, tables, lens, D ** -0.5, segs)
+    check_prompts(out, q, kc, vc, ks, vs, tables, lens, D ** -0.5)
+
+
+@pytest.mark.parametrize("gqa", [1, 4])
+def test_segments_whose_groups_have_any_size(gqa):
+    segs = [(300, 70), (10, 40), (2100, 12)]
+    q, kc, vc, ks, vs, seg_tables, start, tables, lens = segments(segs, gqa, 2, 16, seed=71)
+    g = torch.Generator().manual_seed(72)
+    for i, (p, r) in enumerate(segs):
+        for cache, scales, spread in ((kc, ks, 5.0), (vc, vs, 15.0)):
+            x = grouped(rows(p + r, 2, D, seed=i + 60), torch.exp2(torch.randn(p + r, 2, 2, generator=g) * spread))
+            restore(cache, scales, seg_tables[i], torch.arange(p + r), x)
+    scale = 2.0 ** -18
+    check_prompts(attend(q, kc, vc, ks, vs, seg_tables, start, tables, lens, scale, segs), q, kc, vc, ks, vs, tables, lens, scale)
+
+
+def test_one_group_of_another_size_in_a_cut_segment():
+    """One key's and another's value's second group, in one of the items of a segment: the others go on as they were."""
+    segs = [(2500, 40)]
+    q, kc, vc, ks, vs, seg_tables, start, tables, lens = segments(segs, 4, 2, 16, seed=73)
+    for cache, scales, at, size in ((kc, ks, 1300, 2.0 ** 18), (vc, vs, 1301, 2.0 ** -40), (vc, vs, 77, 2.0 ** 30)):
+        restore(cache, scales, seg_tables[0], torch.tensor([at]), grouped(rows(1, 2, D, seed=at), torch.tensor([1.0, size])))
+    q = grouped(q, torch.tensor([1.0, 2.0 ** -16]))
+    assert ops.kv4_plan(segs, 8, 2, DEV)[0].parts > 1
+    out = attend(q, kc, vc, ks, vs, seg_tables, start, tables, lens, 0.1, segs)
+    check_prompts(out, q, kc, vc, ks, vs, tables, lens, 0.1)
+
+
+@pytest.mark.parametrize("segs", SEGMENTS)
+def test_segments_are_as_far_off_as_their_roundings(segs):
+    q, kc, vc, ks, vs, seg_tables, start, tables, lens = segments(segs, 4, 2, 16, seed=74)
+    out = attend(q, kc, vc, ks, vs, seg_tables, start, tables, lens, D ** -0.5, segs)
+    check_prompts(out, q, kc, vc, ks, vs, tables, lens, D ** -0.5)
