@@ -258,7 +258,8 @@ class Kv4Groups(NamedTuple):
     """Groups of a segment's rows that attend over the 4-bit cache together: ``items`` int32 [n, 8] (first packed row and rows of
     the segment, first row of the group, segment, first and last key, where its sums go, 0) and ``cuts`` [m, 4] (first packed
     row, rows, first part, parts) of groups whose keys are cut into ``parts`` altogether; of ``rows`` packed rows in ``segments``
-    segments, with ``heads`` heads to a kv head."""
+    segments, with ``heads`` heads to a kv head. A group's last item goes on to whatever its rows see: the starts that the plan was
+    made of say how the work is shared, not which keys there are."""
     items: torch.Tensor
     cuts: torch.Tensor
     parts: int
@@ -312,19 +313,20 @@ def kv4_plan(segs, heads: int, kv_heads: int, device, least: int = 1) -> tuple:
     if not groups:
         return None, short
     most = _kv4_cuts([g[4] for g in groups], kv_heads)
-    items, cuts, parts = [], [], 0
+    items, cuts, parts, last = [], [], 0, (1 << 31) - 1
     for row, n, r, i, keys in groups:
         pieces = -(-keys // most)
         if pieces == 1:
-            items.append((row, n, r, i, 0, keys, -1, 0))
+            items.append((keys, (row, n, r, i, 0, last, -1, 0)))
             continue
         each = -(-keys // (pieces * 128)) * 128
         pieces = -(-keys // each)
         cuts.append((row + r, min(n - r, rows), parts, pieces))
-        items.extend((row, n, r, i, e * each, min(keys, (e + 1) * each), parts + e, 0) for e in range(pieces))
+        items.extend((min(keys - e * each, each), (row, n, r, i, e * each, (e + 1) * each if e + 1 < pieces else last, parts + e, 0))
+                     for e in range(pieces))
         parts += pieces
-    items.sort(key=lambda g: g[4] - g[5])                # longest first
-    flat = upload(torch.tensor([x for g in items for x in g] + [x for c in cuts for x in c], dtype=torch.int32), device)
+    items.sort(key=lambda g: -g[0])                      # longest first
+    flat = upload(torch.tensor([x for _, g in items for x in g] + [x for c in cuts for x in c], dtype=torch.int32), device)
     return Kv4Groups(flat[:8 * len(items)].view(-1, 8), flat[8 * len(items):].view(-1, 4), parts, sum(n for _, n in segs), len(segs),
                      heads // kv_heads), short
 

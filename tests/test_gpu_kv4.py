@@ -545,3 +545,13 @@ def test_segments_are_as_far_off_as_their_roundings(segs):
     q, kc, vc, ks, vs, seg_tables, start, tables, lens = segments(segs, 4, 2, 16, seed=74)
     out = attend(q, kc, vc, ks, vs, seg_tables, start, tables, lens, D ** -0.5, segs)
     check_prompts(out, q, kc, vc, ks, vs, tables, lens, D ** -0.5)
+
+
+@pytest.mark.parametrize("planned", [[(2500, 40), (100, 33)], [(0, 40), (4000, 33)], [(1300, 40), (0, 33)]])
+def test_segments_at_other_starts_than_the_plans(planned):
+    """The starts on the device say which keys a row sees: more than the plan was made of, fewer, or none of a cut piece."""
+    segs = [(1300, 40), (700, 33)]
+    q, kc, vc, ks, vs, seg_tables, start, tables, lens = segments(segs, 4, 2, 16, seed=75)
+    plan = ops.kv4_plan(planned, 8, 2, DEV)
+    out = attend(q, kc, vc, ks, vs, seg_tables, start, tables, lens, 0.1, segs, plan)
+    check_prompts(out, q, kc, vc, ks, vs, tables, lens, 0.1)
