@@ -346,11 +346,13 @@ def paged_plan(segs, heads: int, kv_heads: int, device, cache_dtype=torch.bfloat
 def attn_segments_paged(q, k_cache, v_cache, block_tables, context_lens, scale, plan, short, seg_tables, seg_start,
                         k_scale=None, v_scale=None):
     """Rows of long segments on the matrix cores against the paged bf16 or 4-bit cache, the others row by row (GPU only).
-    ``plan`` and ``short``: of paged_plan for this cache's type. A 4-bit value row that is no number makes the rows that
+    ``plan`` and ``short``: of paged_plan for this cache's type and as many rows as q has. A 4-bit value row that is no number makes the rows that
     attend together and see it none as a whole."""
     _check_kv4(k_cache, k_scale, v_scale)
+    if plan is None and q.shape[0] != sum(n for _, n in short):
+        raise ValueError(f"rows {short} (first, how many) that attend row by row, and no others: got q {list(q.shape)}")
     if k_cache.dtype == torch.uint8 and plan is not None and (
-            q.shape[0] < plan.rows or seg_tables.shape[0] < plan.segments or q.shape[1] != plan.heads * k_cache.shape[1]):
+            q.shape[0] != plan.rows or seg_tables.shape[0] < plan.segments or q.shape[1] != plan.heads * k_cache.shape[1]):
         raise ValueError(f"a plan of {plan.rows} rows in {plan.segments} segments with {plan.heads} heads to a kv head: got q {list(q.shape)}, "
                          f"tables {list(seg_tables.shape)}, {k_cache.shape[1]} kv heads")
     out = torch.empty(q.shape, dtype=q.dtype, device=q.device)

@@ -189,3 +189,17 @@ def test_a_plan_of_other_rows_is_refused():
                        seg_start=start, k_scale=scales, v_scale=scales), **bad}
         with pytest.raises(ValueError, match="a plan of 32 rows in 2 segments"):
             ops.attn_segments_paged(**args)
+
+
+def test_a_plan_of_fewer_rows_than_there_are_is_refused():
+    """The rows behind the plan's would be nobody's: their results were left as the memory had them."""
+    plan, short = ops.kv4_plan([(40, 20), (0, 12)], 8, 2, "cpu")
+    cache = torch.zeros(4, 2, 16, 64, dtype=torch.uint8)
+    scales, tables, start = torch.zeros(4, 2, 16, 2, 2, dtype=torch.bfloat16), torch.zeros(2, 4, dtype=torch.int32), torch.zeros(2, dtype=torch.int32)
+    call = lambda rows, plan, short: ops.attn_segments_paged(torch.zeros(rows, 8, 128, dtype=torch.bfloat16), cache, cache, torch.zeros(rows, 4, dtype=torch.int32),
+                                                             torch.zeros(rows, dtype=torch.int32), 0.1, plan, short, tables, start, scales, scales)
+    with pytest.raises(ValueError, match="a plan of 32 rows in 2 segments"):
+        call(33, plan, short)
+    for rows, short in ((33, [(0, 32)]), (5, [(0, 2), (2, 2)]), (1, [])):
+        with pytest.raises(ValueError, match="row by row"):
+            call(rows, None, short)
