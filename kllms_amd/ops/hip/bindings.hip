@@ -213,8 +213,12 @@ void attn_prefill4(torch::Tensor out, torch::Tensor q, torch::Tensor k_cache, to
     TORCH_CHECK(t.scalar_type() == at::kInt && t.is_contiguous() && t.device() == q.device(), "attn_segments_paged: plan, tables or positions");
   TORCH_CHECK(items.dim() == 2 && items.size(1) == 8 && cuts.dim() == 2 && cuts.size(1) == 4 && tables.dim() == 2 &&
                   pos.numel() == tables.size(0) && parts >= 0 && items.size(0) < (1LL << 31), "attn_segments_paged: plan, tables or positions");
-  if (items.size(0) == 0 || q.size(0) == 0 || k_cache.numel() == 0 || tables.size(1) == 0) return;
+  if (items.size(0) == 0 || q.size(0) == 0) return;
   const c10::DeviceGuard device(q.device());
+  if (k_cache.numel() == 0 || tables.size(1) == 0) {     // no row sees a key
+    out.zero_();
+    return;
+  }
   if (!rows_aligned(q)) q = q.clone(at::MemoryFormat::Contiguous);
   auto room = torch::empty({parts * KVH * attn_prefill4_part()}, q.options().dtype(torch::kFloat));
   TORCH_CHECK(launch_attn_prefill4(bf(out), room.data_ptr<float>(), cbf(q), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(),

@@ -555,3 +555,17 @@ def test_segments_at_other_starts_than_the_plans(planned):
     plan = ops.kv4_plan(planned, 8, 2, DEV)
     out = attend(q, kc, vc, ks, vs, seg_tables, start, tables, lens, 0.1, segs, plan)
     check_prompts(out, q, kc, vc, ks, vs, tables, lens, 0.1)
+
+
+def test_segments_of_tables_without_blocks_are_zeros():
+    segs = [(0, 40), (0, 12)]
+    q, kc, vc, ks, vs, seg_tables, start, tables, lens = segments(segs, 4, 2, 16, seed=76)
+    plan = ops.kv4_plan(segs, 8, 2, DEV)
+    for cut in (dict(tables=slice(0, 0)), dict(blocks=0)):
+        full = torch.full(q.shape, 7.0, dtype=torch.bfloat16, device=DEV)      # its memory is the next result's
+        del full
+        if "tables" in cut:
+            out = attend(q, kc, vc, ks, vs, seg_tables[:, :0].contiguous(), start, tables[:, :0].contiguous(), lens * 0, 0.1, segs, plan)
+        else:
+            out = attend(q, kc[:0], vc[:0], ks[:0], vs[:0], seg_tables * 0, start, tables * 0, lens * 0, 0.1, segs, plan)
+        assert not bool(out.any())
