@@ -282,6 +282,7 @@ void rope_store(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor
                   slots.scalar_type() == at::kLong && slots.is_contiguous() && slots.numel() == T &&
                   cos_sin.scalar_type() == at::kFloat && cos_sin.is_contiguous() && cos_sin.size(-1) == 128,
               "rope_store: positions, slots or angles");
+  for (const auto& t : {k, v, k_cache, v_cache, positions, slots, cos_sin}) TORCH_CHECK(t.device() == q.device(), "rope_store: one device");
   const int kind = cache_kind(k_cache);
   if (kind == CACHE_KV4) check_kv4(k_cache, v_cache, k_scale, v_scale, k, "rope_store");
   if (kind == CACHE_FP8)
@@ -290,6 +291,7 @@ void rope_store(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor
                     v_scale.is_contiguous() && v_scale.scalar_type() == at::kFloat,
                 "fp8 rope_store requires [NB, KVH, BS] fp32 k_scale/v_scale");
   if (T == 0) return;
+  const c10::DeviceGuard device(q.device());
   launch_rope_store(bf(q), bf(k), cbf(v), positions.data_ptr<int64_t>(), cos_sin.data_ptr<float>(), k_cache.data_ptr(),
                     v_cache.data_ptr(), kind ? k_scale.data_ptr() : nullptr,
                     kind ? v_scale.data_ptr() : nullptr, slots.data_ptr<int64_t>(), T, H, G, (int)q.stride(0),
@@ -875,6 +877,8 @@ static void add_norm_rows_into(void* out, float* scales, torch::Tensor part, tor
   const int S = part.size(0), M = part.size(1), n = part.size(2);
   TORCH_CHECK(residual.dim() == 2 && residual.size(0) == M && residual.size(1) == n && weight.numel() == n &&
                   n % 4 == 0 && n <= 16384 && S >= 1 && M >= 1, "add_norm_rows: sizes");
+  TORCH_CHECK(residual.device() == part.device() && weight.device() == part.device(), "add_norm_rows: one device");
+  const c10::DeviceGuard device(part.device());
   launch_add_norm_rows((bf16_t*)out, bf(residual), part.data_ptr<float>(), nullptr, nullptr, cbf(weight), S, M, n, 0,
                        (float)eps, nullptr, nullptr, 0, scales, cur_stream());
 }
@@ -928,7 +932,9 @@ torch::Tensor rope_store_rows(torch::Tensor part, torch::Tensor bias, int64_t H,
                   slots.scalar_type() == at::kLong && slots.is_contiguous() && slots.numel() == M &&
                   cos_sin.scalar_type() == at::kFloat && cos_sin.is_contiguous() && cos_sin.size(-1) == 128,
               "rope_store_rows: positions, slots or angles");
-  TORCH_CHECK(bias.numel() == 0 || (bias.scalar_type() == at::kBFloat16 && bias.is_contiguous() &&
+  for (const auto& t : {k_cache, v_cache, positions, slots, cos_sin})
+    TORCH_CHECK(t.device() == part.device(), "rope_store_rows: one device");
+  TORCH_CHECK(bias.numel() == 0 || (bias.scalar_type() == at::kBFloat16 && bias.is_contiguous() && bias.device() == part.device() &&
                                     bias.numel() == part.size(2)), "rope_store_rows: bias");
   const int kind = cache_kind(k_cache);
   if (kind == CACHE_KV4) check_kv4(k_cache, v_cache, k_scale, v_scale, part, "rope_store_rows");
@@ -937,6 +943,7 @@ torch::Tensor rope_store_rows(torch::Tensor part, torch::Tensor bias, int64_t H,
                     k_scale.scalar_type() == at::kFloat && v_scale.numel() == k_scale.numel() &&
                     v_scale.is_contiguous() && v_scale.scalar_type() == at::kFloat,
                 "fp8 rope_store_rows requires [NB, KVH, BS] fp32 k_scale/v_scale");
+  const c10::DeviceGuard device(part.device());
   auto q = torch::empty({M, H, 128}, part.options().dtype(torch::kBFloat16));
   launch_rope_store_rows(bf(q), part.data_ptr<float>(), bias.numel() ? cbf(bias) : nullptr,
                          positions.data_ptr<int64_t>(), cos_sin.data_ptr<float>(), k_cache.data_ptr(),

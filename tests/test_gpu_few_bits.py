@@ -86,3 +86,46 @@ def test_int8_weights_hold_half_the_bytes():
     assert at.qkv_proj.weight.dtype == torch.int8 and at.qkv_proj.weight.is_cuda
     codes, scales = torch_ref.quantize_weights(at.qkv_proj.weight.float().cpu() * at.qkv_proj.weight_scale.cpu()[:, None])
     assert torch.equal(codes, at.qkv_proj.weight.cpu())
+
+
+def step_operands(device, G=2, M=3, H=4):
+    g = torch.Generator().manual_seed(3)
+    sizes = dict(part=torch.randn(2, M, (H + 2 * G) * 128, generator=g), bias=torch.randn((H + 2 * G) * 128, generator=g).bfloat16(), num_heads=H,
+                 positions=torch.arange(M), cos_sin=torch_ref.build_cos_sin_cache(128, 64, 1e4, "cpu"), k_cache=torch.zeros(2, G, 16, 64, dtype=torch.uint8),
+                 v_cache=torch.zeros(2, G, 16, 64, dtype=torch.uint8), slot_mapping=torch.arange(M), k_scale=torch.zeros(2, G, 16, 2, 2).bfloat16(),
+                 v_scale=torch.zeros(2, G, 16, 2, 2).bfloat16())
+    return {k: t.to(device) if isinstance(t, torch.Tensor) else t for k, t in sizes.items()}
+
+
+def test_operands_on_another_device_are_refused():
+    args = step_operands("cuda:0")
+    ops.rope_store_rows(**args)
+    for name, t in args.items():
+        if isinstance(t, torch.Tensor):
+            with pytest.raises(RuntimeError):
+                ops.rope_store_rows(**{**args, name: t.cpu()})
+    rows = torch.randn(3, 8, 128, device="cuda:0").bfloat16()
+    q, k, v = rows.split([4, 2, 2], 1)
+    more = [args[n] for n in ("positions", "cos_sin", "k_cache", "v_cache", "slot_mapping", "k_scale", "v_scale")]
+    ops.rope_store(q, k, v, *more)
+    for i in range(len(more)):
+        with pytest.raises(RuntimeError):
+            ops.rope_store(q, k, v, *more[:i], more[i].cpu(), *more[i + 1:])
+    part, residual, weight = torch.zeros(2, 3, 256), torch.zeros(3, 256).bfloat16(), torch.ones(256).bfloat16()
+    for away in range(3):
+        with pytest.raises(RuntimeError):
+            ops.add_norm_rows_int8(*(t if i == away else t.cuda() for i, t in enumerate((part, residual, weight))), 1e-5)
+
+
+@pytest.mark.skipif(torch.cuda.device_count() < 2, reason="needs two GPUs")
+def test_a_steps_operators_on_a_device_that_is_not_the_current_one():
+    def step(device):
+        args = step_operands(device)
+        q = ops.rope_store_rows(**args)
+        residual = torch.ones(3, 1024, device=device).bfloat16()
+        codes, scales = ops.add_norm_rows_int8(args["part"].contiguous(), residual, residual[0].contiguous(), 1e-5)
+        torch.cuda.synchronize(device)
+        return [t.cpu() for t in (q, args["k_cache"], args["v_scale"], residual, codes, scales)]
+
+    with torch.cuda.device(0):
+        assert all(torch.equal(a, b) for a, b in zip(step("cuda:0"), step("cuda:1")))
