@@ -559,15 +559,19 @@ class Int8Rows(NamedTuple):
     scales: torch.Tensor
 
 
-def _check_int8(x, w: torch.Tensor) -> None:
+def _no_gradient(*operands) -> None:
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in operands):
+        raise RuntimeError("products in 8-bit integers have no gradient: call them under torch.no_grad()")
+
+
+def _check_int8(x, w: torch.Tensor, w_scale: torch.Tensor, bias: Optional[torch.Tensor] = None) -> None:
+    _no_gradient(*(x if isinstance(x, Int8Rows) else (x,)), w_scale, bias)
     if isinstance(x, Int8Rows):
         x, scales = x
         if x.dtype != torch.int8 or scales.dtype != torch.float32 or scales.shape != x.shape[:1]:
             raise ValueError(f"rows as int8 codes with an fp32 scale each: got {x.dtype} {list(x.shape)}, {scales.dtype} {list(scales.shape)}")
     if w.dtype != torch.int8 or w.dim() != 2 or x.dim() != 2 or x.shape[1] != w.shape[1]:
         raise ValueError(f"x [M, K] with int8 weights [N, K]: got {list(x.shape)} with {w.dtype} {list(w.shape)}")
-    if x.requires_grad and torch.is_grad_enabled():
-        raise RuntimeError("products in 8-bit integers have no gradient: call them under torch.no_grad()")
 
 
 def _product_int8(x, w, w_scale, bias, form: int, once: bool) -> torch.Tensor:
@@ -588,13 +592,16 @@ def quantize_rows(x: torch.Tensor) -> Int8Rows:
     several products read; one product quantizes its rows itself."""
     if x.dim() != 2:
         raise ValueError(f"rows [M, K]: got {list(x.shape)}")
+    _no_gradient(x)
     if x.is_cuda and not _force_torch():
         return Int8Rows(*_hip_or_raise().quantize_rows(x))
     return Int8Rows(*torch_ref.quantize_rows(x))
 
 
+@torch.no_grad()
 def quantize_weights(w: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
-    """(int8 [N, K], scales fp32 [N]) of a weight matrix [N, K] of any float type, for linear_int8."""
+    """(int8 [N, K], scales fp32 [N]) of a weight matrix [N, K] of any float type, for linear_int8. They are constants: a
+    gradient does not go through them."""
     if w.dim() != 2:
         raise ValueError(f"weights [N, K]: got {list(w.shape)}")
     parts = [torch_ref.quantize_weights(p) for p in w.split(4096)]       # their fp32 copies are not all there at once
@@ -605,8 +612,9 @@ def linear_int8(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, bias: O
                 once: bool = False) -> torch.Tensor:
     """x @ w^T (+ bias) in 8-bit integers, in x's dtype: x [M, K] quantized row by row (quantize_rows), or Int8Rows; w int8
     [N, K] with a scale for each row (quantize_weights), exact 32-bit sums. On the GPU x is bf16, K a multiple of 16 up to
-    131072, N one of 16. ``once``: weights_once of the caller's model."""
-    _check_int8(x, w)
+    131072, N one of 16. ``once``: weights_once of the caller's model. Operands that want a gradient are refused, here
+    and in the other products of 8-bit integers."""
+    _check_int8(x, w, w_scale, bias)
     if (x.codes if isinstance(x, Int8Rows) else x).is_cuda and not _force_torch():
         return _product_int8(x, w, w_scale, bias, 0, once)
     return torch_ref.linear_int8(x, w, w_scale, bias)
@@ -614,7 +622,7 @@ def linear_int8(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, bias: O
 
 def linear_silu_int8(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, once: bool = False) -> torch.Tensor:
     """silu(gate) * up of linear_int8 with a fused [gate; up] matrix (N a multiple of 32 on the GPU)."""
-    _check_int8(x, w)
+    _check_int8(x, w, w_scale)
     if w.shape[0] % 2:
         raise ValueError("gate and up have the same rows")
     if (x.codes if isinstance(x, Int8Rows) else x).is_cuda and not _force_torch():
@@ -624,6 +632,7 @@ def linear_silu_int8(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, on
 
 def linear_part_int8(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, once: bool = False) -> torch.Tensor:
     """linear_int8 of up to LINEAR_ROWS_MAX rows as fp32 sums [S, M, N] over S shares of K, like linear_part (GPU only)."""
+    _no_gradient(*(x if isinstance(x, Int8Rows) else (x,)), w_scale)
     return _product_int8(x, w, w_scale, None, 2, once)
 
 
@@ -641,6 +650,7 @@ def add_norm_rows(part, residual, weight, eps):
 
 def add_norm_rows_int8(part, residual, weight, eps) -> Int8Rows:
     """quantize_rows(add_norm_rows(...)) in one launch, for rows of a multiple of 128 (GPU only)."""
+    _no_gradient(part, residual, weight)
     return Int8Rows(*_hip_or_raise().add_norm_rows_int8(part, residual, weight, eps))
 
 

@@ -120,3 +120,26 @@ def test_rows_that_are_codes_already():
     for bad in (ops.Int8Rows(x, c.scales), ops.Int8Rows(c.codes, c.scales.double()), ops.Int8Rows(c.codes, c.scales[:2])):
         with pytest.raises(ValueError):
             ops.linear_int8(bad, w, ws)
+
+
+def test_operands_that_want_a_gradient_are_refused():
+    g = torch.Generator().manual_seed(9)
+    x, b = torch.randn(3, 16, generator=g).bfloat16(), torch.randn(32, generator=g).bfloat16()
+    w, ws = ops.quantize_weights(torch.randn(32, 16, generator=g))
+    want = lambda t: t.clone().requires_grad_()
+    codes, scales = ops.quantize_rows(x)
+    calls = [lambda: ops.linear_int8(want(x), w, ws), lambda: ops.linear_int8(x, w, want(ws)), lambda: ops.linear_int8(x, w, ws, want(b)),
+             lambda: ops.linear_int8(ops.Int8Rows(codes, want(scales)), w, ws), lambda: ops.linear_silu_int8(want(x), w, ws),
+             lambda: ops.linear_silu_int8(x, w, want(ws)), lambda: ops.linear_silu_int8(ops.Int8Rows(codes, want(scales)), w, ws),
+             lambda: ops.quantize_rows(want(x)), lambda: ops.linear_part_int8(want(x), w, ws), lambda: ops.linear_part_int8(x, w, want(ws)),
+             lambda: ops.add_norm_rows_int8(x.float()[None], x, want(x[0]), 1e-5)]
+    for call in calls:
+        with pytest.raises(RuntimeError, match="no gradient"):
+            call()
+    with torch.no_grad():
+        assert torch.equal(ops.linear_int8(want(x), w, want(ws), want(b)), ops.linear_int8(x, w, ws, b))
+    # weights that a model trains, held in 8 bits: constants
+    held = torch.nn.Parameter(torch.randn(32, 16, generator=g))
+    codes, scales = ops.quantize_weights(held)
+    assert not scales.requires_grad and torch.equal(scales, ops.quantize_weights(held.detach())[1])
+    assert not ops.linear_int8(x, codes, scales).requires_grad
