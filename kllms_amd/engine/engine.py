@@ -126,6 +126,15 @@ class _DecodeBatchState:
         self.bt[rows, cols] = vals
 
 
+def _check_few_bits(config: EngineConfig, device: torch.device, dtype: torch.dtype) -> None:
+    """Refuses, before a model is built, what the kernels of few bits would at the first step."""
+    if device.type != "cuda" or dtype == torch.bfloat16 or ops._force_torch():
+        return
+    for name, value, few in (("weight_dtype", config.weight_dtype, "int8"), ("kv_cache_dtype", config.kv_cache_dtype, "int4")):
+        if value == few:
+            raise ValueError(f"{name}={few!r} needs dtype='bfloat16' on the GPU: got {config.dtype!r}")
+
+
 class LLMEngine:
     def __init__(self, config: EngineConfig, parallel_ctx=None):
         from ..parallel.tp import ParallelContext
@@ -168,6 +177,7 @@ class LLMEngine:
         # CPU bf16 matmuls are slow and torch CPU attention paths prefer f32
         if self.device.type == "cpu" and self.dtype == torch.bfloat16:
             self.dtype = torch.float32
+        _check_few_bits(config, self.device, self.dtype)
 
         # the RoPE cos/sin table (and thus every position) is bounded by the
         # architecture's max_position_embeddings

@@ -143,3 +143,17 @@ def test_operands_that_want_a_gradient_are_refused():
     codes, scales = ops.quantize_weights(held)
     assert not scales.requires_grad and torch.equal(scales, ops.quantize_weights(held.detach())[1])
     assert not ops.linear_int8(x, codes, scales).requires_grad
+
+
+@pytest.mark.parametrize("few", [dict(weight_dtype="int8"), dict(kv_cache_dtype="int4")])
+@pytest.mark.parametrize("dtype", ["float32", "float16"])
+def test_other_types_on_the_gpu_are_refused_before_a_model_is_built(few, dtype, monkeypatch):
+    from kllms_amd.engine.config import EngineConfig
+    from kllms_amd.engine.engine import LLMEngine
+
+    monkeypatch.setattr(LLMEngine, "_build_model", lambda self: pytest.fail("a model is built"))
+    config = lambda **o: EngineConfig(model="mid-llama", device="cuda:0", dtype=dtype, **o)
+    with pytest.raises(ValueError, match="needs dtype='bfloat16' on the GPU"):
+        LLMEngine(config(**few))
+    with pytest.raises(pytest.fail.Exception, match="a model is built"):
+        LLMEngine(config())
