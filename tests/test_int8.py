@@ -157,3 +157,22 @@ def test_other_types_on_the_gpu_are_refused_before_a_model_is_built(few, dtype, 
         LLMEngine(config(**few))
     with pytest.raises(pytest.fail.Exception, match="a model is built"):
         LLMEngine(config())
+
+
+def test_engine_generates_with_biases():
+    """Products with a bias (qkv), and what they give, through the engine."""
+    from kllms_amd.engine.engine import GenRequest
+    from kllms_amd.engine.sampling import SamplingParams
+
+    eng = engine(model="tiny-qwen", kv_cache_dtype="int4")
+    p = eng.model.layers[0].self_attn.qkv_proj
+    assert p.weight.dtype == torch.int8 and p.bias is not None
+    request = GenRequest(prompt_ids=list(range(1, 30)), n=2, sampling=SamplingParams(temperature=0.0, max_new_tokens=6))
+    out = eng.generate([request])[0]
+    assert out.streams[0].token_ids == out.streams[1].token_ids and len(out.streams[0].token_ids) >= 1
+    x = torch.randn(5, p.weight.shape[1])
+    p.bias.data.copy_(torch.randn(p.bias.shape))
+    plain = (x.double() @ (p.weight.double() * p.weight_scale.double()[:, None]).t() + p.bias.double())
+    # x is off by half of max / 127 in each place at most
+    err = 0.5 / 127 * x.abs().amax(1, keepdim=True).double() * (p.weight.double() * p.weight_scale.double()[:, None]).abs().sum(1)
+    assert bool(((p(x).double() - plain).abs() <= err * 1.001 + 1e-4).all())
