@@ -129,3 +129,49 @@ def test_a_steps_operators_on_a_device_that_is_not_the_current_one():
 
     with torch.cuda.device(0):
         assert all(torch.equal(a, b) for a, b in zip(step("cuda:0"), step("cuda:1")))
+
+
+def test_tails_behind_a_cached_prefix_attend_to_what_the_cache_holds(monkeypatch):
+    """Each layer's attention of tails that share a cached head against 64 bits over the cache's values, for rows of each tail
+    (positions and blocks of rows, where the kernel has those of segments); and the model's rows against the same passes row by row."""
+    from kv4_oracle import prompts64
+
+    head = list(range(5, 5 + 160))
+    g = torch.Generator().manual_seed(2)
+    sizes = (1, 33, 90, 400)
+    tails = [GenRequest(prompt_ids=head + torch.randint(1, 400, (k,), generator=g).tolist(), n=2,
+                        sampling=SamplingParams(temperature=0.0, max_new_tokens=5)) for k in sizes]
+    first = [GenRequest(prompt_ids=head + [7] * 40, n=1, sampling=SamplingParams(temperature=0.0, max_new_tokens=4))]
+    together, plan_of = ops.attn_segments_paged, ops.paged_plan
+    seen = []
+
+    def watched(q, k, v, tables, lens, scale, plan, short, seg_tables, seg_start, ks=None, vs=None):
+        out = together(q, k, v, tables, lens, scale, plan, short, seg_tables, seg_start, ks, vs)
+        ends = torch.tensor([r for r in range(len(lens)) if r + 1 == len(lens) or int(lens[r + 1]) != int(lens[r]) + 1])
+        starts = torch.cat((torch.zeros(1, dtype=torch.long), ends[:-1] + 1))
+        some = torch.cat((starts, (starts + ends) // 2, ends)).unique()
+        want, off = prompts64(*(t.cpu() for t in (q[some], k, v, ks, vs, tables[some], lens[some])), scale)
+        assert bool(((out[some].double().cpu() - want).abs() <= off).all())
+        seen.append((plan is not None, (lens[starts] - 1).tolist(), (ends - starts + 1).tolist()))
+        return out
+
+    runs = []
+    for rows_alone in (False, True):
+        eng = engine(kv_cache_dtype="int4", weight_dtype="int8", prefix_cache_min_tokens=32, max_seq_len=1024)
+        eng.generate(first)
+        hidden, forward = [], eng.model.forward_hidden
+        with monkeypatch.context() as m:
+            m.setattr(eng.model, "forward_hidden", lambda *a: hidden.append(forward(*a)) or hidden[-1])
+            if rows_alone:
+                m.setattr(ops, "paged_plan", lambda segs, *a: (None, [(0, sum(n for _, n in segs))]))
+            else:
+                m.setattr(ops, "attn_segments_paged", watched)
+            saved = eng.prefix_cache.tokens_saved
+            outs = eng.generate(tails)
+        assert eng.prefix_cache.tokens_saved - saved == 160 * len(tails)
+        assert all(len(s.token_ids) > 0 for o in outs for s in o.streams)
+        runs.append(hidden[0].float())
+    assert seen == [(True, [160] * 4, list(sizes))] * eng.kv.num_layers
+    assert ops.paged_plan is plan_of and runs[0].shape == runs[1].shape == (sum(sizes), eng.arch.hidden_size)
+    # a bf16 rounding that falls differently moves a row's codes by one of 127 steps here and there
+    assert float((runs[0] - runs[1]).norm()) < 0.03 * float(runs[1].norm())
