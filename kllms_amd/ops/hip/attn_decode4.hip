@@ -8,8 +8,8 @@
 // vector instructions for the eight values of a word, where a value at a time takes two each and a product. A nibble masked out of its
 // half of a word is an fp16 number as it stands, n * 2^-24 (below the normal ones, which the matrix cores take as they
 // are), or 16 times that, which the other operand or the end makes good. q and p s are fp16 too: q's 8 bits are exact
-// once its largest is scaled into fp16's range, p s is rounded to 11 bits, which is 2^-12 of each and
-// a quarter of what the result's own rounding leaves when it is summed over keys.
+// once its largest is scaled into fp16's range, p s is rounded to 11 bits, at most 2^-11 of each, an eighth of
+// the result's own rounding. Measured against 64 bits, normal values: 0.0018 where that rounding alone leaves 0.0016.
 //
 // A wave takes 64 keys at a time and keeps its own running max and sum; four waves to a workgroup, Z workgroups to a context
 // (deal, attn_decode4_slots), merged by the last of them to arrive or by a second launch where the caller has no counters.
@@ -26,9 +26,10 @@
 // unit was the bound: 16 streams of 6100 33 us, one of 131071 with eight heads to a kv head 48.) A row's 16-byte units are
 // XORed with its key: both kinds of reads are free of bank conflicts. Key 4 r + c of 16 is row 4 c + r of a score tile.
 //
-// What bounds it: the cache's bytes where contexts are many or long, else the chain of loads of one tile. Measured, us: one
-// context of 150, 16 / 4 heads 6.3; 120 of 520 to 577 of which five each share 512, 32 / 8 heads 17.7 (76 MB read by the rows, 21 of them
-// different); 16 of 4500 to 7777 30.0 (113 MB); one of 131071, 64 / 8 heads 32.7 (151 MB, 4.6 TB/s: a large copy's rate).
+// What bounds it: the cache's bytes where contexts are long, the vector units (58 % of their time, the waves waiting for
+// 39 % of theirs) where they are many, else the chain of loads of one tile. Measured, us: one
+// context of 150, 16 / 4 heads 6.3; 120 of 520 to 577 of which five each share 512, 32 / 8 heads 18.0 (83 MB from the L2s, 27 from behind
+// them); 16 of 4500 to 7777 30.5 (120 MB, 4.5 TB/s, and a launch that joins shares); one of 131071, 64 / 8 heads 32.9 (151 MB, 5.2 TB/s, and that launch).
 
 #include <algorithm>
 

@@ -10,16 +10,20 @@
 //     brings it there: none, in a model, and then nothing is multiplied back. Each group has its own: with one for both of a row, values 2^-20
 //     of the other group's were up to 16 % off. q's rows are scaled into fp16's range exactly
 //   - scores and softmax as in attn_prefill.hip: S = K Q^T, a lane has one row's scores, base-2 exponentials of one fma, the
-//     running max renewed when it grows by more than 8; P is fp16 in one part, 2^-12 of it, where bf16 would need two
+//     running max renewed when it grows by more than 8; P is fp16 in one part, 2^-11 of it, where bf16 would need two. Below 2^-14 of
+//     the running max it is off by 2^-25 of that, as much as a sum in fp32 loses of it
 //   - few or long groups are cut along the keys (the plan says where); their sums meet in a second launch
 //
 // A nibble becomes fp16 in three half instructions of two each: masked into 1024 + n, less 1024, times step plus least
 // value, which is rounded once.
 //
 // What bounds it: the vector units, with the softmax's exponentials before all; making the keys is a sixth of their work. The two
-// waves of a SIMD do not cover one's products by the other's exponentials for long: they meet at each stage's barrier; that one half of
-// them loads before its products and the other half after them gave 4 %. Measured, 32 / 8 heads, us: 2100 rows behind 7777 341 (780
-// TFLOP/s), eight segments of 150 behind 1536 66, 146 rows behind 1536 25, 300 behind 100000 553.
+// waves of a SIMD do not cover one's products by the other's exponentials for long: they meet at each stage's barrier (vector
+// instructions 59 % of a SIMD's time, matrix instructions 39 %, so hardly at once); that one half of
+// them loads before its products and the other half after them gave 4 %. Measured, 32 / 8 heads, us: 2100 rows behind 7777 339 (790
+// TFLOP/s), eight segments of 150 behind 1536 67, 146 rows behind 1536 26, 300 behind 100000 553. Against 64 bits, normal values, the
+// first is 0.0023 off, where the result's rounding alone leaves 0.0016 and codes multiplied as they are (attn_decode4.hip) 0.0018: keys and
+// values are rounded once more here.
 //
 // Fragment maps and ds_read_b64_tr_b16: attn_prefill.hip.
 

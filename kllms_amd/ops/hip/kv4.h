@@ -3,8 +3,8 @@
 // 64 neighbouring values are a group: its least value and its step, (most - least) / 15, are bf16 (of bf16 rows the least
 // value is one of them, so it is exact), and a value is the whole number of steps above the least one, to the nearest, halves to even:
 // at most half a step off, 0.09 of a group's standard deviation where that is normal. A group with a value that is no
-// finite number, or whose range is none, is NaN as a whole. The step's own rounding moves the far end of a group by 15 * 2^-9 of a
-// step.
+// finite number, or whose range is none, is NaN as a whole. The step's own rounding moves the far end of a group by up to 15 * 2^-8 of
+// a step.
 //
 // 16 words of 32 bits: nibble p of word n is value 32 (p mod 4) + 16 (p div 4) + n. So a lane that has words 4 c.. of a key has
 // the values of two 16x16x32 fragments of either group by a mask, and one that has word n of eight keys has column n of each

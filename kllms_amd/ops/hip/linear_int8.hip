@@ -15,8 +15,8 @@
 // product of few tiles is shared out over K: each workgroup leaves its sums past the L2 and the last one to arrive adds them up.
 // The counters for that are zeroed by the launch that makes the codes, which comes before anyway.
 //
-// Measured, us: 6144 x 4096, 5 rows 7.9 (25 MB, 3.2 TB/s); 28672 x 4096 with the activation, 120 rows 34 (W at 3.9 TB/s), 7777 rows 805
-// (2270 TOP/s, the card's power limit; the library's 8192^3 has 2083); 4608 x 3584 with bias, 333 rows 17.9.
+// Measured, us: 6144 x 4096, 5 rows 7.9 (25 MB, 3.2 TB/s); 28672 x 4096 with the activation, 120 rows 34 (W at 3.9 TB/s), 7777 rows 790
+// (2310 TOP/s, the card's power limit; the library's 8192^3 has 2083); 4608 x 3584 with bias, 333 rows 17.8.
 //
 // K is a multiple of 16; the codes' rows are filled up to whole stages with zeros, which what W has behind a row meets.
 
